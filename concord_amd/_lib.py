@@ -24,6 +24,10 @@ PROTO_CONSF = 1 << 9
 MUON = 1 << 10
 SALT_PREBUMPED = 1 << 16
 
+# element types of the entry points that take more than one
+F32, BF16, F16 = 0, 1, 2
+DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
 OK, EINVAL, ELAUNCH, EWORKSPACE = 0, -1, -2, -3
 
 # byte offset of the scratch region in the update-side workspace (after its
@@ -49,6 +53,18 @@ class DeviceScalars(ctypes.Structure):
                 ("chase_floor", ctypes.c_void_p), ("leak_floor", ctypes.c_void_p),
                 ("v_bc", ctypes.c_void_p), ("salt_counter", ctypes.c_void_p),
                 ("consolidate", ctypes.c_void_p)]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")] +
+                [(n, ctypes.c_int64) for n in ("q_t", "q_h", "k_t", "k_h", "v_t", "v_h")] +
+                [("out", ctypes.c_void_p), ("o_t", ctypes.c_int64), ("o_h", ctypes.c_int64)] +
+                [(n, ctypes.c_void_p) for n in ("lse", "starts", "k_starts")] +
+                [(n, ctypes.c_int64) for n in ("B", "TQ", "TK")] +
+                [(n, ctypes.c_int32) for n in ("H", "HK", "D", "causal")] + [("scale", ctypes.c_float)] +
+                [("dout", ctypes.c_void_p), ("do_t", ctypes.c_int64), ("do_h", ctypes.c_int64)] +
+                [(n, ctypes.c_void_p) for n in ("dq", "dk", "dv")] +
+                [(n, ctypes.c_int64) for n in ("dq_t", "dq_h", "dk_t", "dk_h", "dv_t", "dv_h")])
 
 
 # (name, restype, argtypes); P = pointer, I = int64, i = int32, F = float, D = double
@@ -122,6 +138,19 @@ _SIGS = {
     "concord_sigmag_noise": (ctypes.c_int, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _Z, _P]),
     "concord_watermark_peak": (ctypes.c_int, [_P, _I, _P, _I, _P, _P, _Z, _P]),
     "concord_coherence_sum": (ctypes.c_int, [_P, _I, _I, _I, _F, _P, _P, _Z, _P]),
+    "concord_layernorm_fwd": (ctypes.c_int, [_P, _I, ctypes.c_int, _P, _P, ctypes.c_int, _I, _I, _F, _P, _I, _P,
+                                             _P, _P]),
+    "concord_layernorm_workspace_bytes": (_Z, [_I, _I]),
+    "concord_layernorm_bwd": (ctypes.c_int, [_P, _I, _P, _I, ctypes.c_int, _P, ctypes.c_int, _P, _P, _I, _I, _P, _I,
+                                             _P, _P, _P, _Z, _P]),
+    "concord_distill_workspace_bytes": (_Z, [_I, _I]),
+    "concord_distill_fwd": (ctypes.c_int, [_P, _I, ctypes.c_int, _I, _I, _P, _I, _P, _I, _i, _F, _P, _P, _P, _Z,
+                                           _P]),
+    "concord_distill_bwd": (ctypes.c_int, [_P, _I, _P, _I, ctypes.c_int, _I, _I, _P, _I, _P, _I, _i, _F, _P, _P, _I,
+                                           _P]),
+    "concord_attention_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P]),
+    "concord_attention_workspace_bytes": (_Z, [ctypes.POINTER(AttnArgs)]),
+    "concord_attention_bwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P, _Z, _P]),
 }
 
 _lib = None
@@ -181,6 +210,15 @@ def stream_of(device):
         if d.index is not None:
             _CUDA_INDEX[device] = index
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def rows_of(t, rows, width):
+    """(t as [rows, width] with adjacent columns, its leading dimension): a
+    view, or a copy where the strides allow none."""
+    t = t.reshape(rows, width)
+    if width > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < width:
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else width)
 
 
 def require_device_tensor(t, name):

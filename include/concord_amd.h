@@ -48,6 +48,11 @@ extern "C" {
 #define CONCORD_MUON (1u << 10)         /* step = supplied drive (docs/MUON_IMPLEMENTATION.md:87-119) */
 #define CONCORD_SALT_PREBUMPED (1u << 16) /* the caller already advanced the salt counter */
 
+/* Element types of the entry points that take more than one. */
+#define CONCORD_F32 0
+#define CONCORD_BF16 1
+#define CONCORD_F16 2
+
 /* Launch-time scalars of the update (concord/packed_b.py:436-445). */
 typedef struct concord_update_params {
   float alpha, beta1, weight_decay, step_cap, v_scale, precond_p;
@@ -506,6 +511,83 @@ size_t concord_sigmag_noise_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int concord_sigmag_noise(uint16_t* grad_w, int64_t ld_g, const uint16_t* dy, int64_t ld_dy, const uint16_t* x,
                          int64_t ld_x, int64_t M, int64_t N, int64_t K, const float* sigma,
                          const int32_t* salt_counter, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Operators of a training step around the packed layers (no counterpart
+ * in the reference, which takes them from its framework) ---- */
+
+/* Layer norm of M rows of C elements: mean mu and r = 1 / sqrt(variance + eps)
+ * of each row, y = (x - mu) r weight + bias.  x and y are of type dtype, weight and
+ * bias [C] of type wdtype (either may be NULL: ones, zeros); statistics are
+ * fp32.  mean and rstd [M] (both or neither) are kept for the backward. */
+int concord_layernorm_fwd(const void* x, int64_t ld_x, int dtype, const void* weight, const void* bias,
+                          int wdtype, int64_t M, int64_t C, float eps, void* y, int64_t ld_y, float* mean,
+                          float* rstd, void* stream);
+/* Its gradients: dx of type dtype and, unless NULL, dweight and dbias [C] of
+ * type wdtype, summed over the rows in fp32 in a fixed order.  workspace:
+ * concord_layernorm_workspace_bytes(M, C) bytes, only where dweight or dbias
+ * is given; it need not be zeroed. */
+size_t concord_layernorm_workspace_bytes(int64_t M, int64_t C);
+int concord_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int dtype,
+                          const void* weight, int wdtype, const float* mean, const float* rstd, int64_t M,
+                          int64_t C, void* dx, int64_t ld_dx, void* dweight, void* dbias, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits, per row of V student logits (type
+ * dtype): with temperature T, q = softmax(logits / T) and p = softmax(teacher
+ * / T) over the row's K entries, loss = T^2 sum_k p_k (log p_k - log
+ * q[index_k]).  Entries whose index lies outside [0, V) are left out; a row
+ * without any has loss 0.  K <= 1024.  stats [M][2] (may be NULL) is kept for
+ * the backward.  workspace: concord_distill_workspace_bytes(M, V) bytes (0:
+ * none needed); it need not be zeroed. */
+size_t concord_distill_workspace_bytes(int64_t M, int64_t V);
+int concord_distill_fwd(const void* logits, int64_t ld_l, int dtype, int64_t M, int64_t V, const float* teacher,
+                        int64_t ld_t, const int64_t* index, int64_t ld_i, int32_t K, float temperature,
+                        float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+/* dlogits = dloss T (q - p), of type dtype; 0 for a row without an entry or
+ * with dloss 0.  Row r's upstream gradient is dloss[r * ld_dloss] (ld_dloss
+ * 0: one value for all). */
+int concord_distill_bwd(const float* dloss, int64_t ld_dloss, const void* logits, int64_t ld_l, int dtype,
+                        int64_t M, int64_t V, const float* teacher, int64_t ld_t, const int64_t* index,
+                        int64_t ld_i, int32_t K, float temperature, const float* stats, void* dlogits,
+                        int64_t ld_d, void* stream);
+
+/* Attention over whole sequences: out = softmax(scale q k^T) v, each query
+ * over the keys of its own sequence, bf16, H query heads that share HK key
+ * heads in groups of H / HK, head dimension D (a multiple of 8 up to 128).
+ * Element (token, head, d) of q lies at token * q_t + head * q_h + d (strides
+ * in elements, multiples of 8; 16-byte aligned), and likewise for the others.
+ *
+ * starts [B + 1] (int32, device): sequence b has tokens [starts[b],
+ * starts[b+1]) of q, and of k and v unless k_starts says otherwise.  starts
+ * NULL: B sequences of TQ / B queries and TK / B keys.  Tokens before the
+ * first and after the last sequence see no key.  causal: query i of a
+ * sequence with Lq queries and Lk keys sees keys j <= i + Lk - Lq.  A query
+ * that sees no key has out 0, and its gradients are 0.
+ *
+ * lse [H][TQ] fp32 (may be NULL): log2 of the sum over the row's keys of
+ * 2^(score log2 e), +inf for a row without a key; kept for the backward. */
+typedef struct concord_attn_args {
+  const uint16_t *q, *k, *v;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;
+  uint16_t* out;
+  int64_t o_t, o_h;
+  float* lse;
+  const int32_t *starts, *k_starts;
+  int64_t B, TQ, TK;
+  int32_t H, HK, D, causal;
+  float scale;
+  /* backward */
+  const uint16_t* dout;
+  int64_t do_t, do_h;
+  uint16_t *dq, *dk, *dv;
+  int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
+} concord_attn_args;
+int concord_attention_fwd(const concord_attn_args* args, void* stream);
+/* dq, dk, dv from dout, the forward's out and lse; dk and dv summed over the
+ * query heads of a group.  Every sum has a fixed order.  workspace:
+ * concord_attention_workspace_bytes(args) bytes; it need not be zeroed. */
+size_t concord_attention_workspace_bytes(const concord_attn_args* args);
+int concord_attention_bwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
