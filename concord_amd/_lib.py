@@ -4,12 +4,14 @@ The library is required: there is no fallback.  If it is missing the import of
 any compute entry point raises, with the command that builds it.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libconcord_amd.so")
+OPS_PATH = os.path.join(_HERE, "_lib", "concord_torch_ops.so")
 
 MASS_PRESERVE = 1 << 0
 APPLY_CHASE = 1 << 1
@@ -26,7 +28,6 @@ SALT_PREBUMPED = 1 << 16
 
 # element types of the entry points that take more than one
 F32, BF16, F16 = 0, 1, 2
-DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 OK, EINVAL, ELAUNCH, EWORKSPACE = 0, -1, -2, -3
 
@@ -59,7 +60,7 @@ class AttnArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")] +
                 [(n, ctypes.c_int64) for n in ("q_t", "q_h", "k_t", "k_h", "v_t", "v_h")] +
                 [("out", ctypes.c_void_p), ("o_t", ctypes.c_int64), ("o_h", ctypes.c_int64)] +
-                [(n, ctypes.c_void_p) for n in ("lse", "starts", "k_starts")] +
+                [(n, ctypes.c_void_p) for n in ("lse", "out_low", "starts", "k_starts")] +
                 [(n, ctypes.c_int64) for n in ("B", "TQ", "TK")] +
                 [(n, ctypes.c_int32) for n in ("H", "HK", "D", "causal")] + [("scale", ctypes.c_float)] +
                 [("dout", ctypes.c_void_p), ("do_t", ctypes.c_int64), ("do_h", ctypes.c_int64)] +
@@ -177,6 +178,24 @@ def lib():
     return _lib
 
 
+_ops = None
+
+
+def ops():
+    """The autograd nodes of csrc/torch_ops.cpp over the library's entries."""
+    global _ops
+    if _ops is None:
+        lib()   # (its absence has its own message)
+        if not os.path.exists(OPS_PATH):
+            raise ConcordError(
+                f"concord_amd: {OPS_PATH} is missing; build it with "
+                "`python -m concord_amd.build` (or __graft_entry__.build())")
+        spec = importlib.util.spec_from_file_location("concord_torch_ops", OPS_PATH)
+        _ops = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_ops)
+    return _ops
+
+
 def exported_symbols():
     return list(_SIGS)
 
@@ -210,15 +229,6 @@ def stream_of(device):
         if d.index is not None:
             _CUDA_INDEX[device] = index
     return torch._C._cuda_getCurrentRawStream(index)
-
-
-def rows_of(t, rows, width):
-    """(t as [rows, width] with adjacent columns, its leading dimension): a
-    view, or a copy where the strides allow none."""
-    t = t.reshape(rows, width)
-    if width > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < width:
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else width)
 
 
 def require_device_tensor(t, name):

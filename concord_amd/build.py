@@ -11,11 +11,15 @@ Per-file extras (FILE_FLAGS): gemm_fast.hip keeps MFMA accumulators in
 ordinary VGPRs (-amdgpu-mfma-vgpr-form); its kernels are written to fit them,
 and the accumulator-register form made the compiler copy accumulators
 around the main loops.
+
+torch_ops.cpp (host code: autograd nodes over the library's entries) becomes
+concord_amd/_lib/concord_torch_ops.so, against the installed torch.
 """
 import glob
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -23,8 +27,10 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libconcord_amd.so")
+OPS = os.path.join(OUT_DIR, "concord_torch_ops.so")
 ARCH = os.environ.get("CONCORD_OFFLOAD_ARCH", "gfx950")
 
+CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
@@ -46,26 +52,46 @@ def _run(cmd):
     return err
 
 
+def _ops_flags():
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "/opt/rocm/include", sysconfig.get_paths()["include"], os.path.join(ROOT, "include")]
+    cflags = ["-O2", "-std=c++17", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              "-DTORCH_EXTENSION_NAME=concord_torch_ops"] + [a for i in inc for a in ("-isystem", i)]
+    libs = ["-L" + os.path.join(root, "lib"), "-L" + OUT_DIR, "-lconcord_amd", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    return cflags, libs
+
+
 def build(verbose=False, jobs=8):
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     objs = [os.path.join(OUT_DIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
 
+    ops_src, ops_obj = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(OUT_DIR, "torch_ops.o")
+    ops_cflags, ops_libs = _ops_flags()
+
     def compile_one(so):
         s, o = so
+        if s.endswith(".cpp"):
+            return _run([CXX] + ops_cflags + ["-c", s, "-o", o])
         return _run([HIPCC] + CFLAGS + FILE_FLAGS.get(os.path.basename(s), []) + ["-c", s, "-o", o])
 
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        for msg in ex.map(compile_one, zip(srcs, objs)):
+        for msg in ex.map(compile_one, [(ops_src, ops_obj)] + list(zip(srcs, objs))):
             if verbose and msg.strip():
                 print(msg, file=sys.stderr)
     tmp = LIB + ".tmp"
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs)
     os.replace(tmp, LIB)
-    for o in objs:
+    _run([CXX, "-shared", "-o", OPS + ".tmp", ops_obj] + ops_libs)
+    os.replace(OPS + ".tmp", OPS)
+    for o in objs + [ops_obj]:
         os.remove(o)
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB} and {OPS}")
     return LIB
 
 

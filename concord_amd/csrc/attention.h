@@ -208,20 +208,54 @@ struct Fixed {
   }
 };
 
+// sum over the head dimension of the lane's row of out and of b, half of
+// it in each half wave: out is the row in bf16 and its left-over bytes
+template <class DIM>
+CONCORD_DEV float row_dot(const Fixed<DIM>& out, const int8_t* low, int left, int64_t low_ld, int D, const Fixed<DIM>& b,
+                          int lane) {
+  const int r = lane & 31, h = lane >> 5;
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < DIM::NK; ++k) {
+    const int c = (2 * k + h) * 8;
+    uint2 w = make_uint2(0, 0);
+    if (r < left && c < D) w = *(const uint2*)(low + (int64_t)r * low_ld + c);
+    const i32x4 hi = __builtin_bit_cast(i32x4, out.f[k]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = e & 1 ? (uint32_t)hi[e >> 1] & 0xFFFF0000u : (uint32_t)hi[e >> 1] << 16;
+      const int32_t byte = __builtin_amdgcn_sbfe((int32_t)(e < 4 ? w.x : w.y), 8 * (e & 3), 8);
+      s = __builtin_fmaf(__uint_as_float(bits + (uint32_t)(byte * 256)), (float)b.f[k][e], s);
+    }
+  }
+  const Halves both = halves(s);
+  return both.lo + both.hi;
+}
+
 // Store a transposed result block (rows: head dimension 32 d .., columns: the
 // tokens of p's rows) times the columns' factor, as bf16.  The half waves
-// exchange registers so that each lane stores 16 bytes of its token.
-CONCORD_DEV void store_block(uint16_t* p, int64_t ld, int left, int D, int d, const f32x16& v, float factor, int lane) {
+// exchange registers so that each lane stores 16 bytes of its token.  low, if
+// given, takes what the rounding left over (concord_attn_args.out_low).
+CONCORD_DEV int32_t left_over(float x, uint32_t bf16) {
+  const int32_t r = (int32_t)(__float_as_uint(x) - (bf16 << 16)) >> 8;   // -128 .. 128
+  return min(r, 127) & 255;
+}
+CONCORD_DEV void store_block(uint16_t* p, int64_t ld, int left, int D, int d, const f32x16& v, float factor, int lane,
+                             int8_t* low = nullptr, int64_t low_ld = 0) {
   const int r = lane & 31, h = lane >> 5;
   if (r >= left) return;
   uint16_t* q = p + (int64_t)r * ld;
 #pragma unroll
   for (int g = 0; g < 4; g += 2) {
-    uint32_t a[2], b[2];
+    uint32_t a[2], b[2], la = 0, lb = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      a[i] = pack_bf16x2(v[4 * g + 2 * i] * factor, v[4 * g + 2 * i + 1] * factor);
-      b[i] = pack_bf16x2(v[4 * g + 4 + 2 * i] * factor, v[4 * g + 5 + 2 * i] * factor);
+      const float x0 = v[4 * g + 2 * i] * factor, x1 = v[4 * g + 2 * i + 1] * factor;
+      const float y0 = v[4 * g + 4 + 2 * i] * factor, y1 = v[4 * g + 5 + 2 * i] * factor;
+      a[i] = pack_bf16x2(x0, x1);
+      b[i] = pack_bf16x2(y0, y1);
+      la |= (uint32_t)(left_over(x0, a[i] & 0xFFFF) | left_over(x1, a[i] >> 16) << 8) << (16 * i);
+      lb |= (uint32_t)(left_over(y0, b[i] & 0xFFFF) | left_over(y1, b[i] >> 16) << 8) << (16 * i);
       // lower half: its own and the upper half's part of group g; upper half:
       // both parts of group g + 1
       const auto s = __builtin_amdgcn_permlane32_swap(a[i], b[i], false, false);
@@ -230,6 +264,10 @@ CONCORD_DEV void store_block(uint16_t* p, int64_t ld, int left, int D, int d, co
     }
     const int c = 32 * d + 8 * (g + h);
     if (c < D) *(i32x4*)(q + c) = i32x4{(int32_t)a[0], (int32_t)a[1], (int32_t)b[0], (int32_t)b[1]};
+    if (low) {
+      const auto s = __builtin_amdgcn_permlane32_swap(la, lb, false, false);
+      if (c < D) *(uint2*)(low + (int64_t)r * low_ld + c) = make_uint2(s[0], s[1]);
+    }
   }
 }
 

@@ -18,8 +18,9 @@ struct AttnFwd {
   uint16_t* out;
   int64_t o_t, o_h;
   float* lse;
+  int8_t* low;
   AttnSeqs seq;
-  int32_t slots, rep, D, causal;   // rep: query heads of a key head
+  int32_t slots, rep, D, causal, heads;   // rep: query heads of a key head
   float c;                         // scale log2(e)
 };
 
@@ -133,8 +134,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   l = both.lo + both.hi;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = a.out + (p.q0 + row0) * a.o_t + (int64_t)head * a.o_h;
+  const int64_t low_t = (int64_t)a.heads * a.D;
+  int8_t* low = a.low ? a.low + (p.q0 + row0) * low_t + (int64_t)head * a.D : nullptr;
 #pragma unroll
-  for (int d = 0; d < ND; ++d) store_block(out, a.o_t, rows, a.D, d, o[d], inv, lane);
+  for (int d = 0; d < ND; ++d) store_block(out, a.o_t, rows, a.D, d, o[d], inv, lane, low, low_t);
   if (a.lse && lane < 32 && lane < rows)
     a.lse[(int64_t)head * a.seq.TQ + p.q0 + qi] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
@@ -147,9 +150,11 @@ extern "C" int concord_attention_fwd(const concord_attn_args* args, void* stream
   CONCORD_CHECK(args, "concord_attention_fwd: NULL argument");
   const concord_attn_args& g = *args;
   if (const int rc = attn_check("concord_attention_fwd", g)) return rc;
+  CONCORD_CHECK(!g.lse == !g.out_low && ((uintptr_t)g.out_low & 15) == 0,
+                "concord_attention_fwd: lse and out_low come together, out_low on 16 bytes");
   if (g.TQ == 0) return CONCORD_OK;
   AttnFwd a{};
-  a.q = g.q, a.k = g.k, a.v = g.v, a.out = g.out, a.lse = g.lse;
+  a.q = g.q, a.k = g.k, a.v = g.v, a.out = g.out, a.lse = g.lse, a.low = g.out_low, a.heads = g.H;
   a.q_t = g.q_t, a.q_h = g.q_h, a.k_t = g.k_t, a.k_h = g.k_h, a.v_t = g.v_t, a.v_h = g.v_h;
   a.o_t = g.o_t, a.o_h = g.o_h;
   a.seq = attn_seqs(g);

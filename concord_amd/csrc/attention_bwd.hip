@@ -18,9 +18,10 @@ struct AttnBwd {
   uint16_t *dq, *dk, *dv;
   int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
   const float* lse;
+  const int8_t* low;
   float* delta;
   AttnSeqs seq;
-  int32_t slots, rep, D, causal;
+  int32_t slots, rep, D, causal, heads;
   float c, scale;
 };
 
@@ -57,16 +58,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
   g.load(a.dout + (p.q0 + row0) * a.do_t + (int64_t)head * a.do_h, rows, a.do_t, a.D, lane);
   const int64_t at = (int64_t)head * a.seq.TQ + p.q0 + qi;
   const float lse = qi < p.lq ? a.lse[at] : INFINITY;
-  float delta = 0.0f;
+  float delta;
   {
     Fixed<DIM> o;
     o.load(a.out + (p.q0 + row0) * a.o_t + (int64_t)head * a.o_h, rows, a.o_t, a.D, lane);
-#pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)o.f[k][e], (float)g.f[k][e], delta);
-    const Halves both = halves(delta);
-    delta = both.lo + both.hi;
+    const int64_t low_t = (int64_t)a.heads * a.D;
+    delta = row_dot(o, a.low + (p.q0 + row0) * low_t + (int64_t)head * a.D, rows, low_t, a.D, g, lane);
     if (lane < 32 && qi < p.lq) a.delta[at] = delta;
   }
   const uint16_t* kp = a.k + p.k0 * a.k_t + (int64_t)hk * a.k_h;
@@ -277,7 +274,8 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
   CONCORD_CHECK(attn_operand(g.dout, g.do_t, g.do_h, g.TQ, g.D) && attn_operand(g.dq, g.dq_t, g.dq_h, g.TQ, g.D) &&
                     attn_operand(g.dk, g.dk_t, g.dk_h, g.TK, g.D) && attn_operand(g.dv, g.dv_t, g.dv_h, g.TK, g.D),
                 "%s: NULL, misaligned or badly strided gradient", what);
-  CONCORD_CHECK(g.lse || g.TQ == 0, "%s: lse is NULL", what);
+  CONCORD_CHECK((g.lse && g.out_low && ((uintptr_t)g.out_low & 15) == 0) || g.TQ == 0,
+                "%s: lse or out_low is NULL or misaligned", what);
   if (g.TQ == 0 && g.TK == 0) return CONCORD_OK;
   const size_t need = concord_attention_workspace_bytes(args);
   if (need && (!workspace || workspace_bytes < need)) {
@@ -289,7 +287,7 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
   a.q_t = g.q_t, a.q_h = g.q_h, a.k_t = g.k_t, a.k_h = g.k_h, a.v_t = g.v_t, a.v_h = g.v_h;
   a.o_t = g.o_t, a.o_h = g.o_h, a.do_t = g.do_t, a.do_h = g.do_h;
   a.dq_t = g.dq_t, a.dq_h = g.dq_h, a.dk_t = g.dk_t, a.dk_h = g.dk_h, a.dv_t = g.dv_t, a.dv_h = g.dv_h;
-  a.lse = g.lse, a.delta = (float*)workspace;
+  a.lse = g.lse, a.low = g.out_low, a.heads = g.H, a.delta = (float*)workspace;
   a.rep = g.H / g.HK, a.D = g.D, a.causal = g.causal != 0, a.c = g.scale * kLog2e, a.scale = g.scale;
   a.seq = attn_seqs(g);
   hipStream_t st = (hipStream_t)stream;

@@ -565,13 +565,17 @@ int concord_distill_bwd(const float* dloss, int64_t ld_dloss, const void* logits
  * that sees no key has out 0, and its gradients are 0.
  *
  * lse [H][TQ] fp32 (may be NULL): log2 of the sum over the row's keys of
- * 2^(score log2 e), +inf for a row without a key; kept for the backward. */
+ * 2^(score log2 e), +inf for a row without a key.  out_low [TQ][H][D] int8
+ * (given with lse, not without): what rounding out to bf16 left over, in
+ * units of 2^-8 of out's last place, so that the backward has out in 16
+ * significant bits.  Both are kept for the backward. */
 typedef struct concord_attn_args {
   const uint16_t *q, *k, *v;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;
   uint16_t* out;
   int64_t o_t, o_h;
   float* lse;
+  int8_t* out_low;
   const int32_t *starts, *k_starts;
   int64_t B, TQ, TK;
   int32_t H, HK, D, causal;
@@ -583,7 +587,7 @@ typedef struct concord_attn_args {
   int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
 } concord_attn_args;
 int concord_attention_fwd(const concord_attn_args* args, void* stream);
-/* dq, dk, dv from dout, the forward's out and lse; dk and dv summed over the
+/* dq, dk, dv from dout, the forward's out, lse and out_low; dk and dv summed over the
  * query heads of a group.  Every sum has a fixed order.  workspace:
  * concord_attention_workspace_bytes(args) bytes; it need not be zeroed. */
 size_t concord_attention_workspace_bytes(const concord_attn_args* args);
