@@ -117,74 +117,88 @@ struct Dim {
 // A tile of ROWS rows of a token-major operand (row: one token's head, up to
 // PITCH bytes) in LDS, loaded by DMA and read as an A operand in both
 // directions:
-//   rows(i, kk): 32 of its rows by 16 of the head dimension (row fragment)
-//   cols(t, d):  32 of the head dimension by 16 of its rows (transposed)
-// Chunk c (16 bytes) of row r lies in slot c ^ swz(r).  LDS has 64 banks: a
-// row fragment's 16-byte reads go 16 rows at a time, a transposed read's
-// 8-byte reads go 4 rows by 64 bytes at a time, and swz spreads both over all
-// banks (the 4 rows differ in the slot's upper two bits, or with 128-byte rows
-// in its upper bit and the row's parity; 16 rows take 16 slots).
+//   rows(i, k): 32 of its rows by 16 of the head dimension (row fragment)
+//   cols(t, d): 32 of the head dimension by 16 of its rows (transposed)
+// A DMA instruction fills a group of GROUP rows, 1 KB, in which the 16-byte
+// chunk c of row r lies in slot c ^ swz(r); PAD bytes follow each group.  LDS
+// has 64 banks.  A row fragment's 16-byte reads go in phases of 16 lanes, four
+// times four rows that start at rows 0, 12, 20, 24 (and 4, 8, 16, 28) of the
+// 32; a transposed read's 8-byte reads go 4 rows by 64 bytes at a time.  The
+// four rows differ in the slot's bits 2 and up (with 128-byte rows in bit 2
+// and the row's parity), the four groups of rows in its bits 0 and 1, by the
+// padding and swz: neither read has bank conflicts (a swizzle for 16 rows in a
+// row cost half as much again in LDS time with 128-byte rows).  swz leaves the
+// slot's bit 1 alone, so two depth steps share an address register (Frags).
 template <class DIM, int ROWS, int WAVES>
 struct Tile {
-  static constexpr int PITCH = DIM::PITCH, BYTES = ROWS * PITCH, SLOTS = PITCH / 16;
-  static constexpr int RPI = 1024 / PITCH, PER = ROWS / RPI / WAVES;   // rows of a DMA instruction; those of a wave
-  static_assert(PER * RPI * WAVES == ROWS, "rows split evenly over the waves");
-  static CONCORD_DEV int swz(int r) {
-    return PITCH == 256 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3);
-  }
-  uint32_t voff[PER];
+  static constexpr int PITCH = DIM::PITCH, GROUP = 1024 / PITCH, GBYTES = 1024 + (PITCH == 256 ? 16 : 32);
+  static constexpr int BYTES = ROWS / GROUP * GBYTES, SLOTS = PITCH / 16;
+  static constexpr int PER = ROWS / GROUP / WAVES;   // DMA instructions of a wave
+  static_assert(PER * GROUP * WAVES == ROWS, "rows split evenly over the waves");
+  static CONCORD_DEV int swz(int r) { return PITCH == 256 ? (r & 3) << 2 : ((r & 2) << 1) | ((r & 4) >> 2); }
+  // the address of row r (a multiple of GROUP) in the tile
+  static constexpr uint32_t at(int r) { return (uint32_t)(r / GROUP * GBYTES); }
+  uint32_t voff;
   uint32_t ld2, row_bytes;
   // ld: elements between rows; D: head dimension
-  CONCORD_DEV void init(int64_t ld, int D, int wave, int lane) {
+  CONCORD_DEV void init(int64_t ld, int D, int lane) {
     ld2 = (uint32_t)(ld * 2);
     row_bytes = (uint32_t)D * 2;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int r = (wave * PER + q) * RPI + lane / SLOTS, c = (lane % SLOTS) ^ swz(r);
-      voff[q] = c * 8 < D ? (uint32_t)r * ld2 + (uint32_t)c * 16 : kOOB;
-    }
+    const int r = lane / SLOTS, c = (lane % SLOTS) ^ swz(r);
+    voff = c * 8 < D ? (uint32_t)r * ld2 + (uint32_t)c * 16 : kOOB;
   }
   // rows [0, left) at p (the others read as zeros) into the tile at LDS address `lds`
   CONCORD_DEV void load(const uint16_t* p, int left, uint32_t lds, int wave) const {
-    const i32x4 rs = rows_rsrc(p, left < ROWS ? left : ROWS, ld2, row_bytes);
+    const int first = wave * PER * GROUP, n = left - first;
+    const i32x4 rs = rows_rsrc(p + (int64_t)first * (ld2 / 2), n < PER * GROUP ? n : PER * GROUP, ld2, row_bytes);
 #pragma unroll
     for (int q = 0; q < PER; ++q)
-      dma16(rs, voff[q], (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (uint32_t)((wave * PER + q) * 1024))));
+      dma16(rs, voff + (uint32_t)(q * GROUP) * ld2,
+            (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (uint32_t)((wave * PER + q) * GBYTES))));
   }
 };
 
-// a lane's addresses in a tile; the tile's place, blocks of rows and ring
-// slots are constants added to them (tiles are 256-byte aligned)
+// (an opaque value: the constants added to an address stay in the instructions'
+// offsets, where the compiler would otherwise keep a register for each sum)
+CONCORD_DEV void pin(uint32_t& v) { asm volatile("" : "+v"(v)); }
+
+// A lane's addresses in the tiles from LDS address `base` on; a tile's place,
+// blocks of rows and depth steps are constants added to them.
 template <class DIM>
 struct Frags {
-  static constexpr int PITCH = DIM::PITCH;
-  uint32_t row[DIM::NK];       // rows(): by depth step
-  uint32_t col[DIM::ND][2];    // cols(): by 32-wide block, lower and upper 8 rows of a step
-  CONCORD_DEV void init(int lane) {
-    typedef Tile<DIM, 64, 4> T;
+  typedef Tile<DIM, 64, 4> T;
+  static constexpr int NR = (DIM::NK + 1) / 2;
+  uint32_t row[NR];          // rows(): by pair of steps
+  uint32_t col[DIM::ND];     // cols(): by 32-wide block
+  CONCORD_DEV void init(uint32_t base, int lane) {
     const int r = lane & 31, h = lane >> 5;
-    const uint32_t r0 = (uint32_t)(r * PITCH + ((h ^ T::swz(r)) << 4));
+    const uint32_t r0 = base + T::at(r & ~(T::GROUP - 1)) + (uint32_t)((r & (T::GROUP - 1)) * DIM::PITCH);
 #pragma unroll
-    for (int k = 0; k < DIM::NK; ++k) row[k] = r0 ^ (uint32_t)(k << 5);
-    const int cr = 4 * h + ((lane >> 2) & 3);
-    const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const uint32_t c0 = (uint32_t)(cr * PITCH + ((chunk ^ T::swz(cr)) << 4) + ((lane & 1) << 3));
+    for (int j = 0; j < NR; ++j)
+      row[j] = r0 + (uint32_t)(((4 * j + h) ^ T::swz(r)) << 4), pin(row[j]);
+    const int cr = 4 * h + ((lane >> 2) & 3), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const uint32_t c0 = base + T::at(cr & ~(T::GROUP - 1)) + (uint32_t)((cr & (T::GROUP - 1)) * DIM::PITCH);
 #pragma unroll
     for (int d = 0; d < DIM::ND; ++d)
+      col[d] = c0 + (uint32_t)((((4 * d + chunk) ^ T::swz(cr)) << 4) + ((lane & 1) << 3)), pin(col[d]);
+  }
+  // to the tiles `bytes` further on
+  CONCORD_DEV void move(int32_t bytes) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) col[d][u] = c0 ^ (uint32_t)((d << 6) | (u << 5));
+    for (int j = 0; j < NR; ++j) row[j] += (uint32_t)bytes;
+#pragma unroll
+    for (int d = 0; d < DIM::ND; ++d) col[d] += (uint32_t)bytes;
   }
   // rows 32 i .. 32 i + 31, head dimension 16 k .. 16 k + 15
   CONCORD_DEV bf16x8 rows(uint32_t tile, int i, int k) const {
-    return __builtin_bit_cast(bf16x8, *(const lds_i32x4*)(lds_at(row[k]) + (tile + (uint32_t)(i * 32 * PITCH))));
+    const uint32_t o = tile + T::at(32 * i) + (uint32_t)((k & 1) * 32);
+    return __builtin_bit_cast(bf16x8, *(const lds_i32x4*)(lds_at(row[k >> 1]) + o));
   }
   // head dimension 32 d .. 32 d + 31, rows 16 t .. 16 t + 15 in the order of
   // a result's registers
   CONCORD_DEV bf16x8 cols(uint32_t tile, int d, int t) const {
-    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_i16x4*)(lds_at(col[d][0]) + (tile + (uint32_t)(t * 16 * PITCH))));
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_i16x4*)(lds_at(col[d][1]) + (tile + (uint32_t)((t * 16 + 8) * PITCH))));
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_at(col[d]) + tile + T::at(16 * t)));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_at(col[d]) + tile + T::at(16 * t + 8)));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };

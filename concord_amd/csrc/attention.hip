@@ -59,11 +59,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   const uint16_t* kp = a.k + p.k0 * a.k_t + (int64_t)hk * a.k_h;
   const uint16_t* vp = a.v + p.k0 * a.v_t + (int64_t)hk * a.v_h;
   T tk, tv;
-  tk.init(a.k_t, a.D, wave, lane);
-  tv.init(a.v_t, a.D, wave, lane);
-  Frags<DIM> fr;
-  fr.init(lane);
+  tk.init(a.k_t, a.D, lane);
+  tv.init(a.v_t, a.D, lane);
   const uint32_t base = lds_addr(lds);
+  Frags<DIM> fr;
+  fr.init(base, lane);
 
   f32x16 o[ND];
 #pragma unroll
@@ -75,15 +75,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
     tk.load(kp + (int64_t)t * kAttnK * a.k_t, p.lk - t * kAttnK, s, wave);
     tv.load(vp + (int64_t)t * kAttnK * a.v_t, p.lk - t * kAttnK, s + T::BYTES, wave);
   };
-  if (tiles > 0) load(0);
-  for (int t = 0; t < tiles; ++t) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's part of tile t has landed
-    lds_barrier();                              // everyone's has, and tile t - 1 has been read
-    if (t + 1 < tiles) load(t + 1);
-    const int j0 = t * kAttnK;
-    if (j0 > jhi) continue;                     // no key for any of the wave's queries
-    const uint32_t kt = base + (uint32_t)((t & 1) * 2 * T::BYTES), vt = kt + T::BYTES;
-
+  auto step = [&](int j0) {
+    constexpr uint32_t kt = 0, vt = T::BYTES;
     f32x16 s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -128,6 +121,15 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] = mfma(fr.cols(vt, d, u), e, o[d]);
     }
+  };
+  if (tiles > 0) load(0);
+  for (int t = 0; t < tiles; ++t) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's part of tile t has landed
+    lds_barrier();                              // everyone's has, and tile t - 1 has been read
+    if (t + 1 < tiles) load(t + 1);
+    // (past jhi no key is left for any of the wave's queries)
+    if (t * kAttnK <= jhi) step(t * kAttnK);
+    fr.move(t & 1 ? -2 * T::BYTES : 2 * T::BYTES);
   }
 
   const Halves both = halves(l);

@@ -69,11 +69,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
   const uint16_t* kp = a.k + p.k0 * a.k_t + (int64_t)hk * a.k_h;
   const uint16_t* vp = a.v + p.k0 * a.v_t + (int64_t)hk * a.v_h;
   T tk, tv;
-  tk.init(a.k_t, a.D, wave, lane);
-  tv.init(a.v_t, a.D, wave, lane);
-  Frags<DIM> fr;
-  fr.init(lane);
+  tk.init(a.k_t, a.D, lane);
+  tv.init(a.v_t, a.D, lane);
   const uint32_t base = lds_addr(lds);
+  Frags<DIM> fr;
+  fr.init(base, lane);
 
   f32x16 dq[ND];
 #pragma unroll
@@ -83,14 +83,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
     tk.load(kp + (int64_t)t * kStep * a.k_t, p.lk - t * kStep, s, wave);
     tv.load(vp + (int64_t)t * kStep * a.v_t, p.lk - t * kStep, s + T::BYTES, wave);
   };
-  if (tiles > 0) load(0);
-  for (int t = 0; t < tiles; ++t) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-    lds_barrier();
-    if (t + 1 < tiles) load(t + 1);
-    const int j0 = t * kStep;
-    if (j0 > jhi) continue;
-    const uint32_t kt = base + (uint32_t)((t & 1) * 2 * T::BYTES), vt = kt + T::BYTES;
+  auto step = [&](int j0) {
+    constexpr uint32_t kt = 0, vt = T::BYTES;
     const bool masked = j0 + kStep - 1 > jlo;
     const int lim = jmax - j0 - 4 * (lane >> 5);
 #pragma unroll
@@ -113,6 +107,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
         for (int d = 0; d < ND; ++d) dq[d] = mfma(fr.cols(kt, d, 2 * i + u), ds, dq[d]);
       }
     }
+  };
+  if (tiles > 0) load(0);
+  for (int t = 0; t < tiles; ++t) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    lds_barrier();
+    if (t + 1 < tiles) load(t + 1);
+    if (t * kStep <= jhi) step(t * kStep);
+    fr.move(t & 1 ? -2 * T::BYTES : 2 * T::BYTES);
   }
   uint16_t* out = a.dq + (p.q0 + row0) * a.dq_t + (int64_t)head * a.dq_h;
 #pragma unroll
@@ -123,7 +125,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
 // (rows: queries), so P and dS are the B operands of dv^T += dout^T P and
 // dk^T += q^T dS as they come.  lse and delta of a step's queries lie in LDS.
 template <int NK, int KB>
-__global__ __launch_bounds__(256, KB == 1 && NK <= 4 ? 2 : 1) void attn_dkv_kernel(AttnBwd a) {
+__global__ __launch_bounds__(256, KB == 1 ? 2 : 1) void attn_dkv_kernel(AttnBwd a) {
   typedef Dim<NK> DIM;
   typedef Tile<DIM, kStep, 4> T;
   constexpr int ND = DIM::ND, KEYS = 128 * KB;
@@ -152,11 +154,11 @@ __global__ __launch_bounds__(256, KB == 1 && NK <= 4 ? 2 : 1) void attn_dkv_kern
     for (int d = 0; d < ND; ++d) dk[b][d] = dv[b][d] = zero16();
   }
   T tq, tg;
-  tq.init(a.q_t, a.D, wave, lane);
-  tg.init(a.do_t, a.D, wave, lane);
-  Frags<DIM> fr;
-  fr.init(lane);
+  tq.init(a.q_t, a.D, lane);
+  tg.init(a.do_t, a.D, lane);
   const uint32_t base = lds_addr(lds), stats = base + 4 * T::BYTES;
+  Frags<DIM> fr;
+  fr.init(base, lane);
 
   auto load = [&](int it) {
     const int r = it / per, i0 = (t0 + it - r * per) * kStep, head = hk * a.rep + r;
@@ -170,79 +172,68 @@ __global__ __launch_bounds__(256, KB == 1 && NK <= 4 ? 2 : 1) void attn_dkv_kern
       dma4(rs, (uint32_t)lane * 4, stats + (uint32_t)(((it & 1) * 2 + wave) * kStep * 4));
     }
   };
+  uint32_t own = stats + (uint32_t)((lane >> 5) * 16);   // lse of the half wave's first row
+  auto step = [&](int i0) {
+    constexpr uint32_t qt = 0, gt = T::BYTES;
+    const bool masked = a.causal && i0 + off < key0 + 32 * KB - 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      bf16x8 pb[KB][2], ds[KB][2];
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) s = mfma(fr.rows(qt, i, kk), k[b].f[kk], s);
+        if (masked) {
+          // key j sees queries from j - off on
+          const int lim = key0 + 32 * b + (lane & 31) - off - i0 - 4 * (lane >> 5);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? -INFINITY : s[r];
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const i32x4 lse = *(const lds_i32x4*)(lds_at(own) + (32 * i + 8 * g) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.c, -__int_as_float(lse[e])));
+        }
+        pb[b][0] = round8(s, 0);
+        pb[b][1] = round8(s, 1);
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) dp = mfma(fr.rows(gt, i, kk), v[b].f[kk], dp);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const i32x4 delta = *(const lds_i32x4*)(lds_at(own) + (kStep + 32 * i + 8 * g) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - __int_as_float(delta[e]));
+        }
+        ds[b][0] = round8(dp, 0);
+        ds[b][1] = round8(dp, 1);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const bf16x8 x = fr.cols(gt, d, 2 * i + u), y = fr.cols(qt, d, 2 * i + u);
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            dv[b][d] = mfma(x, pb[b][u], dv[b][d]);
+            dk[b][d] = mfma(y, ds[b][u], dk[b][d]);
+          }
+        }
+    }
+  };
   if (steps > 0) load(0);
   for (int it = 0; it < steps; ++it) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     lds_barrier();
     if (it + 1 < steps) load(it + 1);
     const int i0 = (t0 + it % per) * kStep;
-    // causal: the step's last query sees none of the wave's keys
-    if (a.causal && i0 + kStep - 1 + off < key0) continue;
-    const uint32_t qt = base + (uint32_t)((it & 1) * 2 * T::BYTES), gt = qt + T::BYTES;
-    const uint32_t st = stats + (uint32_t)((it & 1) * 2 * kStep * 4) + (uint32_t)((lane >> 5) * 16);
-    const bool masked = a.causal && i0 + off < key0 + 32 * KB - 1;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float lse[16], delta[16];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const i32x4 x = *(const lds_i32x4*)(lds_at(st) + (32 * i + 8 * g) * 4);
-        const i32x4 y = *(const lds_i32x4*)(lds_at(st) + (kStep + 32 * i + 8 * g) * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          lse[4 * g + e] = __int_as_float(x[e]);
-          delta[4 * g + e] = __int_as_float(y[e]);
-        }
-      }
-      f32x16 s[KB], dp[KB];
-#pragma unroll
-      for (int b = 0; b < KB; ++b) s[b] = dp[b] = zero16();
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        const bf16x8 x = fr.rows(qt, i, kk);
-#pragma unroll
-        for (int b = 0; b < KB; ++b) s[b] = mfma(x, k[b].f[kk], s[b]);
-      }
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        const bf16x8 x = fr.rows(gt, i, kk);
-#pragma unroll
-        for (int b = 0; b < KB; ++b) dp[b] = mfma(x, v[b].f[kk], dp[b]);
-      }
-      if (masked)
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          // key j sees queries from j - off on
-          const int lim = key0 + 32 * b + (lane & 31) - off - i0 - 4 * (lane >> 5);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[b][r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? -INFINITY : s[b][r];
-        }
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], a.c, -lse[r]));
-          dp[b][r] = s[b][r] * (dp[b][r] - delta[r]);
-        }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        bf16x8 pb[KB], ds[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          pb[b] = round8(s[b], u);
-          ds[b] = round8(dp[b], u);
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const bf16x8 x = fr.cols(gt, d, 2 * i + u), y = fr.cols(qt, d, 2 * i + u);
-#pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            dv[b][d] = mfma(x, pb[b], dv[b][d]);
-            dk[b][d] = mfma(y, ds[b], dk[b][d]);
-          }
-        }
-      }
-    }
+    // (causal: where the step's last query sees none of the wave's keys there is nothing to add)
+    if (!a.causal || i0 + kStep - 1 + off >= key0) step(i0);
+    const int sign = it & 1 ? -1 : 1;
+    fr.move(sign * 2 * T::BYTES);
+    own += (uint32_t)(sign * 2 * kStep * 4);
   }
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
