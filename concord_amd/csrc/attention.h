@@ -10,6 +10,9 @@
 // of a result are the depth indices 16 t + {0 .. 3, 8 .. 11} + 4 (l >> 5), and
 // the A operand is read in that order (Tile::cols).
 #pragma once
+#include <type_traits>
+#include <utility>
+
 #include "common.h"
 
 namespace concord {
@@ -51,6 +54,17 @@ CONCORD_DEV Halves halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return Halves{__uint_as_float(r[0]), __uint_as_float(r[1])};
 }
+
+// f(0), f(1), ... f(N - 1) with compile-time arguments
+template <class F, int... I>
+CONCORD_DEV void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+CONCORD_DEV void static_for(F&& f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>());
+}
+#define CONCORD_INLINE_LAMBDA __attribute__((always_inline))
 
 // ---- LDS and barriers --------------------------------------------------------
 CONCORD_DEV uint32_t lds_addr(const void* p) {

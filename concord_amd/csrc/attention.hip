@@ -32,6 +32,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   typedef Dim<NK> DIM;
   typedef Tile<DIM, kAttnK, 4> T;
   constexpr int ND = DIM::ND;
+  constexpr bool PIPE = NK > 4;
   __shared__ __attribute__((aligned(1024))) char lds[4 * T::BYTES];   // two slots of k and v
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lin = attn_xcd(blockIdx.x, gridDim.x);
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   T tk, tv;
   tk.init(a.k_t, a.D, lane);
   tv.init(a.v_t, a.D, lane);
-  const uint32_t base = lds_addr(lds);
+  const uint32_t base = lds_addr(lds);   // two slots of k, then two of v
   Frags<DIM> fr;
   fr.init(base, lane);
 
@@ -70,38 +71,38 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   for (int d = 0; d < ND; ++d) o[d] = zero16();
   float m = -3.4028235e38f, l = 0.0f;   // of the scaled scores, in powers of two; l: this half wave's keys
 
-  auto load = [&](int t) {
-    const uint32_t s = base + (uint32_t)((t & 1) * 2 * T::BYTES);
-    tk.load(kp + (int64_t)t * kAttnK * a.k_t, p.lk - t * kAttnK, s, wave);
-    tv.load(vp + (int64_t)t * kAttnK * a.v_t, p.lk - t * kAttnK, s + T::BYTES, wave);
+  auto load_k = [&](int t) {
+    tk.load(kp + (int64_t)t * kAttnK * a.k_t, p.lk - t * kAttnK, base + (uint32_t)((t & 1) * T::BYTES), wave);
   };
-  auto step = [&](int j0) {
-    constexpr uint32_t kt = 0, vt = T::BYTES;
-    f32x16 s[2];
+  auto load_v = [&](int t) {
+    tv.load(vp + (int64_t)t * kAttnK * a.v_t, p.lk - t * kAttnK, base + (uint32_t)((2 + (t & 1)) * T::BYTES), wave);
+  };
+  auto lane_max = [&](const f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
+    float x = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      s[i] = zero16();
-#pragma unroll
-      for (int k = 0; k < NK; ++k) s[i] = mfma(fr.rows(kt, i, k), q.f[k], s[i]);
-    }
+    for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
+    return x;
+  };
+  // Before the exponentials of tile t: its mask, and the maximum they are
+  // relative to.  mx: the largest of the lane's scores (unmasked).
+  auto settle = [&](int t, f32x16 (&s)[2], float mx) CONCORD_INLINE_LAMBDA {
+    const int j0 = t * kAttnK;
     if (j0 + kAttnK - 1 > jlo) {
       const int lim = jmax - j0 - 4 * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + 8 * (r >> 2) + (r & 3) > lim ? -INFINITY : s[i][r];
+      mx = lane_max(s);
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
     const Halves both = halves(mx);
-    mx = fmaxf(both.lo, both.hi) * a.c;
+    const float top = fmaxf(both.lo, both.hi) * a.c;
     // The sums are relative to m, which follows the maximum only when that has
     // grown by more than 2^8: the factor of out and l is then nearly never
     // applied, and the probabilities stay within 2^8, exact in their type as
     // those below 1 are.
-    if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {
-      const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
+      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
@@ -109,27 +110,132 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= f;
     }
-#pragma unroll
-    for (int r = 0; r < 32; ++r) {
-      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], a.c, -m));
-      s[r >> 4][r & 15] = e;
-      l += e;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bf16x8 e = round8(s[u >> 1], u & 1);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = mfma(fr.cols(vt, d, u), e, o[d]);
-    }
   };
-  if (tiles > 0) load(0);
-  for (int t = 0; t < tiles; ++t) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's part of tile t has landed
-    lds_barrier();                              // everyone's has, and tile t - 1 has been read
-    if (t + 1 < tiles) load(t + 1);
-    // (past jhi no key is left for any of the wave's queries)
-    if (t * kAttnK <= jhi) step(t * kAttnK);
-    fr.move(t & 1 ? -2 * T::BYTES : 2 * T::BYTES);
+  // Tile t's exponentials and product with v, and (NEXT) the scores of tile
+  // t + 1.  A wave issues in order and an MFMA holds the matrix core for 32
+  // clocks, so the step is laid out by hand: unit j is one MFMA (first those of
+  // the scores, then those with v), the fragment read of unit j + AHEAD, and
+  // its share of the exponentials and of the next maximum; nothing moves
+  // between units.
+  auto step = [&](auto nextc, auto slotc, f32x16 (&s)[2], f32x16 (&next)[2], float& mx) CONCORD_INLINE_LAMBDA {
+    constexpr bool NEXT = decltype(nextc)::value;
+    constexpr int SLOT = decltype(slotc)::value, AHEAD = 2;
+    constexpr int NS = NEXT ? 2 * NK : 0, NU = NS + 4 * ND;          // units of the scores, of the step
+    constexpr uint32_t kt = (1 - SLOT) * T::BYTES, vt = (2 + SLOT) * T::BYTES;
+    bf16x8 frag[AHEAD + 1], e[4];
+    auto read = [&](auto jc) CONCORD_INLINE_LAMBDA {
+      constexpr int j = decltype(jc)::value;
+      if constexpr (j < NS) frag[j % (AHEAD + 1)] = fr.rows(kt, j & 1, j >> 1);
+      else if constexpr (j < NU) frag[j % (AHEAD + 1)] = fr.cols(vt, (j - NS) % ND, (j - NS) / ND);
+    };
+    // exponentials done after n units: all before the last quarter of the
+    // products with v, and each quarter's before its products
+    constexpr auto done = [](int n) constexpr {
+      const int even = (32 * n + NS + 3 * ND - 1) / (NS + 3 * ND);
+      const int need = n >= NS ? 8 * ((n - NS) / ND + 1) : 0;
+      const int v = even > need ? even : need;
+      return v < 32 ? v : 32;
+    };
+    auto exps = [&](auto fromc, auto toc) CONCORD_INLINE_LAMBDA {
+      constexpr int from = decltype(fromc)::value, to = decltype(toc)::value;
+      static_for<to - from>([&](auto rc) CONCORD_INLINE_LAMBDA {
+        constexpr int r = from + decltype(rc)::value;
+        float& x = reinterpret_cast<float*>(&s[r >> 4])[r & 15];
+        x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c, -m));
+        l += x;
+        if constexpr (r % 8 == 7) e[r / 8] = round8(s[r >> 4], (r >> 3) & 1);
+      });
+    };
+    static_for<AHEAD>([&](auto jc) CONCORD_INLINE_LAMBDA { read(jc); });
+    exps(std::integral_constant<int, 0>(), std::integral_constant<int, done(0)>());
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<NU>([&](auto jc) CONCORD_INLINE_LAMBDA {
+      constexpr int j = decltype(jc)::value;
+      read(std::integral_constant<int, j + AHEAD>());
+      if constexpr (j < NS) {
+        constexpr int i = j & 1, k = j >> 1;
+        next[i] = mfma(frag[j % (AHEAD + 1)], q.f[k], k == 0 ? zero16() : next[i]);
+      } else {
+        constexpr int d = (j - NS) % ND, u = (j - NS) / ND;
+        o[d] = mfma(frag[j % (AHEAD + 1)], e[u], o[d]);
+        if constexpr (NEXT) {
+          // 32 scores over the 4 ND units
+          constexpr int from = 32 * (j - NS) / (4 * ND), to = 32 * (j - NS + 1) / (4 * ND);
+#pragma unroll
+          for (int r = from; r < to; ++r) mx = r == 0 ? next[0][0] : fmaxf(mx, next[r >> 4][r & 15]);
+        }
+      }
+      exps(std::integral_constant<int, done(j)>(), std::integral_constant<int, done(j + 1)>());
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  const int own = jhi < 0 ? 0 : min(tiles, jhi / kAttnK + 1);   // tiles with a key for any of the wave's queries
+  typedef std::integral_constant<int, 0> S0;
+  typedef std::integral_constant<int, 1> S1;
+  auto first_scores = [&](f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = zero16();
+#pragma unroll
+      for (int k = 0; k < NK; ++k) s[i] = mfma(fr.rows(0, i, k), q.f[k], s[i]);
+    }
+    return lane_max(s);
+  };
+  if constexpr (!PIPE) {
+    if (tiles > 0) load_k(0), load_v(0);
+    for (int t = 0; t < tiles; ++t) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's part of tile t has landed
+      lds_barrier();                              // everyone's has, and tile t - 1 has been read
+      if (t + 1 < tiles) load_k(t + 1), load_v(t + 1);
+      if (t < own) {
+        f32x16 s[2];
+        float mx = first_scores(s);
+        settle(t, s, mx);
+        step(std::false_type(), S0(), s, s, mx);
+      }
+      fr.move(t & 1 ? -T::BYTES : T::BYTES);
+    }
+  } else if (tiles > 0) {
+    // before tile t: its values and tile t + 1's keys have landed, and those of
+    // the slots to fill next have been read
+    auto turn = [&](int t) CONCORD_INLINE_LAMBDA {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      lds_barrier();
+      if (t + 2 < tiles) load_k(t + 2);
+      if (t + 1 < tiles) load_v(t + 1);
+    };
+    f32x16 sa[2], sb[2];
+    load_k(0);
+    load_v(0);
+    if (tiles > 1) load_k(1);
+    if (tiles > 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * T::PER));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::PER));
+    lds_barrier();
+    float mx = first_scores(sa);
+    int t = 0;
+    for (; t + 2 < own; t += 2) {
+      turn(t);
+      settle(t, sa, mx);
+      step(std::true_type(), S0(), sa, sb, mx);
+      turn(t + 1);
+      settle(t + 1, sb, mx);
+      step(std::true_type(), S1(), sb, sa, mx);
+    }
+    if (t + 1 < own) {
+      turn(t);
+      settle(t, sa, mx);
+      step(std::true_type(), S0(), sa, sb, mx);
+      turn(t + 1);
+      settle(t + 1, sb, mx);
+      step(std::false_type(), S1(), sb, sa, mx);
+      t += 2;
+    } else if (t < own) {
+      turn(t);
+      settle(t, sa, mx);
+      step(std::false_type(), S0(), sa, sb, mx);
+      ++t;
+    }
+    for (; t < tiles; ++t) turn(t);
   }
 
   const Halves both = halves(l);
