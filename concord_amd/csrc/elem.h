@@ -27,6 +27,18 @@ struct alignas(sizeof(T) * VEC) Chunk {
   T v[VEC];
 };
 
+// a store of a result that this kernel does not read again: past the caches,
+// which keep the operands (layer norm of 32768 x 4096 bf16: 108 -> 88 us)
+template <class V>
+CONCORD_DEV void store_stream(V* p, const V& v) {
+  if constexpr (sizeof(V) == 16) {
+    typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(i32x4, v), (i32x4*)p);
+  } else {
+    *p = v;
+  }
+}
+
 // the value of element i of a vector of any of the three types
 CONCORD_DEV float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == CONCORD_F32) return ((const float*)p)[i];

@@ -33,10 +33,13 @@ struct LnArgs {
 // VEC columns from (i W 64 + t) VEC.
 template <class T, int VEC, int E, int W>
 struct LnRow {
-  static constexpr int NV = E / VEC, ROWS = W == 1 ? 4 : 1, THREADS = W * ROWS * 64;
-  // the next row's loads are issued before this row's sums; not in a block of
-  // 16 waves, whose 128 registers a thread hold one row at a time
-  static constexpr bool AHEAD = W < 16;
+  static constexpr int NV = E / VEC, SLOTS = W == 1 ? 4 : 1, THREADS = W * SLOTS * 64;
+  // rows a wave takes at once where it has rows of its own: their loads and sums
+  // overlap, and a short row alone has too few bytes in flight
+  static constexpr int R = W > 1 ? 1 : E == 8 ? 4 : 2;
+  // with one row at a time the next row's loads are issued before this row's
+  // sums; not in a block of 16 waves, whose 128 registers a thread hold one row
+  static constexpr bool AHEAD = W > 1 && W < 16;
   typedef Chunk<T, VEC> V;
   // the thread's place among its row's threads, and its row in the block
   static CONCORD_DEV int lane() { return W == 1 ? threadIdx.x & 63 : threadIdx.x; }
@@ -58,15 +61,18 @@ struct LnRow {
       V r;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<T>(v[i * VEC + e]);
-      if (col(i) < C) *(V*)(q + col(i)) = r;
+      if (col(i) < C) store_stream((V*)(q + col(i)), r);
     }
   }
   template <class P>
   static CONCORD_DEV void vector_of(float (&v)[E], const P* p, int C) {
+    constexpr int PV = VEC * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : VEC;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
+    for (int i = 0; i < E; i += PV) {
       const int c = col(i / VEC) + i % VEC;
-      v[i] = to_f32(p[c < C ? c : 0]);
+      const Chunk<P, PV> w = *(const Chunk<P, PV>*)(p + (c < C ? c : 0));
+#pragma unroll
+      for (int e = 0; e < PV; ++e) v[i + e] = to_f32(w.v[e]);
     }
   }
   // the weight or the bias at the thread's columns (any value past C)
@@ -107,34 +113,54 @@ __global__ __launch_bounds__((LnRow<T, VEC, E, W>::THREADS)) void ln_fwd_kernel(
 #pragma unroll
   for (int k = 1; k < W; ++k) inv_own = wave == k ? inv_n[k] : inv_own;
   const float inv_c = 1.0f / (float)C;
-  const int64_t step = (int64_t)gridDim.x * R::ROWS;
-  int64_t row = (int64_t)blockIdx.x * R::ROWS + R::slot();
-  V raw[NV];
-  if (R::AHEAD && row < a.M) R::load(raw, a.x, row, a.ldx, C);
+  constexpr int NR = R::R;
+  const int64_t step = (int64_t)gridDim.x * R::SLOTS * NR;
+  int64_t row = ((int64_t)blockIdx.x * R::SLOTS + R::slot()) * NR;
+  V raw[NR][NV];
+  auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+      if (NR == 1 || r0 + r < a.M) R::load(raw[r], a.x, r0 + r, a.ldx, C);
+  };
+  if (R::AHEAD && row < a.M) fetch(row);
   // (a block with W > 1 takes one row at a time: its waves leave together)
   for (int par = 0; row < a.M; row += step, par ^= 1) {
-    float x[E];
-    if (!R::AHEAD) R::load(raw, a.x, row, a.ldx, C);
+    float x[NR][E];
+    if (!R::AHEAD) fetch(row);
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = to_f32(raw[i / VEC].v[i % VEC]);
-    if (R::AHEAD && row + step < a.M) R::load(raw, a.x, row + step, a.ldx, C);
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[r][i] = to_f32(raw[r][i / VEC].v[i % VEC]);
+    if (R::AHEAD && row + step < a.M) fetch(row + step);
     // mean, then the squares about it; over several waves each about its own
     // mean, joined as M2 = sum M2_w + n_w (mean_w - mean)^2
-    float s = 0.0f;
+    float s[NR], mean[NR], m2[NR];
 #pragma unroll
-    for (int i = 0; i < E; ++i) s += x[i];
-    s = wave_sum(s);
-    float mean = s * inv_own, m2 = 0.0f;
+    for (int r = 0; r < NR; ++r) {
+      s[r] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float d = x[i] - mean;
-      m2 = R::col(i / VEC) < C ? __builtin_fmaf(d, d, m2) : m2;
+      for (int i = 0; i < E; ++i) s[r] += x[r][i];
     }
-    m2 = wave_sum(m2);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      s[r] = wave_sum(s[r]);
+      mean[r] = s[r] * inv_own;
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      m2[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float d = x[r][i] - mean[r];
+        m2[r] = R::col(i / VEC) < C ? __builtin_fmaf(d, d, m2[r]) : m2[r];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) m2[r] = wave_sum(m2[r]);
     if (W > 1) {
       if ((threadIdx.x & 63) == 0) {
-        red[par][wave][0] = s;
-        red[par][wave][1] = m2;
+        red[par][wave][0] = s[0];
+        red[par][wave][1] = m2[0];
       }
       __syncthreads();
       float tot = 0.0f, tot2 = 0.0f;
@@ -146,17 +172,22 @@ __global__ __launch_bounds__((LnRow<T, VEC, E, W>::THREADS)) void ln_fwd_kernel(
         const float d = red[par][k][0] * inv_n[k] - all;
         tot2 += __builtin_fmaf(n[k] * d, d, red[par][k][1]);
       }
-      mean = all;
-      m2 = tot2;
+      mean[0] = all;
+      m2[0] = tot2;
     }
-    const float rstd = 1.0f / __builtin_sqrtf(m2 * inv_c + a.eps);
-    float y[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = __builtin_fmaf((x[i] - mean) * rstd, w[i], b[i]);
-    R::store(a.out, row, a.ldo, C, y);
-    if (a.mean && R::lane() == 0) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
+    for (int r = 0; r < NR; ++r) {
+      const float rstd = 1.0f / __builtin_sqrtf(m2[r] * inv_c + a.eps);
+      float y[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = __builtin_fmaf((x[r][i] - mean[r]) * rstd, w[i], b[i]);
+      if (NR == 1 || row + r < a.M) {
+        R::store(a.out, row + r, a.ldo, C, y);
+        if (a.mean && R::lane() == 0) {
+          a.mean[row + r] = mean[r];
+          a.rstd[row + r] = rstd;
+        }
+      }
     }
   }
 }
@@ -174,58 +205,76 @@ __global__ __launch_bounds__((LnRow<T, VEC, E, W>::THREADS)) void ln_bwd_kernel(
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
   const float inv_c = 1.0f / (float)C;
-  const int64_t step = (int64_t)gridDim.x * R::ROWS;
-  int64_t row = (int64_t)blockIdx.x * R::ROWS + R::slot();
-  V rx[NV], ry[NV];
-  float mean = 0.0f, rstd = 0.0f;
-  auto fetch = [&](int64_t r) {
-    R::load(rx, a.x, r, a.ldx, C);
-    R::load(ry, a.dy, r, a.ldy, C);
-    mean = a.mean[r];
-    rstd = a.rstd[r];
+  constexpr int NR = R::R;
+  const int64_t step = (int64_t)gridDim.x * R::SLOTS * NR;
+  int64_t row = ((int64_t)blockIdx.x * R::SLOTS + R::slot()) * NR;
+  V rx[NR][NV], ry[NR][NV];
+  float mean[NR], rstd[NR];
+  auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      // (no row there: the first again, its dy taken as zeros)
+      const int64_t at = NR == 1 || r0 + r < a.M ? r0 + r : r0;
+      R::load(rx[r], a.x, at, a.ldx, C);
+      R::load(ry[r], a.dy, at, a.ldy, C);
+      mean[r] = a.mean[at];
+      rstd[r] = a.rstd[at];
+    }
   };
   if (R::AHEAD && row < a.M) fetch(row);
   for (int par = 0; row < a.M; row += step, par ^= 1) {
     if (!R::AHEAD) fetch(row);
-    float h[E], dy[E];
-    float s1 = 0.0f, s2 = 0.0f;
+    float h[NR][E], dy[NR][E], s1[NR], s2[NR], rs[NR];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      // a column past C has dy = 0, so it adds nothing below
-      h[i] = (to_f32(rx[i / VEC].v[i % VEC]) - mean) * rstd;
-      dy[i] = to_f32(ry[i / VEC].v[i % VEC]);
+    for (int r = 0; r < NR; ++r) {
+      rs[r] = rstd[r];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        // a column past C has dy = 0, so it adds nothing below
+        h[r][i] = (to_f32(rx[r][i / VEC].v[i % VEC]) - mean[r]) * rstd[r];
+        dy[r][i] = NR == 1 || row + r < a.M ? to_f32(ry[r][i / VEC].v[i % VEC]) : 0.0f;
+      }
     }
-    const float r = rstd;
     if (R::AHEAD && row + step < a.M) fetch(row + step);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const bool in = R::col(i / VEC) < C;
-      const float hy = in ? dy[i] * h[i] : 0.0f;
-      dw[i] += hy;
-      db[i] += dy[i];
-      s1 = in ? __builtin_fmaf(dy[i], w[i], s1) : s1;
-      s2 = in ? __builtin_fmaf(hy, w[i], s2) : s2;
+    for (int r = 0; r < NR; ++r) {
+      s1[r] = s2[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const bool in = R::col(i / VEC) < C;
+        const float hy = in ? dy[r][i] * h[r][i] : 0.0f;
+        dw[i] += hy;
+        db[i] += dy[r][i];
+        s1[r] = in ? __builtin_fmaf(dy[r][i], w[i], s1[r]) : s1[r];
+        s2[r] = in ? __builtin_fmaf(hy, w[i], s2[r]) : s2[r];
+      }
     }
-    s1 = wave_sum(s1);
-    s2 = wave_sum(s2);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      s1[r] = wave_sum(s1[r]);
+      s2[r] = wave_sum(s2[r]);
+    }
     if (W > 1) {
       if ((threadIdx.x & 63) == 0) {
-        red[par][wave][0] = s1;
-        red[par][wave][1] = s2;
+        red[par][wave][0] = s1[0];
+        red[par][wave][1] = s2[0];
       }
       __syncthreads();
-      s1 = s2 = 0.0f;
+      s1[0] = s2[0] = 0.0f;
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        s1 += red[par][k][0];
-        s2 += red[par][k][1];
+        s1[0] += red[par][k][0];
+        s2[0] += red[par][k][1];
       }
     }
-    const float m1 = s1 * inv_c, m2 = s2 * inv_c;
-    float dx[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) dx[i] = r * (__builtin_fmaf(dy[i], w[i], -m1) - h[i] * m2);
-    R::store(a.out, row, a.ldo, C, dx);
+    for (int r = 0; r < NR; ++r) {
+      const float m1 = s1[r] * inv_c, m2 = s2[r] * inv_c;
+      float dx[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) dx[i] = rs[r] * (__builtin_fmaf(dy[r][i], w[i], -m1) - h[r][i] * m2);
+      if (NR == 1 || row + r < a.M) R::store(a.out, row + r, a.ldo, C, dx);
+    }
   }
   if (!a.part) return;
   float* part = a.part + (int64_t)blockIdx.x * 2 * a.C;
@@ -381,12 +430,14 @@ __global__ __launch_bounds__(1024) void ln_cols_sum_kernel(const float* __restri
 // 0: longer than a block holds
 static int ln_waves(int64_t C) { return C <= 1024 ? 1 : C <= 4096 ? 4 : C <= 8192 ? 8 : C <= 16384 ? 16 : 0; }
 
+// rows a block takes at once (LnRow::SLOTS * LnRow::R)
+static int64_t ln_block_rows(int64_t C) { return C <= 512 ? 16 : C <= 1024 ? 8 : 1; }
+
 // blocks of the backward, each with one partial row of dw and db
 static int64_t ln_bwd_blocks(int64_t M, int64_t C) {
   const int W = ln_waves(C);
   if (W == 0) return std::min<int64_t>(M, 256);
-  const int64_t rows = W == 1 ? 4 : 1;
-  return std::min<int64_t>(cdiv(M, rows), W >= 8 ? 512 : 1024);
+  return std::min<int64_t>(cdiv(M, ln_block_rows(C)), W >= 8 ? 256 : 512);
 }
 
 static size_t elem_size(int dtype) { return dtype == CONCORD_F32 ? 4 : 2; }
@@ -416,9 +467,9 @@ static void ln_pass(bool bwd, const LnArgs& a, hipStream_t st) {
   const int W = ln_waves(a.C);
   const size_t es = sizeof(T);
   const bool vec = a.C % (16 / es) == 0 && chunked(a.x, a.ldx, es) && chunked(a.out, a.ldo, es) &&
-                   (!bwd || chunked(a.dy, a.ldy, es));
-  const int64_t rows = W == 1 ? 4 : 1;
-  const unsigned grid = (unsigned)(bwd ? ln_bwd_blocks(a.M, a.C) : std::min<int64_t>(cdiv(a.M, rows), 2048));
+                   (!bwd || chunked(a.dy, a.ldy, es)) && (((uintptr_t)a.w | (uintptr_t)a.b) & 15) == 0;
+  const unsigned grid =
+      (unsigned)(bwd ? ln_bwd_blocks(a.M, a.C) : std::min<int64_t>(cdiv(a.M, ln_block_rows(a.C)), 2048));
   constexpr int V = 16 / (int)sizeof(T);
   if (W == 0) {
     if (!bwd) hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3(std::min<int64_t>(a.M, 1024)), dim3(1024), 0, st, a);

@@ -347,7 +347,7 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& index,
                         double temperature) {
     const DistillRows r(logits, teacher, index);
-    Tensor stats = at::empty({r.rows, 2}, logits.options().dtype(at::kFloat));
+    Tensor stats = at::empty({r.rows, 4}, logits.options().dtype(at::kFloat));
     Tensor loss = distill_forward(r, logits, temperature, stats);
     ctx->save_for_backward({r.z.t, r.t.t, r.i.t, stats});
     ctx->saved_data["shape"] = logits.sizes().vec();

@@ -536,8 +536,8 @@ int concord_layernorm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t 
  * dtype): with temperature T, q = softmax(logits / T) and p = softmax(teacher
  * / T) over the row's K entries, loss = T^2 sum_k p_k (log p_k - log
  * q[index_k]).  Entries whose index lies outside [0, V) are left out; a row
- * without any has loss 0.  K <= 1024.  stats [M][2] (may be NULL) is kept for
- * the backward.  workspace: concord_distill_workspace_bytes(M, V) bytes (0:
+ * without any has loss 0.  K <= 1024.  stats [M][4] (16-byte aligned, may be
+ * NULL) is kept for the backward.  workspace: concord_distill_workspace_bytes(M, V) bytes (0:
  * none needed); it need not be zeroed. */
 size_t concord_distill_workspace_bytes(int64_t M, int64_t V);
 int concord_distill_fwd(const void* logits, int64_t ld_l, int dtype, int64_t M, int64_t V, const float* teacher,
