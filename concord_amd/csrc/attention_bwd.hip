@@ -20,12 +20,13 @@ struct AttnBwd {
   const float* lse;
   const int8_t* low;
   float* delta;
+  float* part;      // split dk and dv
   AttnSeqs seq;
-  int32_t slots, rep, D, causal, heads;
+  int32_t slots, rep, D, causal, heads, rows_h, splits;   // rows_h: key heads
   float c, scale;
 };
 
-constexpr int kDqRows = 128;   // queries of a dq workgroup
+constexpr int kDqRows = 128, kDkvRows = 128;   // queries of a dq workgroup, keys of a dk / dv one
 constexpr int kStep = 64;      // keys (queries) of a step
 
 // dq and delta: the forward's shape.  A lane holds one query's column of the
@@ -121,38 +122,45 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
   for (int d = 0; d < ND; ++d) store_block(out, a.dq_t, rows, a.D, d, dq[d], a.scale, lane);
 }
 
-// dk and dv: a wave holds KB blocks of 32 keys, and the scores untransposed
-// (rows: queries), so P and dS are the B operands of dv^T += dout^T P and
+// dk and dv: a wave holds 32 keys, and the scores untransposed (rows:
+// queries), so P and dS are the B operands of dv^T += dout^T P and
 // dk^T += q^T dS as they come.  lse and delta of a step's queries lie in LDS.
-template <int NK, int KB>
-__global__ __launch_bounds__(256, KB == 1 ? 2 : 1) void attn_dkv_kernel(AttnBwd a) {
+//
+// SPLIT: a workgroup takes one of `splits` equal shares of the steps and leaves
+// fp32 sums for attn_dkv_sum_kernel.
+template <int NK, bool SPLIT>
+__global__ __launch_bounds__(256, NK <= 4 ? 3 : 2) void attn_dkv_kernel(AttnBwd a) {
   typedef Dim<NK> DIM;
   typedef Tile<DIM, kStep, 4> T;
-  constexpr int ND = DIM::ND, KEYS = 128 * KB;
+  constexpr int ND = DIM::ND;
+  // two slots of q and dout, then two of lse and delta
   __shared__ __attribute__((aligned(1024))) char lds[4 * T::BYTES + 2 * 2 * kStep * 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lin = attn_xcd(blockIdx.x, gridDim.x);
+  int lin = attn_xcd(blockIdx.x, gridDim.x), share = 0;
+  if (SPLIT) {
+    share = lin % a.splits;
+    lin /= a.splits;
+  }
   const int hk = lin / a.slots, slot = lin - hk * a.slots;   // (the first keys have the most queries)
-  const AttnPlace p = attn_place<KEYS, true>(a.seq, slot);
+  const AttnPlace p = attn_place<kDkvRows, true>(a.seq, slot);
   if (p.first < 0 || p.first >= p.lk) return;
 
-  const int key0 = p.first + wave * 32 * KB, off = p.lk - p.lq;
+  const int key0 = p.first + wave * 32, left = p.lk - key0, off = p.lk - p.lq;
   // the first query that sees any of the workgroup's keys
   const int first = a.causal ? max(0, p.first - off) : 0;
   const int t0 = first / kStep;
   const int per = max(0, (p.lq + kStep - 1) / kStep - t0);   // steps of a head
   const int steps = per * a.rep;
+  const int it0 = SPLIT ? (int)((int64_t)steps * share / a.splits) : 0;
+  const int it1 = SPLIT ? (int)((int64_t)steps * (share + 1) / a.splits) : steps;
 
-  Fixed<DIM> k[KB], v[KB];
-  f32x16 dk[KB][ND], dv[KB][ND];
+  Fixed<DIM> k, v;
+  f32x16 dk[ND], dv[ND];
+  const int64_t tok = p.k0 + key0;
+  k.load(a.k + tok * a.k_t + (int64_t)hk * a.k_h, left, a.k_t, a.D, lane);
+  v.load(a.v + tok * a.v_t + (int64_t)hk * a.v_h, left, a.v_t, a.D, lane);
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int64_t tok = p.k0 + key0 + 32 * b;
-    k[b].load(a.k + tok * a.k_t + (int64_t)hk * a.k_h, p.lk - key0 - 32 * b, a.k_t, a.D, lane);
-    v[b].load(a.v + tok * a.v_t + (int64_t)hk * a.v_h, p.lk - key0 - 32 * b, a.v_t, a.D, lane);
-#pragma unroll
-    for (int d = 0; d < ND; ++d) dk[b][d] = dv[b][d] = zero16();
-  }
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zero16();
   T tq, tg;
   tq.init(a.q_t, a.D, lane);
   tg.init(a.do_t, a.D, lane);
@@ -160,91 +168,146 @@ __global__ __launch_bounds__(256, KB == 1 ? 2 : 1) void attn_dkv_kernel(AttnBwd 
   Frags<DIM> fr;
   fr.init(base, lane);
 
-  auto load = [&](int it) {
+  auto load = [&](int it, int ring) {
     const int r = it / per, i0 = (t0 + it - r * per) * kStep, head = hk * a.rep + r;
-    const uint32_t s = base + (uint32_t)((it & 1) * 2 * T::BYTES);
+    const uint32_t s = base + (uint32_t)(ring * 2 * T::BYTES);
     tq.load(a.q + (p.q0 + i0) * a.q_t + (int64_t)head * a.q_h, p.lq - i0, s, wave);
     tg.load(a.dout + (p.q0 + i0) * a.do_t + (int64_t)head * a.do_h, p.lq - i0, s + T::BYTES, wave);
     // (a query past the last reads 0, and q = dout = 0: it adds nothing)
     if (wave < 2) {
       const float* src = (wave ? a.delta : a.lse) + (int64_t)head * a.seq.TQ + p.q0 + i0;
       const i32x4 rs = rows_rsrc((const uint16_t*)src, min(p.lq - i0, kStep), 4, 4);
-      dma4(rs, (uint32_t)lane * 4, stats + (uint32_t)(((it & 1) * 2 + wave) * kStep * 4));
+      dma4(rs, (uint32_t)lane * 4, stats + (uint32_t)((ring * 2 + wave) * kStep * 4));
     }
   };
   uint32_t own = stats + (uint32_t)((lane >> 5) * 16);   // lse of the half wave's first row
   auto step = [&](int i0) {
     constexpr uint32_t qt = 0, gt = T::BYTES;
-    const bool masked = a.causal && i0 + off < key0 + 32 * KB - 1;
+    const bool masked = a.causal && i0 + off < key0 + 31;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      bf16x8 pb[KB][2], ds[KB][2];
+      // P and dv, then dP, dS and dk; with wide heads kept in that order
+      // (sched_barrier), the fewest values at a time.  A spilled register costs
+      // more than its reload here, which waits for the DMA of the next step too
+      // (7 of them: 4416 us where 3900 us without, 2 x 8192 x 32 / 8 x 128).
+      bf16x8 e[2], es[2];
+      f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        f32x16 s = zero16(), dp = zero16();
+      for (int kk = 0; kk < NK; ++kk) s = mfma(fr.rows(qt, i, kk), k.f[kk], s);
+      if (masked) {
+        const int lim = key0 + (lane & 31) - off - i0 - 4 * (lane >> 5);   // key j sees queries from j - off on
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) s = mfma(fr.rows(qt, i, kk), k[b].f[kk], s);
-        if (masked) {
-          // key j sees queries from j - off on
-          const int lim = key0 + 32 * b + (lane & 31) - off - i0 - 4 * (lane >> 5);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? -INFINITY : s[r];
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const i32x4 lse = *(const lds_i32x4*)(lds_at(own) + (32 * i + 8 * g) * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], a.c, -__int_as_float(lse[e])));
-        }
-        pb[b][0] = round8(s, 0);
-        pb[b][1] = round8(s, 1);
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) dp = mfma(fr.rows(gt, i, kk), v[b].f[kk], dp);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const i32x4 delta = *(const lds_i32x4*)(lds_at(own) + (kStep + 32 * i + 8 * g) * 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - __int_as_float(delta[e]));
-        }
-        ds[b][0] = round8(dp, 0);
-        ds[b][1] = round8(dp, 1);
+        for (int r = 0; r < 16; ++r) s[r] = 32 * i + 8 * (r >> 2) + (r & 3) < lim ? -INFINITY : s[r];
       }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const i32x4 lse = *(const lds_i32x4*)(lds_at(own) + (32 * i + 8 * g) * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[4 * g + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + r], a.c, -__int_as_float(lse[r])));
+      }
+      e[0] = round8(s, 0);
+      e[1] = round8(s, 1);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const bf16x8 x = fr.cols(gt, d, 2 * i + u), y = fr.cols(qt, d, 2 * i + u);
+        for (int d = 0; d < ND; ++d) dv[d] = mfma(fr.cols(gt, d, 2 * i + u), e[u], dv[d]);
+      if constexpr (NK > 4) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            dv[b][d] = mfma(x, pb[b][u], dv[b][d]);
-            dk[b][d] = mfma(y, ds[b][u], dk[b][d]);
-          }
-        }
+      for (int kk = 0; kk < NK; ++kk) dp = mfma(fr.rows(gt, i, kk), v.f[kk], dp);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const i32x4 delta = *(const lds_i32x4*)(lds_at(own) + (kStep + 32 * i + 8 * g) * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dp[4 * g + r] = s[4 * g + r] * (dp[4 * g + r] - __int_as_float(delta[r]));
+      }
+      es[0] = round8(dp, 0);
+      es[1] = round8(dp, 1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dk[d] = mfma(fr.cols(qt, d, 2 * i + u), es[u], dk[d]);
+      if constexpr (NK > 4) __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (steps > 0) load(0);
-  for (int it = 0; it < steps; ++it) {
+  if (it0 < it1) load(it0, 0);
+  for (int it = it0; it < it1; ++it) {
+    const int ring = (it - it0) & 1;
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     lds_barrier();
-    if (it + 1 < steps) load(it + 1);
+    if (it + 1 < it1) load(it + 1, ring ^ 1);
     const int i0 = (t0 + it % per) * kStep;
     // (causal: where the step's last query sees none of the wave's keys there is nothing to add)
     if (!a.causal || i0 + kStep - 1 + off >= key0) step(i0);
-    const int sign = it & 1 ? -1 : 1;
+    const int sign = ring ? -1 : 1;
     fr.move(sign * 2 * T::BYTES);
     own += (uint32_t)(sign * 2 * kStep * 4);
   }
+  if constexpr (SPLIT) {
+    if ((lane & 31) >= left) return;
+    // [share][dk, dv][token][key head][D]
+    const int64_t row = (int64_t)a.rows_h * a.D, all = a.seq.TK * row;
+    float* to = a.part + (int64_t)share * 2 * all + (tok + (lane & 31)) * row + (int64_t)hk * a.D + 4 * (lane >> 5);
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int64_t tok = p.k0 + key0 + 32 * b;
-    const int left = p.lk - key0 - 32 * b;
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      store_block(a.dk + tok * a.dk_t + (int64_t)hk * a.dk_h, a.dk_t, left, a.D, d, dk[b][d], a.scale, lane);
-      store_block(a.dv + tok * a.dv_t + (int64_t)hk * a.dv_h, a.dv_t, left, a.D, d, dv[b][d], 1.0f, lane);
-    }
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g;
+        if (c >= a.D) continue;
+        *(float4*)(to + c) = make_float4(dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]);
+        *(float4*)(to + all + c) = make_float4(dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
+      }
+    return;
   }
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    store_block(a.dk + tok * a.dk_t + (int64_t)hk * a.dk_h, a.dk_t, left, a.D, d, dk[d], a.scale, lane);
+    store_block(a.dv + tok * a.dv_t + (int64_t)hk * a.dv_h, a.dv_t, left, a.D, d, dv[d], 1.0f, lane);
+  }
+}
+
+// dk and dv from the shares' sums, in their order: a thread 8 elements of a row
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a) {
+  const int64_t row = (int64_t)a.rows_h * a.D, all = a.seq.TK * row;
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;   // D is a multiple of 8
+  if (e >= all) return;
+  const int64_t tok = e / row;
+  const int in = (int)(e - tok * row), hk = in / a.D, c = in - hk * a.D;
+#pragma unroll
+  for (int what = 0; what < 2; ++what) {
+    float v[8] = {};
+    for (int s = 0; s < a.splits; ++s) {
+      const float4* p = (const float4*)(a.part + ((int64_t)s * 2 + what) * all + e);
+      const float4 x = p[0], y = p[1];
+      v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+      v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+    const float f = what ? 1.0f : a.scale;
+    uint16_t* to = what ? a.dv + tok * a.dv_t + (int64_t)hk * a.dv_h : a.dk + tok * a.dk_t + (int64_t)hk * a.dk_h;
+    *(uint4*)(to + c) = make_uint4(pack_bf16x2(v[0] * f, v[1] * f), pack_bf16x2(v[2] * f, v[3] * f),
+                                   pack_bf16x2(v[4] * f, v[5] * f), pack_bf16x2(v[6] * f, v[7] * f));
+  }
+}
+
+// Shares a key tile's steps are split into.  A launch of the key tiles alone may
+// leave CUs idle (few tiles: a short batch, few key heads) or wait for the tile
+// with the most queries (a causal mask, sequences of different lengths): up to
+// four times the workgroups that the chip holds even that out.  A share has four
+// steps at least, and the shares' sums cost 16 bytes an element, which must stay
+// below a sixth of the launch's time (products at 1 PFLOP/s on a full chip, sums
+// at 5 TB/s; lengths are not known here, so the mean stands for them).  2 x 4096
+// causal, 32 / 8 heads of 128: the whole backward 1270 us in one share, 967 us.
+static int dkv_splits(const concord_attn_args& g) {
+  if (g.TQ < 1 || g.TK < 1) return 1;
+  AttnSeqs s = attn_seqs(g);
+  const double wgs = (double)attn_slots(s, g.TK, kDkvRows) * g.HK, room = g.D <= 64 ? 768.0 : 512.0;
+  const double per_seq = (double)g.TQ / (double)std::max<int64_t>(g.B, 1) * (g.causal ? 0.5 : 1.0);
+  const double steps = per_seq / kStep * (g.H / g.HK);
+  const double time = 8.0 * g.TK * per_seq * g.H * g.D / 1e15 * std::max(1.0, room / wgs);
+  const double share = 16.0 * g.TK * g.HK * g.D / 5e12;
+  double n = (g.causal || g.starts ? 4.0 : 1.0) * room / wgs;
+  n = std::min(std::min(n, steps / 4.0), time / 6.0 / share);
+  return n < 2.0 ? 1 : n < 16.0 ? (int)n : 16;
 }
 
 }  // namespace concord
@@ -252,8 +315,10 @@ __global__ __launch_bounds__(256, KB == 1 ? 2 : 1) void attn_dkv_kernel(AttnBwd 
 using namespace concord;
 
 extern "C" size_t concord_attention_workspace_bytes(const concord_attn_args* args) {
-  if (!args || args->TQ < 1 || args->H < 1) return 0;
-  return (size_t)args->TQ * (size_t)args->H * sizeof(float);   // delta
+  if (!args || args->TQ < 1 || args->H < 1 || args->HK < 1 || args->D < 8) return 0;
+  const int n = dkv_splits(*args);
+  const size_t delta = ((size_t)args->TQ * (size_t)args->H * sizeof(float) + 255) / 256 * 256;
+  return delta + (n > 1 ? (size_t)n * 2 * (size_t)args->TK * (size_t)args->HK * (size_t)args->D * sizeof(float) : 0);
 }
 
 extern "C" int concord_attention_bwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes,
@@ -291,14 +356,20 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
     });
   }
   if (g.TK > 0) {
-    constexpr int KB = 1;
-    const int64_t slots = attn_slots(a.seq, g.TK, 128 * KB);
-    CONCORD_CHECK(slots * g.HK < (1LL << 31), "%s: too many tiles", what);
+    a.splits = dkv_splits(g);
+    a.rows_h = g.HK;
+    a.part = (float*)((char*)workspace + ((size_t)g.TQ * (size_t)g.H * sizeof(float) + 255) / 256 * 256);
+    const int64_t slots = attn_slots(a.seq, g.TK, kDkvRows);
+    CONCORD_CHECK(slots * g.HK * a.splits < (1LL << 31), "%s: too many tiles", what);
     a.slots = (int32_t)slots;
+    const dim3 grid((unsigned)(slots * g.HK * a.splits));
     attn_by_dim(g.D, [&](auto nk) {
-      hipLaunchKernelGGL((attn_dkv_kernel<decltype(nk)::value, KB>), dim3((unsigned)(slots * g.HK)), dim3(256), 0, st,
-                         a);
+      constexpr int NK = decltype(nk)::value;
+      if (a.splits > 1) hipLaunchKernelGGL((attn_dkv_kernel<NK, true>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((attn_dkv_kernel<NK, false>), grid, dim3(256), 0, st, a);
     });
+    if (a.splits > 1)
+      hipLaunchKernelGGL(attn_dkv_sum_kernel, dim3((unsigned)cdiv(g.TK * g.HK * g.D, 2048)), dim3(256), 0, st, a);
   }
   return launch_status("attention_bwd");
 }

@@ -345,7 +345,7 @@ def test_attention_tokens_outside_the_sequences():
     qd, kd, vd = (t.to(DEV).requires_grad_(True) for t in (q, k, v))
     out = ca.attention(qd, kd, vd, starts=_i32([37, 100, 250]))
     grads = torch.autograd.grad(out, (qd, kd, vd), g.to(DEV))
-    for t in (out, *grads):
+    for t in (out.detach(), *grads):
         assert float(t[:37].abs().sum()) == 0.0 and float(t[250:].abs().sum()) == 0.0
     ref = _attn_ref(*(t[37:250].double() for t in (q, k, v, g)), [0, 63, 213], [0, 63, 213], True, 0.125)
     for name, got in (("out", out), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
@@ -385,6 +385,28 @@ def test_attention_score_ranges(spread):
     k = (k.float() * torch.linspace(0.2, 2.0, 260)[:, None, None]).to(torch.bfloat16)
     _attn_check(q, k, v, g)
     _attn_check(q, k.flip(0), v, g, causal=False)
+
+
+@pytest.mark.parametrize("tq,tk,h,hk,d,causal", [
+    (2048, 2048, 4, 1, 64, True), (1500, 1500, 8, 2, 128, True), (1200, 333, 2, 1, 64, False),
+    (900, 900, 6, 2, 96, True), (1000, 1500, 2, 1, 128, False)])
+def test_attention_few_tiles(tq, tk, h, hk, d, causal):
+    """Too few tiles to fill the chip: the work along the long axis is split and
+    joined (backward: dk and dv over the queries)."""
+    q, k, v, g = _attn_inputs(tq, tk, h, hk, d)
+    _attn_check(q, k, v, g, causal=causal, tables=False)
+    if tq == tk:
+        _attn_check(q, k, v, g, starts=[0, 3, 3, 700, tq], causal=causal)
+
+
+@pytest.mark.parametrize("tq,tk,h,hk,d,causal", [
+    (1, 5000, 4, 1, 64, True), (1, 4097, 8, 2, 128, False), (40, 3000, 2, 2, 96, True), (130, 2500, 2, 1, 128, True),
+    (200, 1700, 1, 1, 32, False)])
+def test_attention_few_queries(tq, tk, h, hk, d, causal):
+    """Few queries of many keys: the keys are split and joined."""
+    q, k, v, g = _attn_inputs(tq, tk, h, hk, d)
+    _attn_check(q, k, v, g, causal=causal)
+    _attn_check(q, k, v, g, starts=[0, 0, tq // 2, tq, tq], k_starts=[0, 1, 1200, tk - 1, tk], causal=causal)
 
 
 def test_attention_scale():
