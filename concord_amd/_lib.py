@@ -149,7 +149,8 @@ _SIGS = {
                                            _P]),
     "concord_distill_bwd": (ctypes.c_int, [_P, _I, _P, _I, ctypes.c_int, _I, _I, _P, _I, _P, _I, _i, _F, _P, _P, _I,
                                            _P]),
-    "concord_attention_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P]),
+    "concord_attention_fwd_workspace_bytes": (_Z, [ctypes.POINTER(AttnArgs)]),
+    "concord_attention_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P, _Z, _P]),
     "concord_attention_workspace_bytes": (_Z, [ctypes.POINTER(AttnArgs)]),
     "concord_attention_bwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P, _Z, _P]),
 }

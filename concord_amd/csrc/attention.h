@@ -299,6 +299,21 @@ CONCORD_DEV void store_block(uint16_t* p, int64_t ld, int left, int D, int d, co
   }
 }
 
+// a lane's values of a transposed result (ND blocks), unrounded, to its token's
+// row of D floats
+template <int ND>
+CONCORD_DEV void store_sums(float* row, const f32x16 (&v)[ND], int D, int lane) {
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g;
+      if (c < D)
+        *(float4*)(row + c + 4 * (lane >> 5)) =
+            make_float4(v[d][4 * g], v[d][4 * g + 1], v[d][4 * g + 2], v[d][4 * g + 3]);
+    }
+}
+
 // ---- sequences -------------------------------------------------------------------
 struct AttnSeqs {
   const int32_t *starts, *k_starts;   // NULL: B sequences of equal length
@@ -430,6 +445,23 @@ inline void attn_by_dim(int D, F&& f) {
   else if (D <= 64) f(std::integral_constant<int, 4>());
   else if (D <= 96) f(std::integral_constant<int, 6>());
   else f(std::integral_constant<int, 8>());
+}
+
+// Shares the keys of a tile of 128 queries are split into (forward and dq; `flops`
+// per query-key pair and dimension): where the tiles alone leave CUs idle, as
+// many as fill the chip with two (four with heads up to 64) workgroups a CU, of
+// four steps of 64 keys at least, while the shares' sums (8 bytes an element)
+// stay below a sixth of the launch's time as above (dkv_splits).  One query of
+// 32768 keys, 32 / 8 heads of 128: SPLIT.
+inline int key_splits(const concord_attn_args& g, double flops) {
+  if (g.TQ < 1 || g.TK < 1) return 1;
+  AttnSeqs s = attn_seqs(g);
+  const double wgs = (double)attn_slots(s, g.TQ, 128) * g.H, room = g.D <= 64 ? 1024.0 : 512.0;
+  const double keys = (double)g.TK / (double)std::max<int64_t>(g.B, 1);
+  const double time = flops * g.TQ * keys * g.H * g.D / 1e15 * std::max(1.0, room / wgs);
+  const double share = 8.0 * g.TQ * g.H * g.D / 5e12;
+  const double n = std::min(std::min(room / wgs, keys / 256.0), time / 6.0 / share);
+  return n < 2.0 ? 1 : n < 64.0 ? (int)n : 64;
 }
 
 }  // namespace concord

@@ -19,15 +19,18 @@ struct AttnFwd {
   int64_t o_t, o_h;
   float* lse;
   int8_t* low;
+  float* part;      // split keys: [share][token][head][D] sums, then [share][token][head] (m, l)
   AttnSeqs seq;
-  int32_t slots, rep, D, causal, heads;   // rep: query heads of a key head
+  int32_t slots, rep, D, causal, heads, splits;   // rep: query heads of a key head
   float c;                         // scale log2(e)
 };
 
 constexpr int kAttnQ = 128;   // queries of a workgroup
 constexpr int kAttnK = 64;    // keys of a step
 
-template <int NK>
+// SPLIT: a workgroup takes one of `splits` equal shares of the key tiles and
+// leaves its sums, unnormalised, with their m and l for attn_join_kernel.
+template <int NK, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   typedef Dim<NK> DIM;
   typedef Tile<DIM, kAttnK, 4> T;
@@ -35,11 +38,15 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   constexpr bool PIPE = NK > 4;
   __shared__ __attribute__((aligned(1024))) char lds[4 * T::BYTES];   // two slots of k and v
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lin = attn_xcd(blockIdx.x, gridDim.x);
+  int lin = attn_xcd(blockIdx.x, gridDim.x), share = 0;
+  if (SPLIT) {
+    share = lin % a.splits;
+    lin /= a.splits;
+  }
   const int per = a.rep * a.slots;
   const int hk = lin / per, in = lin - hk * per;
   const int slot = a.slots - 1 - in / a.rep, head = hk * a.rep + in % a.rep;
-  const AttnPlace p = attn_place<kAttnQ, false>(a.seq, slot);
+  AttnPlace p = attn_place<kAttnQ, false>(a.seq, slot);
   if (p.first < 0 || p.first >= p.lq) return;
 
   const int row0 = p.first + wave * 32;                  // the wave's first query
@@ -48,12 +55,21 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   // keys of the workgroup's last query
   const int last = min(p.first + kAttnQ, p.lq) - 1;
   const int keys = a.causal ? max(0, min(p.lk, last + off + 1)) : p.lk;
-  const int tiles = (keys + kAttnK - 1) / kAttnK;
+  int tiles = (keys + kAttnK - 1) / kAttnK;
   // the lane's last key, and the wave's first and last queries' last keys
   const int qi = row0 + (lane & 31);
-  const int jmax = a.causal ? min(p.lk - 1, qi + off) : p.lk - 1;
-  const int jlo = a.causal ? min(p.lk - 1, row0 + off) : p.lk - 1;
-  const int jhi = a.causal ? min(p.lk - 1, row0 + 31 + off) : p.lk - 1;
+  int jmax = a.causal ? min(p.lk - 1, qi + off) : p.lk - 1;
+  int jlo = a.causal ? min(p.lk - 1, row0 + off) : p.lk - 1;
+  int jhi = a.causal ? min(p.lk - 1, row0 + 31 + off) : p.lk - 1;
+  if (SPLIT) {   // keys count from the share's first
+    const int t0 = (int)((int64_t)tiles * share / a.splits), j0 = t0 * kAttnK;
+    tiles = (int)((int64_t)tiles * (share + 1) / a.splits) - t0;
+    p.k0 += j0;
+    p.lk -= j0;
+    jmax -= j0;
+    jlo -= j0;
+    jhi -= j0;
+  }
 
   Fixed<DIM> q;
   q.load(a.q + (p.q0 + row0) * a.q_t + (int64_t)head * a.q_h, rows, a.q_t, a.D, lane);
@@ -240,6 +256,14 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
 
   const Halves both = halves(l);
   l = both.lo + both.hi;
+  if constexpr (SPLIT) {
+    if ((lane & 31) >= rows) return;
+    const int64_t row = (p.q0 + qi) * a.heads + head, all = a.seq.TQ * a.heads;
+    store_sums(a.part + ((int64_t)share * all + row) * a.D, o, a.D, lane);
+    if (lane < 32)
+      *(float2*)(a.part + (int64_t)a.splits * all * a.D + ((int64_t)share * all + row) * 2) = make_float2(m, l);
+    return;
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = a.out + (p.q0 + row0) * a.o_t + (int64_t)head * a.o_h;
   const int64_t low_t = (int64_t)a.heads * a.D;
@@ -250,29 +274,80 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
     a.lse[(int64_t)head * a.seq.TQ + p.q0 + qi] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+// out, lse and out_low of split keys: a thread 8 elements of a row
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
+  const int64_t all = a.seq.TQ * a.heads, e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= all * a.D) return;
+  const int64_t row = e / a.D, tok = row / a.heads;
+  const int c = (int)(e - row * a.D), head = (int)(row - tok * a.heads);
+  const float2* ml = (const float2*)(a.part + (int64_t)a.splits * all * a.D);
+  float m = -3.4028235e38f, l = 0.0f, v[8] = {};
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(int64_t)s * all + row].x);
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 x = ml[(int64_t)s * all + row];
+    const float f = __builtin_amdgcn_exp2f(x.x - m);   // (a share without keys has l = 0 and sums of 0)
+    l = __builtin_fmaf(x.y, f, l);
+    const float4* p = (const float4*)(a.part + ((int64_t)s * all + row) * a.D + c);
+    const float4 y = p[0], z = p[1];
+    const float w[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(w[i], f, v[i]);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint32_t hi[4], lo[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = v[2 * i] * inv, y = v[2 * i + 1] * inv;
+    hi[i] = pack_bf16x2(x, y);
+    lo[i >> 1] |= (uint32_t)(left_over(x, hi[i] & 0xFFFF) | left_over(y, hi[i] >> 16) << 8) << (16 * (i & 1));
+  }
+  *(uint4*)(a.out + tok * a.o_t + (int64_t)head * a.o_h + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  if (a.low) *(uint2*)(a.low + e) = make_uint2(lo[0], lo[1]);
+  if (a.lse && c == 0) a.lse[(int64_t)head * a.seq.TQ + tok] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
 }  // namespace concord
 
 using namespace concord;
 
-extern "C" int concord_attention_fwd(const concord_attn_args* args, void* stream) {
+extern "C" size_t concord_attention_fwd_workspace_bytes(const concord_attn_args* args) {
+  if (!args || args->TQ < 1 || args->H < 1 || args->HK < 1 || args->D < 8) return 0;
+  const int n = key_splits(*args, 4.0);
+  return n > 1 ? (size_t)n * (size_t)args->TQ * (size_t)args->H * (size_t)(args->D + 2) * sizeof(float) : 0;
+}
+
+extern "C" int concord_attention_fwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
   CONCORD_CHECK(args, "concord_attention_fwd: NULL argument");
   const concord_attn_args& g = *args;
   if (const int rc = attn_check("concord_attention_fwd", g)) return rc;
   CONCORD_CHECK(!g.lse == !g.out_low && ((uintptr_t)g.out_low & 15) == 0,
                 "concord_attention_fwd: lse and out_low come together, out_low on 16 bytes");
   if (g.TQ == 0) return CONCORD_OK;
+  const size_t need = concord_attention_fwd_workspace_bytes(args);
+  if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) {
+    set_error("concord_attention_fwd: workspace of %zu bytes on 16 needed", need);
+    return CONCORD_EWORKSPACE;
+  }
   AttnFwd a{};
+  a.splits = key_splits(g, 4.0);
+  a.part = (float*)workspace;
   a.q = g.q, a.k = g.k, a.v = g.v, a.out = g.out, a.lse = g.lse, a.low = g.out_low, a.heads = g.H;
   a.q_t = g.q_t, a.q_h = g.q_h, a.k_t = g.k_t, a.k_h = g.k_h, a.v_t = g.v_t, a.v_h = g.v_h;
   a.o_t = g.o_t, a.o_h = g.o_h;
   a.seq = attn_seqs(g);
   const int64_t slots = attn_slots(a.seq, g.TQ, kAttnQ);
-  CONCORD_CHECK(slots * g.H < (1LL << 31), "concord_attention_fwd: too many tiles");
+  CONCORD_CHECK(slots * g.H * a.splits < (1LL << 31), "concord_attention_fwd: too many tiles");
   a.slots = (int32_t)slots;
   a.rep = g.H / g.HK, a.D = g.D, a.causal = g.causal != 0, a.c = g.scale * kLog2e;
-  const dim3 grid((unsigned)(slots * g.H));
+  const dim3 grid((unsigned)(slots * g.H * a.splits));
+  hipStream_t st = (hipStream_t)stream;
   attn_by_dim(g.D, [&](auto nk) {
-    hipLaunchKernelGGL((attn_fwd_kernel<decltype(nk)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    constexpr int NK = decltype(nk)::value;
+    if (a.splits > 1) hipLaunchKernelGGL((attn_fwd_kernel<NK, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_fwd_kernel<NK, false>), grid, dim3(256), 0, st, a);
   });
+  if (a.splits > 1)
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)cdiv(g.TQ * g.H * g.D, 2048)), dim3(256), 0, st, a);
   return launch_status("attention_fwd");
 }

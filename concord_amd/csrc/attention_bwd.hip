@@ -20,7 +20,7 @@ struct AttnBwd {
   const float* lse;
   const int8_t* low;
   float* delta;
-  float* part;      // split dk and dv
+  float* part;      // the shares' sums
   AttnSeqs seq;
   int32_t slots, rep, D, causal, heads, rows_h, splits;   // rows_h: key heads
   float c, scale;
@@ -31,28 +31,42 @@ constexpr int kStep = 64;      // keys (queries) of a step
 
 // dq and delta: the forward's shape.  A lane holds one query's column of the
 // transposed scores, so lse and delta are lane-local.
-template <int NK>
+// SPLIT: a share of the key tiles, as in the forward; fp32 sums.
+template <int NK, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
   typedef Dim<NK> DIM;
   typedef Tile<DIM, kStep, 4> T;
   constexpr int ND = DIM::ND;
   __shared__ __attribute__((aligned(1024))) char lds[4 * T::BYTES];   // two slots of k and v
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lin = attn_xcd(blockIdx.x, gridDim.x);
+  int lin = attn_xcd(blockIdx.x, gridDim.x), share = 0;
+  if (SPLIT) {
+    share = lin % a.splits;
+    lin /= a.splits;
+  }
   const int per = a.rep * a.slots;
   const int hk = lin / per, in = lin - hk * per;
   const int slot = a.slots - 1 - in / a.rep, head = hk * a.rep + in % a.rep;
-  const AttnPlace p = attn_place<kDqRows, false>(a.seq, slot);
+  AttnPlace p = attn_place<kDqRows, false>(a.seq, slot);
   if (p.first < 0 || p.first >= p.lq) return;
 
   const int row0 = p.first + wave * 32, rows = p.lq - row0, off = p.lk - p.lq;
   const int last = min(p.first + kDqRows, p.lq) - 1;
   const int keys = a.causal ? max(0, min(p.lk, last + off + 1)) : p.lk;
-  const int tiles = (keys + kStep - 1) / kStep;
+  int tiles = (keys + kStep - 1) / kStep;
   const int qi = row0 + (lane & 31);
-  const int jmax = a.causal ? min(p.lk - 1, qi + off) : p.lk - 1;
-  const int jlo = a.causal ? min(p.lk - 1, row0 + off) : p.lk - 1;
-  const int jhi = a.causal ? min(p.lk - 1, row0 + 31 + off) : p.lk - 1;
+  int jmax = a.causal ? min(p.lk - 1, qi + off) : p.lk - 1;
+  int jlo = a.causal ? min(p.lk - 1, row0 + off) : p.lk - 1;
+  int jhi = a.causal ? min(p.lk - 1, row0 + 31 + off) : p.lk - 1;
+  if (SPLIT) {   // keys count from the share's first
+    const int t0 = (int)((int64_t)tiles * share / a.splits), j0 = t0 * kStep;
+    tiles = (int)((int64_t)tiles * (share + 1) / a.splits) - t0;
+    p.k0 += j0;
+    p.lk -= j0;
+    jmax -= j0;
+    jlo -= j0;
+    jhi -= j0;
+  }
 
   Fixed<DIM> q, g;
   q.load(a.q + (p.q0 + row0) * a.q_t + (int64_t)head * a.q_h, rows, a.q_t, a.D, lane);
@@ -65,7 +79,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
     o.load(a.out + (p.q0 + row0) * a.o_t + (int64_t)head * a.o_h, rows, a.o_t, a.D, lane);
     const int64_t low_t = (int64_t)a.heads * a.D;
     delta = row_dot(o, a.low + (p.q0 + row0) * low_t + (int64_t)head * a.D, rows, low_t, a.D, g, lane);
-    if (lane < 32 && qi < p.lq) a.delta[at] = delta;
+    if (share == 0 && lane < 32 && qi < p.lq) a.delta[at] = delta;
   }
   const uint16_t* kp = a.k + p.k0 * a.k_t + (int64_t)hk * a.k_h;
   const uint16_t* vp = a.v + p.k0 * a.v_t + (int64_t)hk * a.v_h;
@@ -117,6 +131,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
     if (t * kStep <= jhi) step(t * kStep);
     fr.move(t & 1 ? -2 * T::BYTES : 2 * T::BYTES);
   }
+  if constexpr (SPLIT) {
+    if ((lane & 31) < rows)
+      store_sums(a.part + (((int64_t)share * a.seq.TQ + p.q0 + qi) * a.heads + head) * a.D, dq, a.D, lane);
+    return;
+  }
   uint16_t* out = a.dq + (p.q0 + row0) * a.dq_t + (int64_t)head * a.dq_h;
 #pragma unroll
   for (int d = 0; d < ND; ++d) store_block(out, a.dq_t, rows, a.D, d, dq[d], a.scale, lane);
@@ -127,7 +146,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnBwd a) {
 // dk^T += q^T dS as they come.  lse and delta of a step's queries lie in LDS.
 //
 // SPLIT: a workgroup takes one of `splits` equal shares of the steps and leaves
-// fp32 sums for attn_dkv_sum_kernel.
+// fp32 sums for attn_sum_kernel.
 template <int NK, bool SPLIT>
 __global__ __launch_bounds__(256, NK <= 4 ? 3 : 2) void attn_dkv_kernel(AttnBwd a) {
   typedef Dim<NK> DIM;
@@ -247,16 +266,9 @@ __global__ __launch_bounds__(256, NK <= 4 ? 3 : 2) void attn_dkv_kernel(AttnBwd 
     if ((lane & 31) >= left) return;
     // [share][dk, dv][token][key head][D]
     const int64_t row = (int64_t)a.rows_h * a.D, all = a.seq.TK * row;
-    float* to = a.part + (int64_t)share * 2 * all + (tok + (lane & 31)) * row + (int64_t)hk * a.D + 4 * (lane >> 5);
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 32 * d + 8 * g;
-        if (c >= a.D) continue;
-        *(float4*)(to + c) = make_float4(dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]);
-        *(float4*)(to + all + c) = make_float4(dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
-      }
+    float* to = a.part + (int64_t)share * 2 * all + (tok + (lane & 31)) * row + (int64_t)hk * a.D;
+    store_sums(to, dk, a.D, lane);
+    store_sums(to + all, dv, a.D, lane);
     return;
   }
 #pragma unroll
@@ -266,26 +278,35 @@ __global__ __launch_bounds__(256, NK <= 4 ? 3 : 2) void attn_dkv_kernel(AttnBwd 
   }
 }
 
-// dk and dv from the shares' sums, in their order: a thread 8 elements of a row
-__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a) {
-  const int64_t row = (int64_t)a.rows_h * a.D, all = a.seq.TK * row;
+// Shares' sums added in their order, a thread 8 elements of a row: N outputs of
+// tokens x heads x D, part [share][N][token][head][D]
+struct AttnSum {
+  const float* part;
+  int64_t all;       // elements of an output
+  int32_t splits, heads, D;
+  uint16_t* to[2];
+  int64_t t[2], h[2];
+  float scale[2];
+};
+template <int N>
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnSum a) {
   const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;   // D is a multiple of 8
-  if (e >= all) return;
-  const int64_t tok = e / row;
-  const int in = (int)(e - tok * row), hk = in / a.D, c = in - hk * a.D;
+  if (e >= a.all) return;
+  const int64_t row = e / a.D, tok = row / a.heads;
+  const int c = (int)(e - row * a.D), head = (int)(row - tok * a.heads);
 #pragma unroll
-  for (int what = 0; what < 2; ++what) {
+  for (int n = 0; n < N; ++n) {
     float v[8] = {};
     for (int s = 0; s < a.splits; ++s) {
-      const float4* p = (const float4*)(a.part + ((int64_t)s * 2 + what) * all + e);
+      const float4* p = (const float4*)(a.part + ((int64_t)s * N + n) * a.all + e);
       const float4 x = p[0], y = p[1];
       v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
       v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
     }
-    const float f = what ? 1.0f : a.scale;
-    uint16_t* to = what ? a.dv + tok * a.dv_t + (int64_t)hk * a.dv_h : a.dk + tok * a.dk_t + (int64_t)hk * a.dk_h;
-    *(uint4*)(to + c) = make_uint4(pack_bf16x2(v[0] * f, v[1] * f), pack_bf16x2(v[2] * f, v[3] * f),
-                                   pack_bf16x2(v[4] * f, v[5] * f), pack_bf16x2(v[6] * f, v[7] * f));
+    const float f = a.scale[n];
+    *(uint4*)(a.to[n] + tok * a.t[n] + (int64_t)head * a.h[n] + c) =
+        make_uint4(pack_bf16x2(v[0] * f, v[1] * f), pack_bf16x2(v[2] * f, v[3] * f),
+                   pack_bf16x2(v[4] * f, v[5] * f), pack_bf16x2(v[6] * f, v[7] * f));
   }
 }
 
@@ -310,15 +331,21 @@ static int dkv_splits(const concord_attn_args& g) {
   return n < 2.0 ? 1 : n < 16.0 ? (int)n : 16;
 }
 
+// the workspace: delta, then the shares' sums
+static size_t delta_bytes(const concord_attn_args& g) {
+  return ((size_t)g.TQ * (size_t)g.H * sizeof(float) + 255) / 256 * 256;
+}
+
 }  // namespace concord
 
 using namespace concord;
 
 extern "C" size_t concord_attention_workspace_bytes(const concord_attn_args* args) {
   if (!args || args->TQ < 1 || args->H < 1 || args->HK < 1 || args->D < 8) return 0;
-  const int n = dkv_splits(*args);
-  const size_t delta = ((size_t)args->TQ * (size_t)args->H * sizeof(float) + 255) / 256 * 256;
-  return delta + (n > 1 ? (size_t)n * 2 * (size_t)args->TK * (size_t)args->HK * (size_t)args->D * sizeof(float) : 0);
+  const size_t n = dkv_splits(*args), m = key_splits(*args, 6.0);
+  const size_t dkv = n > 1 ? n * 2 * (size_t)args->TK * (size_t)args->HK : 0;
+  const size_t dq = m > 1 ? m * (size_t)args->TQ * (size_t)args->H : 0;
+  return delta_bytes(*args) + std::max(dkv, dq) * (size_t)args->D * sizeof(float);   // (one after the other)
 }
 
 extern "C" int concord_attention_bwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes,
@@ -334,8 +361,8 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
                 "%s: lse or out_low is NULL or misaligned", what);
   if (g.TQ == 0 && g.TK == 0) return CONCORD_OK;
   const size_t need = concord_attention_workspace_bytes(args);
-  if (need && (!workspace || workspace_bytes < need)) {
-    set_error("%s: workspace of %zu bytes needed", what, need);
+  if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) {
+    set_error("%s: workspace of %zu bytes on 16 needed", what, need);
     return CONCORD_EWORKSPACE;
   }
   AttnBwd a{};
@@ -346,30 +373,45 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
   a.lse = g.lse, a.low = g.out_low, a.heads = g.H, a.delta = (float*)workspace;
   a.rep = g.H / g.HK, a.D = g.D, a.causal = g.causal != 0, a.c = g.scale * kLog2e, a.scale = g.scale;
   a.seq = attn_seqs(g);
+  a.part = (float*)((char*)workspace + delta_bytes(g));
   hipStream_t st = (hipStream_t)stream;
+  AttnSum sum{};
+  sum.part = a.part, sum.D = g.D;
   if (g.TQ > 0) {
+    a.splits = key_splits(g, 6.0);
     const int64_t slots = attn_slots(a.seq, g.TQ, kDqRows);
-    CONCORD_CHECK(slots * g.H < (1LL << 31), "%s: too many tiles", what);
+    CONCORD_CHECK(slots * g.H * a.splits < (1LL << 31), "%s: too many tiles", what);
     a.slots = (int32_t)slots;
+    const dim3 grid((unsigned)(slots * g.H * a.splits));
     attn_by_dim(g.D, [&](auto nk) {
-      hipLaunchKernelGGL((attn_dq_kernel<decltype(nk)::value>), dim3((unsigned)(slots * g.H)), dim3(256), 0, st, a);
+      constexpr int NK = decltype(nk)::value;
+      if (a.splits > 1) hipLaunchKernelGGL((attn_dq_kernel<NK, true>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((attn_dq_kernel<NK, false>), grid, dim3(256), 0, st, a);
     });
+    if (a.splits > 1) {
+      sum.all = g.TQ * g.H * g.D, sum.splits = a.splits, sum.heads = g.H;
+      sum.to[0] = g.dq, sum.t[0] = g.dq_t, sum.h[0] = g.dq_h, sum.scale[0] = g.scale;
+      hipLaunchKernelGGL((attn_sum_kernel<1>), dim3((unsigned)cdiv(sum.all, 2048)), dim3(256), 0, st, sum);
+    }
   }
   if (g.TK > 0) {
     a.splits = dkv_splits(g);
-    a.rows_h = g.HK;
-    a.part = (float*)((char*)workspace + ((size_t)g.TQ * (size_t)g.H * sizeof(float) + 255) / 256 * 256);
     const int64_t slots = attn_slots(a.seq, g.TK, kDkvRows);
     CONCORD_CHECK(slots * g.HK * a.splits < (1LL << 31), "%s: too many tiles", what);
     a.slots = (int32_t)slots;
+    a.rows_h = g.HK;
     const dim3 grid((unsigned)(slots * g.HK * a.splits));
     attn_by_dim(g.D, [&](auto nk) {
       constexpr int NK = decltype(nk)::value;
       if (a.splits > 1) hipLaunchKernelGGL((attn_dkv_kernel<NK, true>), grid, dim3(256), 0, st, a);
       else hipLaunchKernelGGL((attn_dkv_kernel<NK, false>), grid, dim3(256), 0, st, a);
     });
-    if (a.splits > 1)
-      hipLaunchKernelGGL(attn_dkv_sum_kernel, dim3((unsigned)cdiv(g.TK * g.HK * g.D, 2048)), dim3(256), 0, st, a);
+    if (a.splits > 1) {
+      sum.all = g.TK * g.HK * g.D, sum.splits = a.splits, sum.heads = g.HK;
+      sum.to[0] = g.dk, sum.t[0] = g.dk_t, sum.h[0] = g.dk_h, sum.scale[0] = g.scale;
+      sum.to[1] = g.dv, sum.t[1] = g.dv_t, sum.h[1] = g.dv_h, sum.scale[1] = 1.0f;
+      hipLaunchKernelGGL((attn_sum_kernel<2>), dim3((unsigned)cdiv(sum.all, 2048)), dim3(256), 0, st, sum);
+    }
   }
   return launch_status("attention_bwd");
 }

@@ -243,6 +243,12 @@ concord_attn_args attn_args(const Operand& q, const Operand& k, const Operand& v
   return a;
 }
 
+void attn_forward(const concord_attn_args& a, const Tensor& q) {
+  const size_t need = concord_attention_fwd_workspace_bytes(&a);
+  const Tensor ws = need ? bytes(need, q) : Tensor();
+  check(concord_attention_fwd(&a, ptr(ws), need, stream_of(q)), kAttn);
+}
+
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const MaybeTensor& starts_, const MaybeTensor& k_starts_, bool causal, double scale) {
@@ -252,7 +258,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     Tensor lse = at::empty({q.numel() / q.size(-1)}, q.options().dtype(at::kFloat));
     Tensor low = at::empty(q.sizes(), q.options().dtype(at::kChar));
     const concord_attn_args a = attn_args(oq, ok, ov, out, lse, low, starts, k_starts, causal, scale);
-    check(concord_attention_fwd(&a, stream_of(q)), kAttn);
+    attn_forward(a, q);
     ctx->save_for_backward({oq.t, ok.t, ov.t, out, lse, low, starts, k_starts});
     ctx->saved_data["strides"] = std::vector<int64_t>{oq.token, oq.head, ok.token, ok.head, ov.token, ov.head};
     ctx->saved_data["causal"] = causal;
@@ -293,7 +299,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeT
   Tensor out = at::empty(q.sizes(), q.options());
   const concord_attn_args a =
       attn_args(operand(q), operand(k), operand(v), out, Tensor(), Tensor(), starts, k_starts, causal, scale);
-  check(concord_attention_fwd(&a, stream_of(q)), kAttn);
+  attn_forward(a, q);
   return out;
 }
 

@@ -586,10 +586,14 @@ typedef struct concord_attn_args {
   uint16_t *dq, *dk, *dv;
   int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
 } concord_attn_args;
-int concord_attention_fwd(const concord_attn_args* args, void* stream);
+/* workspace: concord_attention_fwd_workspace_bytes(args) bytes on 16 (0: none
+ * needed; it holds the sums of few queries' shares of long keys); it need not
+ * be zeroed. */
+size_t concord_attention_fwd_workspace_bytes(const concord_attn_args* args);
+int concord_attention_fwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* dq, dk, dv from dout, the forward's out, lse and out_low; dk and dv summed over the
  * query heads of a group.  Every sum has a fixed order.  workspace:
- * concord_attention_workspace_bytes(args) bytes; it need not be zeroed. */
+ * concord_attention_workspace_bytes(args) bytes on 16; it need not be zeroed. */
 size_t concord_attention_workspace_bytes(const concord_attn_args* args);
 int concord_attention_bwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 

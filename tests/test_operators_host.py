@@ -129,17 +129,23 @@ def test_attention_entry_refusals(L):
            dict(k_t=68), dict(v_h=4), dict(q_t=1 << 24), dict(k_starts=1)]
     for kw in bad:
         a = _attn_args(buf, **kw)
-        assert L.concord_attention_fwd(ctypes.byref(a), None) == C.EINVAL, kw
+        assert L.concord_attention_fwd(ctypes.byref(a), None, 0, None) == C.EINVAL, kw
         assert L.concord_attention_bwd(ctypes.byref(a), buf, 64, None) == C.EINVAL, kw
     for kw in (dict(dout=None), dict(dk=8), dict(dv_t=12), dict(lse=None), dict(out_low=None)):
         assert L.concord_attention_bwd(ctypes.byref(_attn_args(buf, **kw)), buf, 64, None) == C.EINVAL, kw
     a = _attn_args(buf)
     need = L.concord_attention_workspace_bytes(ctypes.byref(a))
     assert L.concord_attention_bwd(ctypes.byref(a), buf, need - 1, None) == C.EWORKSPACE
-    assert L.concord_attention_fwd(None, None) == C.EINVAL
+    assert L.concord_attention_fwd(None, None, 0, None) == C.EINVAL
+    # one query of many keys: the forward needs room for its shares' sums
+    long = _attn_args(buf, TQ=1, TK=32768)
+    need = L.concord_attention_fwd_workspace_bytes(ctypes.byref(long))
+    assert need > 0 and L.concord_attention_fwd_workspace_bytes(ctypes.byref(a)) == 0
+    assert L.concord_attention_fwd(ctypes.byref(long), None, 0, None) == C.EWORKSPACE
+    assert L.concord_attention_fwd(ctypes.byref(long), buf, need - 1, None) == C.EWORKSPACE
     # no token: nothing to do
     empty = _attn_args(buf, TQ=0, TK=0, B=0)
-    assert L.concord_attention_fwd(ctypes.byref(empty), None) == C.OK
+    assert L.concord_attention_fwd(ctypes.byref(empty), None, 0, None) == C.OK
     assert L.concord_attention_bwd(ctypes.byref(empty), None, 0, None) == C.OK
 
 
