@@ -56,17 +56,16 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   const int last = min(p.first + kAttnQ, p.lq) - 1;
   const int keys = a.causal ? max(0, min(p.lk, last + off + 1)) : p.lk;
   int tiles = (keys + kAttnK - 1) / kAttnK;
-  // the lane's last key, and the wave's first and last queries' last keys
+  // the wave's first and last queries' last keys
   const int qi = row0 + (lane & 31);
-  int jmax = a.causal ? min(p.lk - 1, qi + off) : p.lk - 1;
-  int jlo = a.causal ? min(p.lk - 1, row0 + off) : p.lk - 1;
+  int jlo_raw = row0 + off, jlo = a.causal ? min(p.lk - 1, jlo_raw) : p.lk - 1;
   int jhi = a.causal ? min(p.lk - 1, row0 + 31 + off) : p.lk - 1;
   if (SPLIT) {   // keys count from the share's first
     const int t0 = (int)((int64_t)tiles * share / a.splits), j0 = t0 * kAttnK;
     tiles = (int)((int64_t)tiles * (share + 1) / a.splits) - t0;
     p.k0 += j0;
     p.lk -= j0;
-    jmax -= j0;
+    jlo_raw -= j0;
     jlo -= j0;
     jhi -= j0;
   }
@@ -104,7 +103,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   auto settle = [&](int t, f32x16 (&s)[2], float mx) CONCORD_INLINE_LAMBDA {
     const int j0 = t * kAttnK;
     if (j0 + kAttnK - 1 > jlo) {
-      const int lim = jmax - j0 - 4 * (lane >> 5);
+      // (the lane's last key: from the first query's, so that no register holds it meanwhile)
+      uint32_t in_wave = lane & 31;
+      pin(in_wave);
+      const int end = a.causal ? min(jlo_raw + (int)in_wave, p.lk - 1) : p.lk - 1;
+      const int lim = end - j0 - 4 * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
