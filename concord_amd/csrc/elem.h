@@ -68,6 +68,19 @@ CONCORD_DEV float wave_sum(float v) {
   return lane_value(v, 63);
 }
 
+// Sum over each group of 16 lanes, to each of them: lanes 1, 2 apart, then the
+// mirrored half and the mirrored other half.
+CONCORD_DEV float row16_sum(float v) {
+#define CONCORD_DPP_ADD(ctrl) \
+  v = __fadd_rn(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true)))
+  CONCORD_DPP_ADD(0xB1);    // quad_perm 1, 0, 3, 2
+  CONCORD_DPP_ADD(0x4E);    // quad_perm 2, 3, 0, 1
+  CONCORD_DPP_ADD(0x141);   // row_half_mirror
+  CONCORD_DPP_ADD(0x140);   // row_mirror
+#undef CONCORD_DPP_ADD
+  return v;
+}
+
 // Maximum over the wave's 64 lanes, to every lane.  Lanes without a source
 // keep their own value (old = v).
 CONCORD_DEV float wave_max_f32(float v) {

@@ -85,6 +85,7 @@ def _norm_check(x, w, b, dy, eps=1e-5, to=lambda t: t.to(DEV)):
 # one column, one vector and its neighbours, each count of waves a row takes
 # and its ends, rows longer than a block holds
 @pytest.mark.parametrize("rows,width", [
+    (70, 24), (130, 120), (65, 128), (66, 129), (600, 33),
     (1, 1), (3, 2), (5, 7), (4, 8), (1, 384), (130, 384), (7, 511), (7, 512), (9, 513), (6, 1000), (5, 1024),
     (5, 1025), (1, 1280), (3, 2048), (3, 2051), (2, 4096), (3, 4097), (2, 8192), (2, 8200), (2, 12288), (2, 16384),
     (2, 16385), (3, 20000), (2500, 64), (1100, 1032)])
