@@ -372,6 +372,7 @@ static void distill_split(DistillArgs& a, int splits) {
   a.seg = cdiv(cdiv(a.V, a.splits), 8) * 8;
   a.splits = (int)cdiv(a.V, a.seg);
 }
+static bool distill_fits(const DistillArgs& a) { return a.M * a.splits < (1LL << 31); }
 
 template <class T>
 static void distill_fwd(const DistillArgs& a, hipStream_t st) {
@@ -438,6 +439,7 @@ extern "C" int concord_distill_fwd(const void* logits, int64_t ld_l, int dtype, 
   CONCORD_CHECK(((uintptr_t)stats & 15) == 0, "concord_distill_fwd: stats must lie on 16 bytes");
   a.loss = loss, a.stat = stats, a.part = (float*)workspace;
   distill_split(a, distill_splits(M, V));
+  CONCORD_CHECK(distill_fits(a), "concord_distill_fwd: bad size");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CONCORD_F32) distill_fwd<float>(a, st);
   else if (dtype == CONCORD_BF16) distill_fwd<BF16>(a, st);
@@ -458,6 +460,7 @@ extern "C" int concord_distill_bwd(const float* dloss, int64_t ld_dloss, const v
   a.g = dloss, a.ldg = ld_dloss, a.stat = (float*)stats, a.dz = dlogits, a.lddz = ld_d;
   // (segments of about 16 KB; of 24 KB: 351 us)
   distill_split(a, V <= kWaveRow ? 1 : (int)std::max<int64_t>(1, V * (dtype == CONCORD_F32 ? 4 : 2) / 16384));
+  CONCORD_CHECK(distill_fits(a), "concord_distill_bwd: bad size");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CONCORD_F32) distill_bwd<float>(a, st);
   else if (dtype == CONCORD_BF16) distill_bwd<BF16>(a, st);

@@ -1,5 +1,7 @@
 /*
- * concord_amd.h -- C ABI of the MI355X (gfx950) packed-weight linear path.
+ * concord_amd.h -- C ABI of the MI355X (gfx950) packed-weight linear path, and
+ * of the operators that stand between such layers in a training step (layer
+ * norm, attention, distillation; at the end).
  *
  * Every entry point takes raw device pointers, sizes and leading dimensions,
  * plus the hipStream_t (passed as void*) to enqueue on.  No entry point

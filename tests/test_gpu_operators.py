@@ -481,7 +481,7 @@ def test_attention_empty():
     q = torch.randn(5, 2, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
     out = ca.attention(q, z, z, starts=_i32([0, 5]), k_starts=_i32([0, 0]))
     out.sum().backward()
-    assert float(out.abs().sum()) == 0.0 and float(q.grad.abs().sum()) == 0.0
+    assert float(out.detach().abs().sum()) == 0.0 and float(q.grad.abs().sum()) == 0.0
     k = torch.randn(5, 2, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
     out = ca.attention(z, k, k, starts=_i32([0, 0]), k_starts=_i32([0, 5]))
     out.sum().backward()
@@ -703,3 +703,68 @@ def test_distill_empty():
     loss = ca.distill_loss(z, torch.zeros(0, 4, device=DEV), torch.zeros(0, 4, dtype=torch.int64, device=DEV))
     loss.sum().backward()
     assert loss.shape == (0,) and z.grad.shape == z.shape
+
+
+# ---- all three ------------------------------------------------------------------
+def _all_three(tokens, gen):
+    """A training step through layer norm, attention and the loss: (inputs, step)."""
+    import concord_amd as ca
+    x = torch.randn(tokens, 384, generator=gen).to(torch.bfloat16).to(DEV).requires_grad_(True)
+    w, b = ((torch.randn(384, generator=gen) * 0.1 + c).to(DEV).requires_grad_(True) for c in (1.0, 0.0))
+    starts = _i32([0, 1, tokens // 3, tokens])
+    t = torch.randn(tokens, 8, generator=gen).to(DEV)
+    i = torch.randint(0, 128, (tokens, 8), generator=gen).to(DEV)
+
+    def step():
+        q, k, v = ca.layer_norm(x, w, b).view(tokens, 6, 64).split([4, 1, 1], dim=1)
+        z = ca.attention(q, k, v, starts=starts).reshape(tokens, 256)[:, :128]
+        loss = ca.distill_loss(z, t, i, temperature=2.0).mean()
+        return (loss, *torch.autograd.grad(loss, (x, w, b)))
+    return x, step
+
+
+def test_operators_in_a_captured_step():
+    """One HIP graph of the step, replayed with new inputs and with eager work
+    between the replays: the eager results, bit for bit."""
+    gen = _gen("graph")
+    x, step = _all_three(700, gen)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [t.detach() for t in step()]
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=gen).to(x.dtype))
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_operators_are_differentiable_once():
+    import concord_amd as ca
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    q = torch.randn(4, 1, 64, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    idx = torch.zeros(4, 1, dtype=torch.int64, device=DEV)
+    for y, leaf in ((ca.layer_norm(x), x), (ca.attention(q, q, q), q),
+                    (ca.distill_loss(x, torch.zeros(4, 1, device=DEV), idx), x)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), leaf, create_graph=True)
+
+
+def test_operators_see_a_change_of_a_saved_tensor():
+    """An input overwritten between forward and backward is an error, not a wrong gradient."""
+    import concord_amd as ca
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    h = x * 1.0
+    y = ca.layer_norm(h)
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
