@@ -262,8 +262,9 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
   const int lane = Lanes<W>::id(), slot = W == 1 ? Lanes<W>::wave() : 0, kp = (a.K + 3) & ~3;
   int32_t* place = entries + slot * 2 * kp;
   float* prob = (float*)(place + kp);
-  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + slot : blockIdx.x / a.splits;
-  if (W == 1 && row >= a.M) return;   // (a wave for itself: no barrier below)
+  // the last rows first: the forward read them last, and they are still cached
+  const int64_t nth = W == 1 ? (int64_t)blockIdx.x * 4 + slot : blockIdx.x / a.splits, row = a.M - 1 - nth;
+  if (W == 1 && nth >= a.M) return;   // (a wave for itself: no barrier below)
   const int64_t v0 = W == 1 ? 0 : (int64_t)(blockIdx.x % a.splits) * a.seg;
   const int64_t n = W == 1 ? a.V : min<int64_t>(a.seg, a.V - v0);
   const T* z = (const T*)a.z + row * a.ldz + v0;

@@ -223,7 +223,8 @@ __global__ __launch_bounds__((LnRow<T, VEC, E, W, L>::THREADS)) void ln_bwd_kern
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       // (no row there: the first again, its dy taken as zeros)
-      const int64_t at = NR == 1 || r0 + r < a.M ? r0 + r : r0;
+      // the last rows first: their producer wrote them last, and they are still cached
+      const int64_t at = a.M - 1 - (NR == 1 || r0 + r < a.M ? r0 + r : r0);
       R::load(rx[r], a.x, at, a.ldx, C);
       R::load(ry[r], a.dy, at, a.ldy, C);
       mean[r] = a.mean[at];
@@ -282,7 +283,7 @@ __global__ __launch_bounds__((LnRow<T, VEC, E, W, L>::THREADS)) void ln_bwd_kern
       float dx[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) dx[i] = rs[r] * (__builtin_fmaf(dy[r][i], w[i], -m1) - h[r][i] * m2);
-      if (NR == 1 || row + r < a.M) R::store(a.out, row + r, a.ldo, C, dx);
+      if (NR == 1 || row + r < a.M) R::store(a.out, a.M - 1 - (row + r), a.ldo, C, dx);
     }
   }
   if (!a.part) return;
