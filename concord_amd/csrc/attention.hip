@@ -105,28 +105,25 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
     for (int r = 1; r < 32; ++r) x = fmaxf(x, s[r >> 4][r & 15]);
     return x;
   };
-  // Before the exponentials of tile t: its mask, and the maximum they are
-  // relative to.  mx: the largest of the lane's scores (unmasked).
-  auto settle = [&](int t, f32x16 (&s)[2], float mx) CONCORD_INLINE_LAMBDA {
-    const int j0 = t * kAttnK;
-    if (j0 + kAttnK - 1 > jlo) {
-      // (the lane's last key: from the first query's, so that no register holds it meanwhile)
-      uint32_t in_wave = lane & 31;
-      pin(in_wave);
-      const int end = a.causal ? min(jlo_raw + (int)in_wave, p.lk - 1) : p.lk - 1;
-      const int lim = end - j0 - 4 * (lane >> 5);
+  auto masked = [&](int t) CONCORD_INLINE_LAMBDA { return (t + 1) * kAttnK - 1 > jlo; };
+  auto mask = [&](int t, f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
+    // (the lane's last key: from the first query's, so that no register holds it meanwhile)
+    uint32_t in_wave = lane & 31;
+    pin(in_wave);
+    const int end = a.causal ? min(jlo_raw + (int)in_wave, p.lk - 1) : p.lk - 1;
+    const int lim = end - t * kAttnK - 4 * (lane >> 5);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + 8 * (r >> 2) + (r & 3) > lim ? -INFINITY : s[i][r];
-      mx = lane_max(s);
-    }
+      for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + 8 * (r >> 2) + (r & 3) > lim ? -INFINITY : s[i][r];
+  };
+  // The sums are relative to m, which follows the maximum only when that has
+  // grown by more than 2^8: the factor of out and l is then nearly never
+  // applied, and the probabilities' rounding is relative to each.
+  // mx: the largest of the lane's scores.
+  auto raise = [&](float mx) CONCORD_INLINE_LAMBDA {
     const Halves both = halves(mx);
     const float top = fmaxf(both.lo, both.hi) * a.c;
-    // The sums are relative to m, which follows the maximum only when that has
-    // grown by more than 2^8: the factor of out and l is then nearly never
-    // applied, and the probabilities stay within 2^8, exact in their type as
-    // those below 1 are.
     if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
       const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -136,6 +133,14 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= f;
     }
+  };
+  // before the exponentials of tile t; mx: the largest of the lane's scores, unmasked
+  auto settle = [&](int t, f32x16 (&s)[2], float mx) CONCORD_INLINE_LAMBDA {
+    if (masked(t)) {
+      mask(t, s);
+      mx = lane_max(s);
+    }
+    raise(mx);
   };
   // Tile t's exponentials and product with v, and (NEXT) the scores of tile
   // t + 1.  A wave issues in order and an MFMA holds the matrix core for 32
@@ -198,16 +203,30 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
   const int own = jhi < 0 ? 0 : min(tiles, jhi / kAttnK + 1);   // tiles with a key for any of the wave's queries
   typedef std::integral_constant<int, 0> S0;
   typedef std::integral_constant<int, 1> S1;
-  auto first_scores = [&](f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
+  auto scores = [&](f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       s[i] = zero16();
 #pragma unroll
       for (int k = 0; k < NK; ++k) s[i] = mfma(fr.rows(0, i, k), q.f[k], s[i]);
     }
-    return lane_max(s);
   };
   if constexpr (!PIPE) {
+    // Narrow heads have few MFMAs to an exponential, so past the first tile the
+    // maximum is not even formed: m stays until a lane's 32 probabilities add up
+    // to more than 2^20 (or to no number).  The scores are then formed again from
+    // the tile, which still lies in LDS, and m is raised.  (2 x 4096 x 64 heads of
+    // 64: 554 -> 539 us.)
+    auto exps = [&](f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 4][r & 15], a.c, -m));
+        s[r >> 4][r & 15] = e;
+        sum += e;
+      }
+      return sum;
+    };
     if (tiles > 0) load_k(0), load_v(0);
     for (int t = 0; t < tiles; ++t) {
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's part of tile t has landed
@@ -215,9 +234,23 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
       if (t + 1 < tiles) load_k(t + 1), load_v(t + 1);
       if (t < own) {
         f32x16 s[2];
-        float mx = first_scores(s);
-        settle(t, s, mx);
-        step(std::false_type(), S0(), s, s, mx);
+        scores(s);
+        if (masked(t)) mask(t, s);
+        if (t == 0) raise(lane_max(s));
+        float sum = exps(s);
+        if (__builtin_amdgcn_ballot_w64(!(sum <= 0x1p20f))) {
+          scores(s);
+          if (masked(t)) mask(t, s);
+          raise(lane_max(s));
+          sum = exps(s);
+        }
+        l += sum;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const bf16x8 e = round8(s[u >> 1], u & 1);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[d] = mfma(fr.cols(2 * T::BYTES, d, u), e, o[d]);
+        }
       }
       fr.move(t & 1 ? -T::BYTES : T::BYTES);
     }
@@ -237,7 +270,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
     if (tiles > 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * T::PER));
     else __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::PER));
     lds_barrier();
-    float mx = first_scores(sa);
+    scores(sa);
+    float mx = lane_max(sa);
     int t = 0;
     for (; t + 2 < own; t += 2) {
       turn(t);
