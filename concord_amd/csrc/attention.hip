@@ -14,7 +14,8 @@
 // small launch runs at 2.2).  2 x 8192 x 32 / 8 heads of 128 without a mask 1930
 // us, 1140 TFLOP/s, MFMA pipes busy 0.64 of the time; a library's 16384^3
 // product reaches 1341 TFLOP/s here.  Heads of 64 have half the MFMAs to the
-// same exponentials: 2 x 4096 x 64 heads 676 us, 814 TFLOP/s, busy 0.50.
+// same exponentials: 2 x 4096 x 64 heads 539 us, 1020 TFLOP/s (up to 660 us
+// while the clock is lower).
 #include "attention.h"
 
 namespace concord {

@@ -11,10 +11,11 @@
 // of a row whose upstream gradient g is 0, whatever its logits hold.
 //
 // Bound by memory: forward reads the logits once (running maximum and sum of
-// exponentials), backward reads them again and writes the gradient: 161 us (5.1
-// TB/s) and 319 us (5.2 TB/s) at 8192 x 50257 bf16, where a copy moves 5.0
-// TB/s.  All statistics are fp32.  A row is one wave's (V <= 1024), one block's, or is
-// split over several blocks when the rows are too few to fill the chip.
+// exponentials), backward reads them again and writes the gradient: 166 us (5.0
+// TB/s) and 296 us (5.6 TB/s: what the forward read last is still cached) at
+// 8192 x 50257 bf16, where a copy moves 5.0 TB/s.  All statistics are fp32.  A
+// row is one wave's (V <= 1024), one block's, or is split over several blocks
+// when the rows are too few to fill the chip.
 #include "elem.h"
 
 namespace concord {
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillArgs a) {
 // (Measured at 8192 x 50257 bf16, K 64: entries read, and their logits gathered,
 // ahead of the pass, and a search that leaves the sum to the entries that
 // share a place, rows in segments of about 16 KB, so that the blocks in flight
-// sweep memory in order: 389 -> 319 us, 5.2 TB/s.)
+// sweep memory in order: 389 -> 319 us; with the last rows first 296.)
 template <class T, int W>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
   constexpr int TH = W * 64, VEC = Span<T>::VEC, NE = W == 1 ? 1 : kTopMax / TH;
