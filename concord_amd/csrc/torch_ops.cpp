@@ -75,6 +75,26 @@ Rows rows_of(const Tensor& t, int64_t rows, int64_t width) {
   return {r, rows > 1 ? r.stride(0) : width};
 }
 
+// ---- saved tensors ----------------------------------------------------------------
+// A saved-tensor hook (offloading to the host, recomputation) may give a saved
+// tensor back in another layout: the backwards take strides from what comes
+// back and keep none of the forward's.
+
+// a vector or table that the kernels index without strides: its elements
+// adjacent, on 16 bytes
+Tensor packed(const Tensor& t) {
+  if (!t.defined()) return t;
+  Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone() : c;
+}
+
+// its type, extent and device have to be what was saved (like: the upstream gradient)
+void came_back(const Tensor& t, at::ScalarType type, int64_t numel, const Tensor& like, const char* op,
+               const char* name) {
+  TORCH_CHECK(t.defined() && t.scalar_type() == type && t.numel() == numel && t.device() == like.device(), op,
+              ": the saved ", name, " came back as another tensor");
+}
+
 // ---- layer norm -----------------------------------------------------------------
 const char* const kNorm = "layer_norm";
 
@@ -118,7 +138,6 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     Tensor stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
     Tensor y = norm_forward(r, x, weight, bias, (int)wdtype, eps, stats);
     ctx->save_for_backward({r.t, weight, stats});
-    ctx->saved_data["ld"] = r.ld;
     ctx->saved_data["wdtype"] = wdtype;
     ctx->saved_data["has_bias"] = bias.defined();
     return y;
@@ -126,11 +145,15 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     only_once(kNorm);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2], &dy = grads[0];
-    const c10::OptionalDeviceGuard guard(x.device());
-    const int64_t rows = stats.size(1), width = dy.size(-1), wdtype = ctx->saved_data["wdtype"].toInt();
-    const Rows g = rows_of(dy, rows, width);
+    const Tensor &x = saved[0], &dy = grads[0];
+    const c10::OptionalDeviceGuard guard(dy.device());
+    const int64_t width = dy.size(-1), rows = dy.numel() / width, wdtype = ctx->saved_data["wdtype"].toInt();
+    const Tensor weight = saved[1].defined() ? saved[1].contiguous() : Tensor(), stats = packed(saved[2]);
     const auto wtype = wdtype == CONCORD_F32 ? at::kFloat : wdtype == CONCORD_BF16 ? at::kBFloat16 : at::kHalf;
+    came_back(x, dy.scalar_type(), dy.numel(), dy, kNorm, "x");
+    came_back(stats, at::kFloat, 2 * rows, dy, kNorm, "statistics");
+    if (weight.defined()) came_back(weight, wtype, width, dy, kNorm, "weight");
+    const Rows r = rows_of(x, rows, width), g = rows_of(dy, rows, width);
     Tensor dx = at::empty(dy.sizes(), x.options()), dw, db, ws;
     // (numbered among the tensors that were given)
     const size_t at_bias = weight.defined() ? 2 : 1;
@@ -143,9 +166,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
       ws = bytes(need, x);
     }
     float* mean = stats.data_ptr<float>();
-    check(concord_layernorm_bwd(ptr(g.t), g.ld, ptr(x), ctx->saved_data["ld"].toInt(), dtype_of(x), ptr(weight),
-                                (int)wdtype, mean, mean + rows, rows, width, ptr(dx), width, ptr(dw), ptr(db), ptr(ws),
-                                need, stream_of(x)),
+    check(concord_layernorm_bwd(ptr(g.t), g.ld, ptr(r.t), r.ld, dtype_of(x), ptr(weight), (int)wdtype, mean, mean + rows,
+                                rows, width, ptr(dx), width, ptr(dw), ptr(db), ptr(ws), need, stream_of(x)),
           "layer_norm backward");
     return {dx, dw, db, Tensor(), Tensor()};
   }
@@ -225,15 +247,15 @@ void attn_check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
 }
 
 // the part of the arguments that both passes share
-concord_attn_args attn_args(const Operand& q, const Operand& k, const Operand& v, const Tensor& out, const Tensor& lse,
-                            const Tensor& low, const Tensor& starts, const Tensor& k_starts, bool causal,
-                            double scale) {
+concord_attn_args attn_args(const Operand& q, const Operand& k, const Operand& v, const Operand& out,
+                            const Tensor& lse, const Tensor& low, const Tensor& starts, const Tensor& k_starts,
+                            bool causal, double scale) {
   concord_attn_args a{};
   a.q = (const uint16_t*)ptr(q.t), a.q_t = q.token, a.q_h = q.head;
   a.k = (const uint16_t*)ptr(k.t), a.k_t = k.token, a.k_h = k.head;
   a.v = (const uint16_t*)ptr(v.t), a.v_t = v.token, a.v_h = v.head;
   const int64_t h = q.t.size(-2), d = q.t.size(-1), hk = k.t.size(-2);
-  a.out = (uint16_t*)ptr(out), a.o_t = h * d, a.o_h = d;
+  a.out = (uint16_t*)ptr(out.t), a.o_t = out.token, a.o_h = out.head;
   a.lse = (float*)ptr(lse), a.out_low = (int8_t*)ptr(low);
   a.starts = (const int32_t*)ptr(starts), a.k_starts = (const int32_t*)ptr(k_starts);
   const int64_t batch = q.t.dim() == 4 ? q.t.size(0) : 1;
@@ -242,6 +264,9 @@ concord_attn_args attn_args(const Operand& q, const Operand& k, const Operand& v
   a.H = (int32_t)h, a.HK = (int32_t)hk, a.D = (int32_t)d, a.causal = causal, a.scale = (float)scale;
   return a;
 }
+
+// the result as an operand
+Operand fresh(const Tensor& out) { return {out, out.size(-2) * out.size(-1), out.size(-1)}; }
 
 void attn_forward(const concord_attn_args& a, const Tensor& q) {
   const size_t need = concord_attention_fwd_workspace_bytes(&a);
@@ -257,10 +282,9 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     Tensor out = at::empty(q.sizes(), q.options());
     Tensor lse = at::empty({q.numel() / q.size(-1)}, q.options().dtype(at::kFloat));
     Tensor low = at::empty(q.sizes(), q.options().dtype(at::kChar));
-    const concord_attn_args a = attn_args(oq, ok, ov, out, lse, low, starts, k_starts, causal, scale);
+    const concord_attn_args a = attn_args(oq, ok, ov, fresh(out), lse, low, starts, k_starts, causal, scale);
     attn_forward(a, q);
     ctx->save_for_backward({oq.t, ok.t, ov.t, out, lse, low, starts, k_starts});
-    ctx->saved_data["strides"] = std::vector<int64_t>{oq.token, oq.head, ok.token, ok.head, ov.token, ov.head};
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return out;
@@ -268,12 +292,19 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     only_once(kAttn);
     const auto s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2];
-    const c10::OptionalDeviceGuard guard(q.device());
-    const auto st = ctx->saved_data["strides"].toIntVector();
-    const Operand g = operand(grads[0]);
-    concord_attn_args a = attn_args({q, st[0], st[1]}, {k, st[2], st[3]}, {v, st[4], st[5]}, s[3], s[4], s[5], s[6], s[7],
-                                    ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &dout = grads[0];
+    const c10::OptionalDeviceGuard guard(dout.device());
+    const Tensor lse = packed(s[4]), low = packed(s[5]), starts = packed(s[6]), k_starts = packed(s[7]);
+    const double scale = ctx->saved_data["scale"].toDouble();
+    TORCH_CHECK(q.sizes() == dout.sizes() && s[3].sizes() == dout.sizes(), "attention: the saved q and out came back as ",
+                q.sizes(), " and ", s[3].sizes());
+    attn_check(q, k, v, starts, k_starts, scale);
+    came_back(s[3], at::kBFloat16, q.numel(), dout, kAttn, "out");
+    came_back(lse, at::kFloat, q.numel() / q.size(-1), dout, kAttn, "lse");
+    came_back(low, at::kChar, q.numel(), dout, kAttn, "low part of out");
+    const Operand oq = operand(q), ok = operand(k), ov = operand(v), out = operand(s[3]), g = operand(dout);
+    concord_attn_args a =
+        attn_args(oq, ok, ov, out, lse, low, starts, k_starts, ctx->saved_data["causal"].toBool(), scale);
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
     Tensor dv = at::empty(k.sizes(), k.options());
     a.dout = (const uint16_t*)ptr(g.t), a.do_t = g.token, a.do_h = g.head;
@@ -298,7 +329,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeT
     return AttentionNode::apply(q, k, v, maybe(starts), maybe(k_starts), causal, scale);
   Tensor out = at::empty(q.sizes(), q.options());
   const concord_attn_args a =
-      attn_args(operand(q), operand(k), operand(v), out, Tensor(), Tensor(), starts, k_starts, causal, scale);
+      attn_args(operand(q), operand(k), operand(v), fresh(out), Tensor(), Tensor(), starts, k_starts, causal, scale);
   attn_forward(a, q);
   return out;
 }
@@ -357,27 +388,33 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
     Tensor loss = distill_forward(r, logits, temperature, stats);
     ctx->save_for_backward({r.z.t, r.t.t, r.i.t, stats});
     ctx->saved_data["shape"] = logits.sizes().vec();
-    ctx->saved_data["lds"] = std::vector<int64_t>{r.z.ld, r.t.ld, r.i.ld, r.top};
+    ctx->saved_data["top"] = (int64_t)r.top;
+    ctx->saved_data["type"] = (int64_t)logits.scalar_type();
     ctx->saved_data["temperature"] = temperature;
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     only_once(kDistill);
     const auto s = ctx->get_saved_variables();
-    const Tensor &z = s[0], &stats = s[3], &dloss = grads[0];
-    const c10::OptionalDeviceGuard guard(z.device());
+    const Tensor& dloss = grads[0];
+    const c10::OptionalDeviceGuard guard(dloss.device());
+    const Tensor stats = packed(s[3]);
     const auto shape = ctx->saved_data["shape"].toIntVector();
-    const auto ld = ctx->saved_data["lds"].toIntVector();
-    const int64_t rows = stats.size(0), vocab = shape.back();
+    const int64_t rows = dloss.numel(), vocab = shape.back(), top = ctx->saved_data["top"].toInt();
+    came_back(s[0], (at::ScalarType)ctx->saved_data["type"].toInt(), rows * vocab, dloss, kDistill, "logits");
+    came_back(s[1], at::kFloat, rows * top, dloss, kDistill, "teacher_logits");
+    came_back(s[2], at::kLong, rows * top, dloss, kDistill, "teacher_index");
+    came_back(stats, at::kFloat, rows * 4, dloss, kDistill, "statistics");
+    const Rows z = rows_of(s[0], rows, vocab), t = rows_of(s[1], rows, top), i = rows_of(s[2], rows, top);
     // one value for all rows (a sum's or a mean's gradient) stays one value
     bool one = dloss.numel() > 0;
     for (int64_t d = 0; d < dloss.dim(); ++d) one = one && (dloss.stride(d) == 0 || dloss.size(d) == 1);
     const Rows g = one ? Rows{dloss, 0} : rows_of(dloss, rows, 1);
-    Tensor dz = at::empty(shape, z.options());
-    check(concord_distill_bwd((const float*)ptr(g.t), g.ld, ptr(z), ld[0], dtype_of(z), rows, vocab,
-                              (const float*)ptr(s[1]), ld[1], (const int64_t*)ptr(s[2]), ld[2], (int32_t)ld[3],
+    Tensor dz = at::empty(shape, z.t.options());
+    check(concord_distill_bwd((const float*)ptr(g.t), g.ld, ptr(z.t), z.ld, dtype_of(z.t), rows, vocab,
+                              (const float*)ptr(t.t), t.ld, (const int64_t*)ptr(i.t), i.ld, (int32_t)top,
                               (float)ctx->saved_data["temperature"].toDouble(), stats.data_ptr<float>(), ptr(dz), vocab,
-                              stream_of(z)),
+                              stream_of(z.t)),
           "distill_loss backward");
     return {dz, Tensor(), Tensor(), Tensor()};
   }
