@@ -8,6 +8,7 @@
 // alone.  They check arguments, hand out memory from torch's allocator on the
 // current stream and call the entries; the C++ exceptions thrown here become
 // Python's (ValueError, TypeError, RuntimeError).
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -55,6 +56,14 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A dual tensor need not require grad, so the choice of a node by requires_grad
+// alone would drop its tangent without a word.
+void no_tangent(const char* op, std::initializer_list<const Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op, " has no derivative in forward mode");
+}
 
 void only_once(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, " is differentiable once: its backward has no gradient of its own");
@@ -175,6 +184,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight_, const MaybeTensor& bias_, double eps) {
   Tensor weight = value(weight_), bias = value(bias_);
+  no_tangent(kNorm, {&x, &weight, &bias});
   const int wdtype = norm_check(x, weight, bias);
   const c10::OptionalDeviceGuard guard(x.device());
   if (weight.defined()) weight = weight.contiguous();
@@ -323,6 +333,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeT
   const Tensor starts = starts_ ? starts_->contiguous() : Tensor();
   const Tensor k_starts = k_starts_ ? k_starts_->contiguous() : Tensor();
   const double scale = scale_ ? *scale_ : q.dim() && q.size(-1) ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0;
+  no_tangent(kAttn, {&q, &k, &v});
   attn_check(q, k, v, starts, k_starts, scale);
   const c10::OptionalDeviceGuard guard(q.device());
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v)))
@@ -421,6 +432,7 @@ struct DistillNode : torch::autograd::Function<DistillNode> {
 };
 
 Tensor distill_loss(const Tensor& logits, const Tensor& teacher, const Tensor& index, double temperature) {
+  no_tangent(kDistill, {&logits});
   distill_check(logits, teacher, index, temperature);
   const c10::OptionalDeviceGuard guard(logits.device());
   const Tensor t = teacher.detach();

@@ -5,7 +5,9 @@ every view that is not dense; recomputation may).
 On the CPU: the nodes of csrc/torch_ops.cpp are compiled over C entries that
 record their operands (operators_stub.cpp).  Each operand has to hold the values
 that it holds without a hook, whatever the layout that comes back; it comes back
-inside a larger buffer of NaN, so that a wrong stride reads those."""
+inside a larger buffer of NaN, so that a wrong stride reads those.
+
+The same module shows what the nodes do with the tangents of forward mode."""
 import importlib.util
 import os
 import subprocess
@@ -165,6 +167,35 @@ def test_another_tensor_is_refused(stub, other):
         with pytest.raises((RuntimeError, TypeError, ValueError), match="came back|must be|attention"):
             y.sum().backward()
     assert not stub.recorded()[0]
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("enabled", [True, False])
+def test_forward_mode_is_refused(stub, requires_grad, enabled):
+    """A tangent on any differentiable input is an error, in no_grad too (which
+    leaves forward mode on); with forward mode off there is nothing to drop."""
+    import torch.autograd.forward_ad as fw
+
+    def inputs(args, dual):
+        args = [a.detach().clone().requires_grad_(requires_grad) for a in args]
+        args[dual] = fw.make_dual(args[dual], torch.ones_like(args[dual]))
+        assert fw.unpack_dual(args[dual]).tangent is not None
+        return args
+    x, w = _randn(6, 24), _randn(24)
+    q = _randn(6, 2, 8, dtype=torch.bfloat16)
+    ops = [(stub.layer_norm, [x, w, w], (1e-5,)), (stub.attention, [q, q, q], (None, None, True, None)),
+           (stub.distill_loss, [x], (_randn(6, 4), torch.zeros(6, 4, dtype=torch.int64), 1.0))]
+    with fw.dual_level():
+        for op, args, rest in ops:
+            for dual in range(len(args)):
+                given = inputs(args, dual)
+                if enabled:
+                    for mode in (torch.enable_grad, torch.no_grad):
+                        with mode(), pytest.raises(RuntimeError, match="forward mode"):
+                            op(*given, *rest)
+                else:
+                    with fw._set_fwd_grad_enabled(False):
+                        op(*given, *rest)
 
 
 # ---- on the GPU: the kernels themselves --------------------------------------------
