@@ -400,14 +400,14 @@ inline bool attn_operand(const void* p, int64_t t, int64_t h, int64_t T, int D) 
   return T == 0 || (p && ((uintptr_t)p & 15) == 0 && t % 8 == 0 && h % 8 == 0 && t >= D && t < (1 << 24) && h >= 0);
 }
 
-inline int attn_check(const char* what, const concord_attn_args& a) {
+// what the arithmetic on the sizes alone rests on
+inline int attn_sizes(const char* what, const concord_attn_args& a) {
   CONCORD_CHECK(a.TQ >= 0 && a.TK >= 0 && a.TQ < (1LL << 31) - 256 && a.TK < (1LL << 31) - 256 && a.B >= 0 &&
                     a.B < (1LL << 24),
                 "%s: bad size", what);
   CONCORD_CHECK(a.D >= 8 && a.D <= 128 && a.D % 8 == 0, "%s: the head dimension must be a multiple of 8 up to 128",
                 what);
   CONCORD_CHECK(a.H >= 1 && a.HK >= 1 && a.H % a.HK == 0 && a.H < (1 << 16), "%s: H must be a multiple of HK", what);
-  CONCORD_CHECK(a.scale > 0.0f && a.scale < INFINITY, "%s: the scale must be positive", what);
   CONCORD_CHECK(a.B > 0 || a.starts || (a.TQ == 0 && a.TK == 0), "%s: no sequence", what);
   if (!a.starts) {
     CONCORD_CHECK(!a.k_starts, "%s: k_starts without starts", what);
@@ -415,6 +415,12 @@ inline int attn_check(const char* what, const concord_attn_args& a) {
   } else {
     CONCORD_CHECK(a.k_starts || a.TQ == a.TK, "%s: k_starts needed where TK differs from TQ", what);
   }
+  return CONCORD_OK;
+}
+
+inline int attn_check(const char* what, const concord_attn_args& a) {
+  if (const int rc = attn_sizes(what, a)) return rc;
+  CONCORD_CHECK(a.scale > 0.0f && a.scale < INFINITY, "%s: the scale must be positive", what);
   CONCORD_CHECK(attn_operand(a.q, a.q_t, a.q_h, a.TQ, a.D) && attn_operand(a.out, a.o_t, a.o_h, a.TQ, a.D) &&
                     attn_operand(a.k, a.k_t, a.k_h, a.TK, a.D) && attn_operand(a.v, a.v_t, a.v_h, a.TK, a.D),
                 "%s: NULL, misaligned or badly strided argument", what);

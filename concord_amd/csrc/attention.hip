@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
 using namespace concord;
 
 extern "C" size_t concord_attention_fwd_workspace_bytes(const concord_attn_args* args) {
-  if (!args || args->TQ < 1 || args->H < 1 || args->HK < 1 || args->D < 8) return 0;
+  if (!args || attn_sizes("concord_attention_fwd_workspace_bytes", *args) || args->TQ < 1) return 0;
   const int n = key_splits(*args, 4.0);
   return n > 1 ? (size_t)n * (size_t)args->TQ * (size_t)args->H * (size_t)(args->D + 2) * sizeof(float) : 0;
 }

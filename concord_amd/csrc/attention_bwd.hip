@@ -346,7 +346,7 @@ static size_t delta_bytes(const concord_attn_args& g) {
 using namespace concord;
 
 extern "C" size_t concord_attention_workspace_bytes(const concord_attn_args* args) {
-  if (!args || args->TQ < 1 || args->H < 1 || args->HK < 1 || args->D < 8) return 0;
+  if (!args || attn_sizes("concord_attention_workspace_bytes", *args) || args->TQ < 1) return 0;
   const size_t n = dkv_splits(*args), m = key_splits(*args, 6.0);
   const size_t dkv = n > 1 ? n * 2 * (size_t)args->TK * (size_t)args->HK : 0;
   const size_t dq = m > 1 ? m * (size_t)args->TQ * (size_t)args->H : 0;

@@ -590,7 +590,7 @@ typedef struct concord_attn_args {
 } concord_attn_args;
 /* workspace: concord_attention_fwd_workspace_bytes(args) bytes on 16 (0: none
  * needed; it holds the sums of few queries' shares of long keys); it need not
- * be zeroed. */
+ * be zeroed.  Both size queries give 0 for sizes that the entries refuse. */
 size_t concord_attention_fwd_workspace_bytes(const concord_attn_args* args);
 int concord_attention_fwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* dq, dk, dv from dout, the forward's out, lse and out_low; dk and dv summed over the

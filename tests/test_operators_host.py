@@ -180,3 +180,34 @@ def test_distill_entry_refusals(L):
         args = list(bwd)
         args[at] = v
         assert L.concord_distill_bwd(*args) == C.EINVAL, at
+
+
+BAD_ATTENTION_SIZES = [dict(B=0), dict(B=0, TQ=0), dict(B=0, TK=0), dict(B=-1), dict(B=1 << 24), dict(B=3), dict(TQ=-1), dict(TK=-4),
+                       dict(TQ=1 << 31), dict(TK=1 << 31), dict(TQ=1 << 62, TK=1 << 62), dict(D=4), dict(D=0), dict(D=-8),
+                       dict(D=136), dict(D=60), dict(H=0), dict(H=3, HK=2), dict(HK=0), dict(HK=-1), dict(H=1 << 16),
+                       dict(k_starts=1)]
+
+
+def test_attention_workspace_of_sizes_that_the_entries_refuse():
+    """0, and no arithmetic on them: in a process of its own, since a division by
+    B = 0 ends it."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import ctypes, sys\n"
+            "sys.path[:0] = [%r, %r]\n"
+            "from concord_amd import _lib as C\n"
+            "from test_operators_host import BAD_ATTENTION_SIZES, _attn_args\n"
+            "L, buf = C.lib(), ctypes.create_string_buffer(64)\n"
+            "for kw in BAD_ATTENTION_SIZES:\n"
+            "    a = _attn_args(buf, **kw)\n"
+            "    assert L.concord_attention_fwd(ctypes.byref(a), None, 0, None) == C.EINVAL, kw\n"
+            "    assert L.concord_attention_bwd(ctypes.byref(a), None, 0, None) == C.EINVAL, kw\n"
+            "    for f in (L.concord_attention_fwd_workspace_bytes, L.concord_attention_workspace_bytes):\n"
+            "        print(kw, flush=True)\n"
+            "        assert f(ctypes.byref(a)) == 0, kw\n"
+            "assert L.concord_attention_workspace_bytes(None) == 0 == L.concord_attention_fwd_workspace_bytes(None)\n"
+            % (os.path.dirname(here), here))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stdout[-200:], r.stderr[-2000:])
