@@ -6,6 +6,7 @@ any compute entry point raises, with the command that builds it.
 import ctypes
 import importlib.util
 import os
+import threading
 
 import torch
 
@@ -180,6 +181,7 @@ def lib():
 
 
 _ops = None
+_ops_lock = threading.Lock()
 
 
 def ops():
@@ -191,9 +193,12 @@ def ops():
             raise ConcordError(
                 f"concord_amd: {OPS_PATH} is missing; build it with "
                 "`python -m concord_amd.build` (or __graft_entry__.build())")
-        spec = importlib.util.spec_from_file_location("concord_torch_ops", OPS_PATH)
-        _ops = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_ops)
+        with _ops_lock:
+            if _ops is None:   # (no other thread has loaded it meanwhile)
+                spec = importlib.util.spec_from_file_location("concord_torch_ops", OPS_PATH)
+                m = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(m)
+                _ops = m   # only now: before, it has no functions
     return _ops
 
 

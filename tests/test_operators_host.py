@@ -211,3 +211,49 @@ def test_attention_workspace_of_sizes_that_the_entries_refuse():
             % (os.path.dirname(here), here))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stdout[-200:], r.stderr[-2000:])
+
+
+def test_a_module_that_fails_to_load_is_not_kept(monkeypatch):
+    """ops() hands out the module once it has run, never before: a second thread
+    would find no functions in it, and so would every call after a failed load."""
+    import threading
+
+    from concord_amd import _lib as C
+    whole = C.ops()
+    monkeypatch.setattr(C, "_ops", None)
+    real, fail, started = C.importlib.util.spec_from_file_location, [True], []
+
+    class Loader:
+        def __init__(self, loader):
+            self.loader = loader
+
+        def create_module(self, spec):
+            return self.loader.create_module(spec)
+
+        def exec_module(self, m):
+            assert C._ops is None
+            started.append(threading.get_ident())
+            if fail[0]:
+                raise ImportError("no such symbol")
+            other = threading.Thread(target=lambda: seen.append(C.ops()))
+            other.start()
+            other.join(0.2)   # it waits for this load, or has its own
+            threads.append(other)
+            self.loader.exec_module(m)
+
+    def spec(name, path):
+        s = real(name, path)
+        s.loader = Loader(s.loader)
+        return s
+    seen, threads = [], []
+    monkeypatch.setattr(C.importlib.util, "spec_from_file_location", spec)
+    for _ in range(2):
+        with pytest.raises(ImportError, match="no such symbol"):
+            C.ops()
+    fail[0] = False
+    m = C.ops()
+    threads[0].join(10)
+    assert len(seen) == 1 and len(started) == 3
+    for n in ("layer_norm", "attention", "distill_loss"):
+        assert callable(getattr(m, n)) and callable(getattr(seen[0], n)) and callable(getattr(whole, n))
+    assert seen[0] is m and C.ops() is m
