@@ -13,7 +13,8 @@ and the accumulator-register form made the compiler copy accumulators
 around the main loops.
 
 torch_ops.cpp (host code: autograd nodes over the library's entries) becomes
-concord_amd/_lib/concord_torch_ops.so, against the installed torch.
+concord_amd/_lib/concord_torch_ops.so, against the installed torch.  Where that
+fails the build does, with the C library in place.
 """
 import glob
 import os
@@ -71,25 +72,33 @@ def build(verbose=False, jobs=8):
     objs = [os.path.join(OUT_DIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
 
     ops_src, ops_obj = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(OUT_DIR, "torch_ops.o")
-    ops_cflags, ops_libs = _ops_flags()
 
-    def compile_one(so):
-        s, o = so
-        if s.endswith(".cpp"):
-            return _run([CXX] + ops_cflags + ["-c", s, "-o", o])
+    def compile_one(s, o):
         return _run([HIPCC] + CFLAGS + FILE_FLAGS.get(os.path.basename(s), []) + ["-c", s, "-o", o])
 
+    def compile_ops():
+        cflags, libs = _ops_flags()
+        return _run([CXX] + cflags + ["-c", ops_src, "-o", ops_obj]), libs
+
+    def show(msg):
+        if verbose and msg.strip():
+            print(msg, file=sys.stderr)
+
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        for msg in ex.map(compile_one, [(ops_src, ops_obj)] + list(zip(srcs, objs))):
-            if verbose and msg.strip():
-                print(msg, file=sys.stderr)
-    tmp = LIB + ".tmp"
-    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs)
-    os.replace(tmp, LIB)
+        ops = ex.submit(compile_ops)
+        for msg in ex.map(compile_one, srcs, objs):
+            show(msg)
+        # the C library first: a binding without torch needs neither g++ nor torch's headers
+        tmp = LIB + ".tmp"
+        _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs)
+        os.replace(tmp, LIB)
+        for o in objs:
+            os.remove(o)
+        msg, ops_libs = ops.result()
+        show(msg)
     _run([CXX, "-shared", "-o", OPS + ".tmp", ops_obj] + ops_libs)
     os.replace(OPS + ".tmp", OPS)
-    for o in objs + [ops_obj]:
-        os.remove(o)
+    os.remove(ops_obj)
     if verbose:
         print(f"built {LIB} and {OPS}")
     return LIB
