@@ -382,7 +382,7 @@ extern "C" int concord_attention_fwd(const concord_attn_args* args, void* worksp
   a.o_t = g.o_t, a.o_h = g.o_h;
   a.seq = attn_seqs(g);
   const int64_t slots = attn_slots(a.seq, g.TQ, kAttnQ);
-  CONCORD_CHECK(slots * g.H * a.splits < (1LL << 31), "concord_attention_fwd: too many tiles");
+  CONCORD_CHECK(grid_fits(slots * g.H * a.splits, 256), "concord_attention_fwd: too many tiles");
   a.slots = (int32_t)slots;
   a.rep = g.H / g.HK, a.D = g.D, a.causal = g.causal != 0, a.c = g.scale * kLog2e;
   const dim3 grid((unsigned)(slots * g.H * a.splits));

@@ -382,12 +382,16 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
   hipStream_t st = (hipStream_t)stream;
   AttnSum sum{};
   sum.part = a.part, sum.D = g.D;
+  AttnSeqs keys = a.seq;
+  const int q_splits = key_splits(g, 6.0), k_splits = dkv_splits(g);
+  const int64_t q_slots = g.TQ > 0 ? attn_slots(a.seq, g.TQ, kDqRows) : 0;
+  const int64_t k_slots = g.TK > 0 ? attn_slots(keys, g.TK, kDkvRows) : 0;
+  CONCORD_CHECK(grid_fits(q_slots * g.H * q_splits, 256) && grid_fits(k_slots * g.HK * k_splits, 256),
+                "%s: too many tiles", what);
   if (g.TQ > 0) {
-    a.splits = key_splits(g, 6.0);
-    const int64_t slots = attn_slots(a.seq, g.TQ, kDqRows);
-    CONCORD_CHECK(slots * g.H * a.splits < (1LL << 31), "%s: too many tiles", what);
-    a.slots = (int32_t)slots;
-    const dim3 grid((unsigned)(slots * g.H * a.splits));
+    a.splits = q_splits;
+    a.slots = (int32_t)q_slots;
+    const dim3 grid((unsigned)(q_slots * g.H * a.splits));
     attn_by_dim(g.D, [&](auto nk) {
       constexpr int NK = decltype(nk)::value;
       if (a.splits > 1) hipLaunchKernelGGL((attn_dq_kernel<NK, true>), grid, dim3(256), 0, st, a);
@@ -400,12 +404,11 @@ extern "C" int concord_attention_bwd(const concord_attn_args* args, void* worksp
     }
   }
   if (g.TK > 0) {
-    a.splits = dkv_splits(g);
-    const int64_t slots = attn_slots(a.seq, g.TK, kDkvRows);
-    CONCORD_CHECK(slots * g.HK * a.splits < (1LL << 31), "%s: too many tiles", what);
-    a.slots = (int32_t)slots;
+    a.seq = keys;
+    a.splits = k_splits;
+    a.slots = (int32_t)k_slots;
     a.rows_h = g.HK;
-    const dim3 grid((unsigned)(slots * g.HK * a.splits));
+    const dim3 grid((unsigned)(k_slots * g.HK * a.splits));
     attn_by_dim(g.D, [&](auto nk) {
       constexpr int NK = decltype(nk)::value;
       if (a.splits > 1) hipLaunchKernelGGL((attn_dkv_kernel<NK, true>), grid, dim3(256), 0, st, a);

@@ -32,6 +32,9 @@ int launch_status(const char* what);
     }                                 \
   } while (0)
 
+// a launch has 32 bits of work items
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= 0xFFFFFFFFLL / threads; }
+
 // ---- integer helpers (wrap-around) -----------------------------------------
 CONCORD_DEV int32_t wadd(int32_t a, int32_t b) { return (int32_t)((uint32_t)a + (uint32_t)b); }
 CONCORD_DEV int32_t wsub(int32_t a, int32_t b) { return (int32_t)((uint32_t)a - (uint32_t)b); }

@@ -374,7 +374,7 @@ static void distill_split(DistillArgs& a, int splits) {
   a.seg = cdiv(cdiv(a.V, a.splits), 8) * 8;
   a.splits = (int)cdiv(a.V, a.seg);
 }
-static bool distill_fits(const DistillArgs& a) { return a.M * a.splits < (1LL << 31); }
+static bool distill_fits(const DistillArgs& a) { return grid_fits(a.M * a.splits, 256); }
 
 template <class T>
 static void distill_fwd(const DistillArgs& a, hipStream_t st) {

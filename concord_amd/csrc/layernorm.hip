@@ -541,6 +541,7 @@ extern "C" int concord_layernorm_bwd(const void* dy, int64_t ld_dy, const void* 
   CONCORD_CHECK(M == 0 || (dy && x && dx && mean && rstd), "concord_layernorm_bwd: NULL argument");
   hipStream_t st = (hipStream_t)stream;
   const bool cols = dweight || dbias;
+  CONCORD_CHECK(!cols || grid_fits(cdiv(2 * C, 64), 1024), "concord_layernorm_bwd: too many columns for their sums");
   if (M > 0) {
     if (cols && (!workspace || workspace_bytes < concord_layernorm_workspace_bytes(M, C))) {
       set_error("concord_layernorm_bwd: workspace of %zu bytes needed", concord_layernorm_workspace_bytes(M, C));

@@ -257,3 +257,31 @@ def test_a_module_that_fails_to_load_is_not_kept(monkeypatch):
     for n in ("layer_norm", "attention", "distill_loss"):
         assert callable(getattr(m, n)) and callable(getattr(seen[0], n)) and callable(getattr(whole, n))
     assert seen[0] is m and C.ops() is m
+
+
+def test_launches_past_the_grid_are_refused(L):
+    """A launch has 32 bits of work items: 2^24 workgroups of 256 are too many."""
+    from concord_amd import _lib as C
+    buf, most = ctypes.create_string_buffer(64), (2 ** 32 - 1) // 256
+    # dense: one tile a sequence and head; tables: TQ / 128 + B + 2 slots a head
+    for kw in (dict(B=(most + 16) // 16, TQ=(most + 16) // 16, TK=(most + 16) // 16, H=16, HK=16),
+               dict(B=1, TQ=2 ** 30, TK=64, H=64, HK=64),
+               dict(B=2 ** 23, TQ=2 ** 23, TK=2 ** 23, H=2, HK=1, starts=16)):
+        a = _attn_args(buf, **kw)
+        assert L.concord_attention_fwd(ctypes.byref(a), None, 0, None) == C.EINVAL, kw
+        assert b"too many tiles" in L.concord_last_error()
+        need = L.concord_attention_workspace_bytes(ctypes.byref(a))
+        assert L.concord_attention_bwd(ctypes.byref(a), buf, need, None) == C.EINVAL, kw
+        assert b"too many tiles" in L.concord_last_error()
+    # few queries, many keys: the backward's second launch
+    a = _attn_args(buf, B=1, TQ=1, TK=2 ** 30, H=64, HK=64)
+    need = L.concord_attention_workspace_bytes(ctypes.byref(a))
+    assert L.concord_attention_bwd(ctypes.byref(a), buf, need, None) == C.EINVAL
+    assert b"too many tiles" in L.concord_last_error()
+    # gradients of logits in segments; sums over the columns, 64 a workgroup of 1024
+    M, V, b = 2 ** 24 - 1, 20000, ctypes.addressof(buf) + 15 & ~15
+    assert L.concord_distill_bwd(b, 0, b, V, C.F32, M, V, b, 4, b, 4, 4, 1.0, b, b, V, None) == C.EINVAL
+    width = (2 ** 32 - 1) // 1024 * 32 + 32
+    need = L.concord_layernorm_workspace_bytes(1, width)
+    args = [b, width, b, width, C.F32, None, C.F32, b, b, 1, width, b, width, b, None, b, need, None]
+    assert L.concord_layernorm_bwd(*args) == C.EINVAL
