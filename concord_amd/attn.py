@@ -15,7 +15,10 @@ def attention(q, k, v, starts=None, k_starts=None, causal=True, scale=None):
 
     causal: query i of a sequence with Lq queries and Lk keys sees the keys up
     to i + Lk - Lq.  A query that sees no key, and one before starts[0] or
-    past starts[-1], gives 0.  scale: 1 / sqrt(dim) unless given.
+    past starts[-1], gives 0.  scale: 1 / sqrt(dim) unless given.  Other
+    sequences never show, whatever they hold; an infinity or NaN in a key or
+    value that the mask hides can reach queries of the same sequence whose last
+    key lies less than 96 before it (the step of 64 keys is shared by 32 queries).
 
     The values of starts are not read on the host: they must not decrease
     (positions past the tensors are taken as their ends).  Scores, softmax

@@ -458,7 +458,7 @@ inline void attn_by_dim(int D, F&& f) {
 // many as fill the chip with two (four with heads up to 64) workgroups a CU, of
 // four steps of 64 keys at least, while the shares' sums (8 bytes an element)
 // stay below a sixth of the launch's time as above (dkv_splits).  One query of
-// 32768 keys, 32 / 8 heads of 128: 466 us in one share, 67 us in 16.
+// 32768 keys, 32 / 8 heads of 128: 483 us in one share, 56 + 12 us in 16.
 inline int key_splits(const concord_attn_args& g, double flops) {
   if (g.TQ < 1 || g.TK < 1) return 1;
   AttnSeqs s = attn_seqs(g);

@@ -6,16 +6,15 @@
 // of each query's softmax.  Everything is transposed: a wave forms the scores
 // as k q^T, so a lane holds one query's column and the maximum, the sum and
 // the rescaling are lane-local (one exchange between the half waves for the
-// maximum); the probabilities, rounded to bf16 (a relative 2^-9 each, below
-// the rounding of out itself), are the B operand of out^T += v^T p without
-// leaving the lane.
+// maximum); the probabilities, rounded to bf16 (off by up to 2^-8 of themselves,
+// as out is by its own rounding; the matrix core takes no wider operand at this
+// rate), are the B operand of out^T += v^T p without leaving the lane.
 //
-// Bound by power: with every CU in MFMAs the clock falls to 1.6 - 1.75 GHz (a
-// small launch runs at 2.2).  2 x 8192 x 32 / 8 heads of 128 without a mask 1930
-// us, 1140 TFLOP/s, MFMA pipes busy 0.64 of the time; a library's 16384^3
+// Bound by power: with every CU in MFMAs the clock falls to 1.7 - 1.75 GHz (a
+// small launch runs at 2.1).  2 x 8192 x 32 / 8 heads of 128 without a mask 1985
+// us, 1108 TFLOP/s, MFMA pipes busy 0.62 of the time; a library's 16384^3
 // product reaches 1341 TFLOP/s here.  Heads of 64 have half the MFMAs to the
-// same exponentials: 2 x 4096 x 64 heads 539 us, 1020 TFLOP/s (up to 660 us
-// while the clock is lower).
+// same exponentials: 2 x 4096 x 64 heads 580 - 610 us, 900 - 950 TFLOP/s, busy 0.52.
 #include "attention.h"
 
 namespace concord {
@@ -216,8 +215,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnFwd a) {
     // Narrow heads have few MFMAs to an exponential, so past the first tile the
     // maximum is not even formed: m stays until a lane's 32 probabilities add up
     // to more than 2^20 (or to no number).  The scores are then formed again from
-    // the tile, which still lies in LDS, and m is raised.  (2 x 4096 x 64 heads of
-    // 64: 554 -> 539 us.)
+    // the tile, which still lies in LDS, and m is raised.  (2 x 4096 x 10 heads of
+    // 64: 112 -> 109.5 us; 64 heads: 600 us before, 582 and 609 in two runs since.)
     auto exps = [&](f32x16 (&s)[2]) CONCORD_INLINE_LAMBDA {
       float sum = 0.0f;
 #pragma unroll

@@ -10,8 +10,8 @@
 // of five.  dS is rounded to bf16 for its two products.
 //
 // dq is bound by power as the forward is: 2 x 8192 x 32 / 8 heads of 128 without a
-// mask 2720 us (three products, 1210 TFLOP/s), MFMA pipes busy 0.64.  dk / dv
-// take 3840 us (four products, 1145 TFLOP/s), busy 0.53: their sums fill the
+// mask 2800 us (three products, 1178 TFLOP/s), MFMA pipes busy 0.65.  dk / dv
+// take 3890 us (four products, 1131 TFLOP/s), busy 0.56: their sums fill the
 // registers of two waves per SIMD, which leaves few fragment reads in flight.
 #include "attention.h"
 
@@ -213,7 +213,8 @@ __global__ __launch_bounds__(256, NK <= 4 ? 3 : 2) void attn_dkv_kernel(AttnBwd 
       // P and dv, then dP, dS and dk; with wide heads kept in that order
       // (sched_barrier), the fewest values at a time.  A spilled register costs
       // more than its reload here, which waits for the DMA of the next step too
-      // (7 of them: 4416 us where 3900 us without, 2 x 8192 x 32 / 8 x 128).
+      // (15 packed sequences, 16384 tokens, 32 / 8 x 128: 1197 us with 7 of them, 1050
+      // without).
       bf16x8 e[2], es[2];
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AttnSum a) {
 // steps at least, and the shares' sums cost 16 bytes an element, which must stay
 // below a sixth of the launch's time (products at 1 PFLOP/s on a full chip, sums
 // at 5 TB/s; lengths are not known here, so the mean stands for them).  2 x 4096
-// causal, 32 / 8 heads of 128: the whole backward 1270 us in one share, 967 us.
+// causal, 32 / 8 heads of 128: the whole backward 1273 us in one share, 957 us.
 static int dkv_splits(const concord_attn_args& g) {
   if (g.TQ < 1 || g.TK < 1) return 1;
   AttnSeqs s = attn_seqs(g);

@@ -12,7 +12,7 @@
 //
 // Bound by memory: forward reads the logits once (running maximum and sum of
 // exponentials), backward reads them again and writes the gradient: 166 us (5.0
-// TB/s) and 296 us (5.6 TB/s: what the forward read last is still cached) at
+// TB/s) and 295 us (5.6 TB/s: what the forward read last is still cached) at
 // 8192 x 50257 bf16, where a copy moves 5.0 TB/s.  All statistics are fp32.  A
 // row is one wave's (V <= 1024), one block's, or is split over several blocks
 // when the rows are too few to fill the chip.
@@ -48,11 +48,12 @@ struct DistillArgs {
 struct MaxSum {
   float m, s;
 };
-// (an empty part has m = -inf, s = 0; a maximum of -inf gives factor 2^0)
+// (an empty part has m = -inf, s = 0, and is passed over wherever parts meet: its
+// factor would be 2^(-inf + inf), no number)
 CONCORD_DEV float rel_exp2(float z, float m, float c) { return __builtin_amdgcn_exp2f((z - m) * c); }
 CONCORD_DEV MaxSum join(MaxSum a, MaxSum b, float c) {
   const float m = fmaxf(a.m, b.m);
-  // an empty side adds nothing (its factor would be 2^(-inf + inf))
+  // an empty side adds nothing
   const float x = a.s == 0.0f ? 0.0f : a.s * rel_exp2(a.m, m, c);
   const float y = b.s == 0.0f ? 0.0f : b.s * rel_exp2(b.m, m, c);
   return MaxSum{m, x + y};
@@ -254,7 +255,8 @@ __global__ __launch_bounds__(256) void distill_join_kernel(DistillArgs a) {
 // (Measured at 8192 x 50257 bf16, K 64: entries read, and their logits gathered,
 // ahead of the pass, and a search that leaves the sum to the entries that
 // share a place, rows in segments of about 16 KB, so that the blocks in flight
-// sweep memory in order: 389 -> 319 us; with the last rows first 296.)
+// sweep memory in order: 344 -> 293 us.  With the last rows first 282, and the next
+// forward, which finds the first rows cached, 175 -> 163.)
 template <class T, int W>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
   constexpr int TH = W * 64, VEC = Span<T>::VEC, NE = W == 1 ? 1 : kTopMax / TH;
@@ -460,7 +462,7 @@ extern "C" int concord_distill_bwd(const float* dloss, int64_t ld_dloss, const v
   CONCORD_CHECK(dloss && stats && dlogits && ((uintptr_t)stats & 15) == 0,
                 "concord_distill_bwd: NULL argument or stats not on 16 bytes");
   a.g = dloss, a.ldg = ld_dloss, a.stat = (float*)stats, a.dz = dlogits, a.lddz = ld_d;
-  // (segments of about 16 KB; of 24 KB: 351 us)
+  // (segments of about 16 KB: forward and backward of 8192 x 50257 bf16 444 us; of 24 KB 451)
   distill_split(a, V <= kWaveRow ? 1 : (int)std::max<int64_t>(1, V * (dtype == CONCORD_F32 ? 4 : 2) / 16384));
   CONCORD_CHECK(distill_fits(a), "concord_distill_bwd: bad size");
   hipStream_t st = (hipStream_t)stream;

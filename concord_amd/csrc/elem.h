@@ -28,7 +28,8 @@ struct alignas(sizeof(T) * VEC) Chunk {
 };
 
 // a store of a result that this kernel does not read again: past the caches,
-// which keep the operands (layer norm of 32768 x 4096 bf16: 108 -> 88 us)
+// which keep the operands (layer norm in bf16, 16384 x 384: forward 9.5 -> 7.5 us;
+// 32768 x 4096: backward 160 -> 149 us, forward 96 either way)
 template <class V>
 CONCORD_DEV void store_stream(V* p, const V& v) {
   if constexpr (sizeof(V) == 16) {

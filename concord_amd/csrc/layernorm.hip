@@ -10,9 +10,10 @@
 // written once.  A row belongs to W waves (or 16 lanes of one) whose threads hold
 // E elements each at fixed columns, so the weight, the bias and the column sums of
 // dw and db stay in registers over all rows that a workgroup takes.  All sums
-// are fp32.  32768 x 4096 bf16: forward 87 us (6.1 TB/s), backward 150 us (5.4
-// TB/s, its second kernel included), where a 1 GiB copy moves 5.0 TB/s;
-// 16384 x 384: 6.8 and 14.1 us, near the cost of a launch and its latencies.
+// are fp32.  Kernel times in a trace, 32768 x 4096 bf16: forward 97 us (5.5 TB/s),
+// backward 155 us (5.2 TB/s, its second kernel included), where a 1 GiB copy moves
+// 5.0 TB/s; 16384 x 384: 7.8 and 15.9 us, near the cost of the launches and their
+// latencies.
 #include "elem.h"
 
 namespace concord {

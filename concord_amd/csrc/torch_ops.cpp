@@ -3,9 +3,9 @@
 //
 // A training step calls these operators many times on few tokens' work, and
 // the launches of a small one take less time than an autograd node written in
-// Python takes to run (layer norm of 16384 x 384, forward and backward: 34 us
-// of kernels, 127 us a pass from Python): the nodes are C++ for that reason
-// alone.  They check arguments, hand out memory from torch's allocator on the
+// Python takes to run (layer norm of 16384 x 384, forward and backward: 23 us
+// of kernels; when they took 34, a pass from Python took 127 us, from C++ 65): the
+// nodes are C++ for that reason alone.  They check arguments, hand out memory from torch's allocator on the
 // current stream and call the entries; the C++ exceptions thrown here become
 // Python's (ValueError, TypeError, RuntimeError).
 #include <c10/core/AutogradState.h>
