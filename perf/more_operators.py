@@ -410,7 +410,8 @@ def _exact_gelu(x, tanh):
         du = math.sqrt(2.0 / math.pi) * (1.0 + 0.134145 * x ** 2)
         return 0.5 * x * (1.0 + t), 0.5 * (1.0 + t) + 0.5 * x * (1.0 - t * t) * du
     phi = torch.exp(-x * x / 2.0) * (2.0 * math.pi) ** -0.5
-    return x * torch.special.ndtr(x), torch.special.ndtr(x) + x * phi
+    cdf = torch.special.erfc(-x / 2.0 ** 0.5) / 2.0   # (1 + erf, or ndtr, loses the left tail)
+    return x * cdf, cdf + x * phi
 
 
 def _exact_act(s):
