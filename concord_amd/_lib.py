@@ -69,6 +69,17 @@ class AttnArgs(ctypes.Structure):
                 [(n, ctypes.c_int64) for n in ("dq_t", "dq_h", "dk_t", "dk_h", "dv_t", "dv_h")])
 
 
+class QkArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k")] + [(n, ctypes.c_int64) for n in ("q_t", "q_h", "k_t", "k_h")] +
+                [(n, ctypes.c_void_p) for n in ("q_out", "k_out", "q_weight", "k_weight", "positions")] +
+                [(n, ctypes.c_int64) for n in ("T", "seq", "pos_seq")] +
+                [(n, ctypes.c_int32) for n in ("H", "HK", "D", "R", "adjacent", "pos64", "dtype", "wtype")] +
+                [("eps", ctypes.c_float), ("base", ctypes.c_double)] +
+                [(n, ctypes.c_void_p) for n in ("dq_out", "dk_out")] +
+                [(n, ctypes.c_int64) for n in ("dq_t", "dq_h", "dk_t", "dk_h")] +
+                [(n, ctypes.c_void_p) for n in ("dq", "dk", "dq_weight", "dk_weight")])
+
+
 # (name, restype, argtypes); P = pointer, I = int64, i = int32, F = float, D = double
 _P, _I, _i, _F, _D, _Z = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float,
                           ctypes.c_double, ctypes.c_size_t)
@@ -154,6 +165,20 @@ _SIGS = {
     "concord_attention_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P, _Z, _P]),
     "concord_attention_workspace_bytes": (_Z, [ctypes.POINTER(AttnArgs)]),
     "concord_attention_bwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), _P, _Z, _P]),
+    "concord_embedding_fwd": (ctypes.c_int, [_P, ctypes.c_int, _I, _P, _I, ctypes.c_int, _I, _I, _F, _P, _I,
+                                             ctypes.c_int, _P]),
+    "concord_embedding_workspace_bytes": (_Z, [_I, _I, _I]),
+    "concord_embedding_bwd": (ctypes.c_int, [_P, ctypes.c_int, _I, _P, _I, ctypes.c_int, _I, _I, _F, _P, _I,
+                                             ctypes.c_int, _P, _Z, _P]),
+    "concord_qk_norm_rope_fwd": (ctypes.c_int, [ctypes.POINTER(QkArgs), _P]),
+    "concord_qk_norm_rope_workspace_bytes": (_Z, [ctypes.POINTER(QkArgs)]),
+    "concord_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(QkArgs), _P, _Z, _P]),
+    "concord_pack8": (ctypes.c_int, [_P, _I, ctypes.c_int, _I, _I, _P, _P, _P]),
+    "concord_unpack8": (ctypes.c_int, [_P, _P, _I, _I, _P, _I, ctypes.c_int, _P]),
+    "concord_gelu8_fwd": (ctypes.c_int, [_P, _I, ctypes.c_int, _I, _I, ctypes.c_int, ctypes.c_int, _P, _I, _P, _P,
+                                         _P]),
+    "concord_gelu8_bwd": (ctypes.c_int, [_P, _I, _P, _P, ctypes.c_int, _I, _I, ctypes.c_int, ctypes.c_int, _P, _I,
+                                         _P]),
 }
 
 _lib = None

@@ -12,7 +12,7 @@ ordinary VGPRs (-amdgpu-mfma-vgpr-form); its kernels are written to fit them,
 and the accumulator-register form made the compiler copy accumulators
 around the main loops.
 
-torch_ops.cpp (host code: autograd nodes over the library's entries) becomes
+torch_ops*.cpp (host code: autograd nodes over the library's entries) become
 concord_amd/_lib/concord_torch_ops.so, against the installed torch.  Where that
 fails the build does, with the C library in place.
 """
@@ -71,21 +71,22 @@ def build(verbose=False, jobs=8):
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     objs = [os.path.join(OUT_DIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
 
-    ops_src, ops_obj = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(OUT_DIR, "torch_ops.o")
+    ops_srcs = sorted(glob.glob(os.path.join(CSRC, "torch_ops*.cpp")))
+    ops_objs = [os.path.join(OUT_DIR, os.path.basename(s)[:-4] + ".o") for s in ops_srcs]
 
     def compile_one(s, o):
         return _run([HIPCC] + CFLAGS + FILE_FLAGS.get(os.path.basename(s), []) + ["-c", s, "-o", o])
 
-    def compile_ops():
+    def compile_ops(s, o):
         cflags, libs = _ops_flags()
-        return _run([CXX] + cflags + ["-c", ops_src, "-o", ops_obj]), libs
+        return _run([CXX] + cflags + ["-c", s, "-o", o]), libs
 
     def show(msg):
         if verbose and msg.strip():
             print(msg, file=sys.stderr)
 
     with ThreadPoolExecutor(max_workers=jobs) as ex:
-        ops = ex.submit(compile_ops)
+        ops = [ex.submit(compile_ops, s, o) for s, o in zip(ops_srcs, ops_objs)]
         for msg in ex.map(compile_one, srcs, objs):
             show(msg)
         # the C library first: a binding without torch needs neither g++ nor torch's headers
@@ -94,11 +95,13 @@ def build(verbose=False, jobs=8):
         os.replace(tmp, LIB)
         for o in objs:
             os.remove(o)
-        msg, ops_libs = ops.result()
-        show(msg)
-    _run([CXX, "-shared", "-o", OPS + ".tmp", ops_obj] + ops_libs)
+        for job in ops:
+            msg, ops_libs = job.result()
+            show(msg)
+    _run([CXX, "-shared", "-o", OPS + ".tmp"] + ops_objs + ops_libs)
     os.replace(OPS + ".tmp", OPS)
-    os.remove(ops_obj)
+    for o in ops_objs:
+        os.remove(o)
     if verbose:
         print(f"built {LIB} and {OPS}")
     return LIB

@@ -1,0 +1,132 @@
+// act8.h -- activations in 8 bits, and the functions whose input is kept so.
+//
+// 32 adjacent values of a row (a block; a row's last one may be shorter) share a
+// step 2^e, the smallest power of two with max|x| <= 127 2^e and e >= -126:
+//   code = x 2^-e rounded half to even, -127 .. 127;   exponent byte = e + 127 (1 .. 249)
+//   value = code 2^e, limited to the type's largest finite number
+// Scaling by a power of two is exact, so the codes have one definition whatever
+// computes them, each value is off by at most half a step (2^-7 of the block's
+// largest), and one significant byte fits bf16 and fp16 without a further rounding.
+// A block that holds an infinity or NaN has exponent byte 255 and codes 0: all of it
+// reads back as NaN.
+#pragma once
+#include "elem.h"
+
+namespace concord {
+
+constexpr int kBlock8 = 32;
+constexpr uint32_t kBad8 = 255;
+
+CONCORD_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// exponent byte of a block whose largest magnitude has these bits: the exponent
+// less 6, one more where the mantissa is above 127 / 64
+CONCORD_DEV uint32_t exponent8(uint32_t top) {
+  return top >= 0x7F800000u ? kBad8 : max((int)((top + 0x1FFFFu) >> 23) - 6, 1);
+}
+// 1 / step (byte 255: not used)
+CONCORD_DEV float inverse_step8(uint32_t e8) { return __uint_as_float((254u - e8) << 23); }
+CONCORD_DEV float step8(uint32_t e8) { return __uint_as_float(e8 << 23); }   // (byte 255: infinity)
+
+// the low byte of 1.5 2^23 + x / step is the code: the sum rounds half to even
+CONCORD_DEV uint32_t code8(float x, float inv) { return __float_as_uint(__builtin_fmaf(x, inv, 12582912.0f)); }
+
+// four codes, in order (0: those of a block without a step)
+CONCORD_DEV uint32_t codes8(const float* x, float inv, bool bad) {
+  const uint32_t lo = __builtin_amdgcn_perm(code8(x[1], inv), code8(x[0], inv), 0x0C0C0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(code8(x[3], inv), code8(x[2], inv), 0x0C0C0400u);
+  return bad ? 0u : lo | hi << 16;
+}
+
+template <class T>
+struct Largest;   // the type's largest finite number, and the exponent byte from which 127 steps exceed it
+template <>
+struct Largest<float> {
+  static constexpr float value = 3.4028234663852886e38f;
+  static constexpr uint32_t e8 = 249;
+};
+template <>
+struct Largest<BF16> {
+  static constexpr float value = 3.3895313892515355e38f;
+  static constexpr uint32_t e8 = 249;
+};
+template <>
+struct Largest<_Float16> {
+  static constexpr float value = 65504.0f;
+  static constexpr uint32_t e8 = 137;
+};
+
+// code times step, as a value of T; NaN for a block of byte 255 (0 times infinity)
+template <class T>
+CONCORD_DEV float value8(int code, float step, bool large) {
+  float v = (float)code * step;
+  if (large) v = fabsf(v) > Largest<T>::value ? copysignf(Largest<T>::value, v) : v;
+  return v;
+}
+
+// ---- gelu ---------------------------------------------------------------------
+// Phi(x), the normal distribution, and its density times x where that is wanted.
+// With a = |x|: Phi(-a) = exp(-a^2 / 2) q(a), and q, half of the scaled
+// complementary error function of a / sqrt(2), is t P(t) with t = 1 / (1 + 0.35 a),
+// P of degree 8 fitted to q's values (relative error 3.2e-8 for a up to 17).  The
+// exponent's rounding is taken back with its remainder: in all 4e-7 of Phi(-a), also
+// far out, where 1 + erf would have lost every digit.
+struct Gelu {
+  static CONCORD_DEV void parts(float x, float& cdf, float& xpdf) {
+    const float a = fabsf(x), s = a * a, rest = __builtin_fmaf(a, a, -s);
+    const float y = s * -0.72134752f;
+    const float lost = __builtin_fmaf(s, -0.72134752f, -y) + __builtin_fmaf(rest, -0.72134752f, s * -9.6298149e-9f);
+    float e = __builtin_amdgcn_exp2f(y);
+    e = __builtin_fmaf(e, lost * 0.69314718f, e);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, a, 1.0f));
+    float p = __builtin_fmaf(-0.029165321961045265f, t, 0.14406773447990417f);
+    p = __builtin_fmaf(p, t, -0.2559165060520172f);
+    p = __builtin_fmaf(p, t, 0.1594100296497345f);
+    p = __builtin_fmaf(p, t, -0.02327592857182026f);
+    p = __builtin_fmaf(p, t, 0.10558006167411804f);
+    p = __builtin_fmaf(p, t, 0.11981412768363953f);
+    p = __builtin_fmaf(p, t, 0.13986453413963318f);
+    p = __builtin_fmaf(p, t, 0.13962124288082123f);
+    const float tail = p * t * e;
+    cdf = x < 0.0f ? tail : 1.0f - tail;
+    xpdf = x * e * 0.3989422804f;
+  }
+  static CONCORD_DEV float limit(float x) { return fabsf(x) > 16.0f ? copysignf(16.0f, x) : x; }   // (NaN stays)
+  static CONCORD_DEV float value(float x) {
+    float cdf, xpdf;
+    parts(limit(x), cdf, xpdf);
+    return x * cdf;
+  }
+  static CONCORD_DEV void both(float x, float& v, float& d) {
+    float cdf, xpdf;
+    parts(limit(x), cdf, xpdf);
+    v = x * cdf;
+    d = cdf + xpdf;
+  }
+};
+
+// x (1 + tanh(u)) / 2 = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3).
+// Past |x| = 16 the sigmoid is 0 or 1 to the last bit, and x^3 would overflow.
+struct GeluTanh {
+  // e = exp(-2 u), sig = 1 / (1 + e)
+  static CONCORD_DEV void parts(float x, float& e, float& sig) {
+    e = __builtin_amdgcn_exp2f(x * __builtin_fmaf(x * x, -0.1029432397f, -2.302208198f));
+    sig = __builtin_amdgcn_rcpf(1.0f + e);
+  }
+  static CONCORD_DEV float value(float x) {
+    float e, sig;
+    parts(Gelu::limit(x), e, sig);
+    return x * sig;
+  }
+  static CONCORD_DEV void both(float x, float& v, float& d) {
+    float e, sig;
+    const float c = Gelu::limit(x);
+    parts(c, e, sig);
+    v = x * sig;
+    // sig + x sig (1 - sig) 2 u'; 1 - sig = e sig keeps its digits where sig is near 1
+    const float rest = c > 0.0f ? e * sig : 1.0f - sig;
+    d = __builtin_fmaf(c * sig * rest, __builtin_fmaf(c * c, 0.2140644488f, 1.5957691216f), sig);
+  }
+};
+
+}  // namespace concord

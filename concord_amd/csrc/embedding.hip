@@ -1,0 +1,537 @@
+// embedding.hip -- rows of a table by token, scaled, and the table's gradient by
+// sorted tokens.
+//
+//   y[i] = s W[t_i];   dW[v] = s sum over { i : t_i = v } of dy[i]
+//
+// Both passes are bound by memory: the forward reads the rows it names and
+// writes the result, the backward reads dy and writes the whole table's gradient,
+// zeros included.
+//
+// The backward sorts (token, position) pairs by token, stably, with a radix sort
+// of up to 9 bits a pass; a token's rows then stand one after another, in the
+// order of their positions.  The sorted pairs are cut into pieces of equal
+// length, whatever the tokens' counts, and each wave adds the rows of a piece for
+// one slab of columns in registers.  A token inside one piece is stored at once;
+// one that crosses pieces leaves its sums in the workspace, and a second kernel
+// adds those in order.  No sum depends on the order in which waves run: there are
+// no atomics on floating point numbers.
+#include "elem.h"
+
+namespace concord {
+
+constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
+constexpr int kTile = 4096;          // pairs a block of the sort takes
+constexpr int kOneBlock = 4096;      // pairs that one block sorts alone
+
+struct EmbArgs {
+  const void* tokens;
+  int idx64;
+  int64_t n;            // < 2^31
+  uint32_t V;
+  int64_t C;
+  float scale;
+  const void* src;      // the table, or dy
+  int64_t lds;
+  void* dst;            // y, or dW
+  int64_t ldd;
+  const uint32_t* keys; // sorted tokens, V for those outside the table
+  const uint32_t* pos;  // their positions
+  float* part;          // [pieces][2][C]: sums of a run's head (it began earlier), of its first rows
+  int piece;            // pairs a wave adds
+  int64_t pieces;
+  int64_t fill_at;      // first block of those that write zeros
+};
+
+CONCORD_DEV uint32_t token_key(const void* tokens, int idx64, int64_t i, uint32_t V) {
+  const int64_t t = idx64 ? ((const int64_t*)tokens)[i] : (int64_t)((const int32_t*)tokens)[i];
+  return (uint64_t)t < V ? (uint32_t)t : V;
+}
+
+// ---- forward ------------------------------------------------------------------
+// 2^lg threads a row, VEC columns a thread and step
+template <class TW, class TO, int VEC>
+__global__ __launch_bounds__(256) void emb_fwd_kernel(EmbArgs a, int lg) {
+  const int64_t step = (int64_t)gridDim.x << (8 - lg);
+  for (int64_t row = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg); row < a.n; row += step) {
+    const uint32_t t = token_key(a.tokens, a.idx64, row, a.V);
+    const bool there = t < a.V;
+    const TW* src = (const TW*)a.src + (int64_t)(there ? t : 0) * a.lds;
+    TO* dst = (TO*)a.dst + row * a.ldd;
+    for (int64_t c = (int64_t)(threadIdx.x & ((1 << lg) - 1)) * VEC; c < a.C; c += (int64_t)VEC << lg) {
+      Chunk<TW, VEC> v = {};
+      if (there) v = *(const Chunk<TW, VEC>*)(src + c);
+      Chunk<TO, VEC> r;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<TO>(to_f32(v.v[e]) * a.scale);
+      *(Chunk<TO, VEC>*)(dst + c) = r;
+    }
+  }
+}
+
+// ---- sort -----------------------------------------------------------------------
+// lanes of the wave whose digit of `bits` bits is this lane's
+CONCORD_DEV uint64_t same_digit(uint32_t d, int bits) {
+  uint64_t m = ~0ull;
+  for (int b = 0; b < bits; ++b) {
+    const bool bit = (d >> b) & 1;
+    const uint64_t set = __builtin_amdgcn_ballot_w64(bit);
+    m &= bit ? set : ~set;
+  }
+  return m;
+}
+// how many of the wave's earlier pairs have the digit d: counts, one for each digit, goes on from step to step
+CONCORD_DEV uint32_t digit_rank(uint32_t* counts, uint32_t d, int bits) {
+  const uint64_t m = same_digit(d, bits);
+  const uint32_t before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  const uint32_t prior = counts[d];
+  __builtin_amdgcn_wave_barrier();
+  if (before == 0) counts[d] = prior + (uint32_t)__builtin_popcountll(m);
+  __builtin_amdgcn_wave_barrier();
+  return prior + before;
+}
+
+// exclusive sums over the block's first `bins` threads' values (W waves; all threads call)
+template <int W>
+CONCORD_DEV uint32_t block_exclusive(uint32_t v, uint32_t (&sums)[W]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t s = v;
+#pragma unroll
+  for (int h = 1; h < 64; h <<= 1) {
+    const uint32_t o = __shfl_up(s, h, 64);
+    if (lane >= h) s += o;
+  }
+  if (lane == 63) sums[wave] = s;
+  __syncthreads();
+  uint32_t base = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) base += w < wave ? sums[w] : 0;
+  return base + s - v;
+}
+
+// All of up to IT * 1024 pairs in one block: pair e belongs to wave e / (64 IT).
+template <int IT>
+__global__ __launch_bounds__(1024) void emb_sort_block_kernel(EmbArgs a, int passes, int bits, uint32_t* keys,
+                                                             uint32_t* pos) {
+  __shared__ uint32_t lk[IT * 1024], lp[IT * 1024], cnt[16][kMaxBins], sums[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << bits;
+  const int e0 = wave * IT * 64 + lane, n = (int)a.n;
+  uint32_t k[IT], p[IT], rank[IT];
+#pragma unroll
+  for (int j = 0; j < IT; ++j) {
+    const int e = e0 + j * 64;
+    // (behind the last pair: the largest digits, so they stay behind it)
+    k[j] = e < n ? token_key(a.tokens, a.idx64, e, a.V) : 0xFFFFFFFFu;
+    p[j] = (uint32_t)e;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    for (int i = lane; i < bins; i += 64) cnt[wave][i] = 0;
+    __builtin_amdgcn_wave_barrier();
+    const int shift = pass * bits;
+#pragma unroll
+    for (int j = 0; j < IT; ++j) rank[j] = digit_rank(cnt[wave], (k[j] >> shift) & (bins - 1), bits);
+    __syncthreads();
+    uint32_t total = 0;
+    if ((int)threadIdx.x < bins) {
+#pragma unroll
+      for (int w = 0; w < 16; ++w) total += cnt[w][threadIdx.x];
+    }
+    uint32_t at = block_exclusive<16>(total, sums);
+    if ((int)threadIdx.x < bins) {
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const uint32_t c = cnt[w][threadIdx.x];
+        cnt[w][threadIdx.x] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+      const uint32_t dst = cnt[wave][(k[j] >> shift) & (bins - 1)] + rank[j];
+      lk[dst] = k[j];
+      lp[dst] = p[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+      k[j] = lk[e0 + j * 64];
+      p[j] = lp[e0 + j * 64];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < IT; ++j)
+    if (e0 + j * 64 < n) {
+      keys[e0 + j * 64] = k[j];
+      pos[e0 + j * 64] = p[j];
+    }
+}
+
+// One pass over many blocks, kTile pairs each: the digits' counts of each block ...
+struct SortPass {
+  const uint32_t *keys, *pos;   // NULL in the first pass: the tokens
+  uint32_t *out_keys, *out_pos;
+  uint32_t* counts;             // [blocks][bins]
+  int shift, bits;
+};
+__global__ __launch_bounds__(512) void emb_count_kernel(EmbArgs a, SortPass s) {
+  __shared__ uint32_t cnt[kMaxBins];
+  const int bins = 1 << s.bits;
+  if ((int)threadIdx.x < bins) cnt[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+  for (int j = 0; j < kTile / 512; ++j) {
+    const int64_t i = first + j * 512 + threadIdx.x;
+    if (i < a.n) {
+      const uint32_t k = s.keys ? s.keys[i] : token_key(a.tokens, a.idx64, i, a.V);
+      atomicAdd(&cnt[(k >> s.shift) & (bins - 1)], 1u);
+    }
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < bins) s.counts[(int64_t)blockIdx.x * bins + threadIdx.x] = cnt[threadIdx.x];
+}
+// ... and the pairs to their places: behind all smaller digits, behind the same digit of earlier blocks
+__global__ __launch_bounds__(512) void emb_scatter_kernel(EmbArgs a, SortPass s) {
+  constexpr int IT = kTile / 512;
+  __shared__ uint32_t cnt[8][kMaxBins], sums[8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << s.bits;
+  const int64_t e0 = (int64_t)blockIdx.x * kTile + wave * IT * 64 + lane;
+  uint32_t k[IT], p[IT], rank[IT];
+#pragma unroll
+  for (int j = 0; j < IT; ++j) {
+    const int64_t i = e0 + j * 64;
+    const bool in = i < a.n;
+    k[j] = !in ? 0xFFFFFFFFu : s.keys ? s.keys[i] : token_key(a.tokens, a.idx64, i, a.V);
+    p[j] = in && s.pos ? s.pos[i] : (uint32_t)i;
+  }
+  uint32_t before = 0, all = 0;
+  if ((int)threadIdx.x < bins) {
+    const uint32_t* c = s.counts + threadIdx.x;
+    for (int64_t b = 0; b < gridDim.x; ++b) {
+      const uint32_t v = c[b * bins];
+      before += b < blockIdx.x ? v : 0;
+      all += v;
+    }
+  }
+  for (int i = lane; i < bins; i += 64) cnt[wave][i] = 0;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < IT; ++j) rank[j] = digit_rank(cnt[wave], (k[j] >> s.shift) & (bins - 1), s.bits);
+  uint32_t at = block_exclusive<8>(all, sums) + before;   // (its barrier stands between the counts and their use)
+  if ((int)threadIdx.x < bins) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint32_t c = cnt[w][threadIdx.x];
+      cnt[w][threadIdx.x] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < IT; ++j) {
+    // (what stands for no pair is counted last of the last block: nothing comes after it)
+    if (e0 + j * 64 >= a.n) continue;
+    const uint32_t dst = cnt[wave][(k[j] >> s.shift) & (bins - 1)] + rank[j];
+    s.out_keys[dst] = k[j];
+    s.out_pos[dst] = p[j];
+  }
+}
+
+// ---- sums -------------------------------------------------------------------------
+// one row of the gradient, or zeros
+template <class TW, int VEC>
+CONCORD_DEV void store_row(const EmbArgs& a, uint32_t v, int64_t c, const float (&s)[VEC]) {
+  if (c >= a.C) return;
+  Chunk<TW, VEC> r;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<TW>(s[e] * a.scale);
+  *(Chunk<TW, VEC>*)((TW*)a.dst + (int64_t)v * a.ldd + c) = r;
+}
+template <int VEC>
+CONCORD_DEV void store_part(const EmbArgs& a, int64_t piece, int which, int64_t c, const float (&s)[VEC]) {
+  if (c >= a.C) return;
+  float* p = a.part + (piece * 2 + which) * a.C + c;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) p[e] = s[e];
+}
+
+// first of keys[lo, hi) that is not less than v
+CONCORD_DEV int64_t first_not_less(const uint32_t* keys, int64_t lo, int64_t hi, uint32_t v) {
+  while (lo < hi) {
+    const int64_t m = (lo + hi) >> 1;
+    if (keys[m] < v) lo = m + 1;
+    else hi = m;
+  }
+  return lo;
+}
+
+constexpr int kFillRows = 16;   // rows of the table that a wave looks at for zeros
+
+template <class TG, class TW, int VEC>
+__global__ __launch_bounds__(256) void emb_sum_kernel(EmbArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if ((int64_t)blockIdx.x >= a.fill_at) {
+    // rows of the table without a token (each lane looks for one)
+    const int64_t v0 = (((int64_t)blockIdx.x - a.fill_at) * 4 + wave) * kFillRows;
+    const int64_t v = v0 + (lane & (kFillRows - 1));
+    bool empty = false;
+    if (v < a.V) {
+      const int64_t at = first_not_less(a.keys, 0, a.n, (uint32_t)v);
+      empty = at >= a.n || a.keys[at] != (uint32_t)v;
+    }
+    uint64_t todo = __builtin_amdgcn_ballot_w64(empty) & ((1u << kFillRows) - 1);
+    const float zero[VEC] = {};
+    while (todo) {
+      const int i = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      for (int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC; c < a.C; c += (int64_t)gridDim.y * 64 * VEC)
+        store_row<TW, VEC>(a, (uint32_t)(v0 + i), c, zero);
+    }
+    return;
+  }
+  const int64_t piece = (int64_t)blockIdx.x * 4 + wave;
+  if (piece >= a.pieces) return;
+  const int64_t p0 = piece * a.piece, p1 = min(p0 + a.piece, a.n);
+  const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC;
+  uint32_t cur = a.keys[p0];
+  bool head = p0 > 0 && a.keys[p0 - 1] == cur;
+  float s[VEC] = {};
+  constexpr int U = 8;
+  for (int64_t i = p0; i < p1 && cur < a.V; i += U) {
+    Chunk<TG, VEC> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = {};
+      if (i + u < p1 && c < a.C)
+        r[u] = *(const Chunk<TG, VEC>*)((const TG*)a.src + (int64_t)a.pos[i + u] * a.lds + c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u < p1 && cur < a.V) {
+        const uint32_t k = a.keys[i + u];
+        if (k != cur) {
+          if (head) store_part<VEC>(a, piece, 0, c, s);
+          else store_row<TW, VEC>(a, cur, c, s);
+          head = false;
+          cur = k;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += to_f32(r[u].v[e]);
+      }
+    }
+  }
+  if (cur >= a.V) return;   // (tokens outside the table stand last)
+  const bool goes_on = p1 < a.n && a.keys[p1] == cur;
+  if (head) store_part<VEC>(a, piece, 0, c, s);
+  else if (goes_on) store_part<VEC>(a, piece, 1, c, s);
+  else store_row<TW, VEC>(a, cur, c, s);
+}
+
+// Tokens that cross pieces: the block of the piece that such a run begins in
+// adds its sums, each wave every fourth of them, then the waves' sums in order.
+template <class TW, int VEC>
+__global__ __launch_bounds__(256) void emb_join_kernel(EmbArgs a) {
+  __shared__ float part[4][64 * VEC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t piece = blockIdx.x, p0 = piece * a.piece, p1 = p0 + a.piece;
+  if (p1 >= a.n) return;
+  const uint32_t cur = a.keys[p1 - 1];
+  if (cur >= a.V || a.keys[p1] != cur) return;
+  if (p0 > 0 && a.keys[p0 - 1] == cur) return;   // it began earlier
+  const int64_t last = (first_not_less(a.keys, p1, a.n, cur + 1) - 1) / a.piece;
+  const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC;
+  float s[VEC] = {};
+  if (c < a.C) {
+    for (int64_t q = piece + 1 + wave; q <= last; q += 4) {
+      const float* h = a.part + q * 2 * a.C + c;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] += h[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) part[wave][lane * VEC + e] = s[e];
+  __syncthreads();
+  if (wave == 0 && c < a.C) {
+    const float* t = a.part + (piece * 2 + 1) * a.C + c;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      s[e] = t[e];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) s[e] += part[w][lane * VEC + e];
+    }
+    store_row<TW, VEC>(a, cur, c, s);
+  }
+}
+
+// ---- host -------------------------------------------------------------------
+static bool emb_dtype_ok(int t) { return t == CONCORD_F32 || t == CONCORD_BF16 || t == CONCORD_F16; }
+static size_t emb_size(int t) { return t == CONCORD_F32 ? 4 : 2; }
+
+// pairs a wave adds: as many as leave about 4096 waves
+static int emb_piece(int64_t n, int64_t C) {
+  const int64_t waves = n * cdiv(C, 256);
+  int p = 8;
+  while (p < 256 && waves / p > 4096) p *= 2;
+  return p;
+}
+
+struct EmbWorkspace {
+  size_t keys[2], pos[2], counts, part, bytes;
+};
+static EmbWorkspace emb_workspace(int64_t n, int64_t C) {
+  EmbWorkspace w{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t r = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return r;
+  };
+  for (int i = 0; i < 2; ++i) {
+    w.keys[i] = take((size_t)n * 4);
+    w.pos[i] = take((size_t)n * 4);
+  }
+  w.counts = take((size_t)cdiv(n, kTile) * kMaxBins * 4);
+  w.part = take((size_t)cdiv(n, emb_piece(n, C)) * 2 * (size_t)C * 4);
+  w.bytes = at;
+  return w;
+}
+
+static bool emb_chunked(const void* p, int64_t ld, size_t bytes, size_t es) {
+  return ((uintptr_t)p & (bytes - 1)) == 0 && (ld * es) % bytes == 0;
+}
+
+template <class TA, class TB>
+struct EmbVec {
+  // columns of a lane and step: 16 bytes of the narrower type
+  static constexpr int V = sizeof(TA) == 2 || sizeof(TB) == 2 ? 8 : 4;
+};
+
+template <class TW, class TO>
+static void emb_fwd(const EmbArgs& a, hipStream_t st) {
+  constexpr int V = EmbVec<TW, TO>::V;
+  const bool vec = a.C % V == 0 && emb_chunked(a.src, a.lds, 16, sizeof(TW)) && emb_chunked(a.dst, a.ldd, 16, sizeof(TO));
+  const int64_t steps = vec ? a.C / V : a.C;
+  int lg = 0;
+  while (lg < 8 && (1 << lg) < steps) ++lg;
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.n, 256 >> lg), 1 << 20));
+  if (vec) hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, V>), grid, dim3(256), 0, st, a, lg);
+  else hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, 1>), grid, dim3(256), 0, st, a, lg);
+}
+
+template <class TG, class TW, int V>
+static void emb_sums(EmbArgs& a, hipStream_t st) {
+  const unsigned slabs = (unsigned)cdiv(a.C, 64 * V);
+  a.fill_at = cdiv(a.pieces, 4);
+  hipLaunchKernelGGL((emb_sum_kernel<TG, TW, V>), dim3((unsigned)(a.fill_at + cdiv(a.V, 4 * kFillRows)), slabs), dim3(256),
+                     0, st, a);
+  if (a.pieces > 1)
+    hipLaunchKernelGGL((emb_join_kernel<TW, V>), dim3((unsigned)a.pieces, slabs), dim3(256), 0, st, a);
+}
+template <class TG, class TW>
+static void emb_bwd(EmbArgs& a, hipStream_t st) {
+  constexpr int V = EmbVec<TG, TW>::V;
+  if (a.C % V == 0 && emb_chunked(a.src, a.lds, 16, sizeof(TG)) && emb_chunked(a.dst, a.ldd, 16, sizeof(TW)))
+    emb_sums<TG, TW, V>(a, st);
+  else
+    emb_sums<TG, TW, 1>(a, st);
+}
+
+// f<A, B>() for two of the three types
+template <class A, class F>
+static void emb_type2(int b, F&& f) {
+  if (b == CONCORD_F32) f(A{}, float{});
+  else if (b == CONCORD_BF16) f(A{}, BF16{});
+  else f(A{}, (_Float16)0);
+}
+template <class F>
+static void emb_types(int a, int b, F&& f) {
+  if (a == CONCORD_F32) emb_type2<float>(b, f);
+  else if (a == CONCORD_BF16) emb_type2<BF16>(b, f);
+  else emb_type2<_Float16>(b, f);
+}
+
+static bool emb_sizes_ok(int64_t n, int64_t V, int64_t C) {
+  return n >= 0 && V >= 0 && C >= 1 && n < (1LL << 31) && V < (1LL << 31) - 1 && C < (1LL << 21);
+}
+
+}  // namespace concord
+
+using namespace concord;
+
+extern "C" int concord_embedding_fwd(const void* tokens, int index64, int64_t n, const void* table, int64_t ld_t,
+                                     int wdtype, int64_t V, int64_t C, float scale, void* out, int64_t ld_o, int dtype,
+                                     void* stream) {
+  CONCORD_CHECK(emb_sizes_ok(n, V, C), "concord_embedding_fwd: bad size");
+  CONCORD_CHECK(emb_dtype_ok(dtype) && emb_dtype_ok(wdtype), "concord_embedding_fwd: bad type");
+  CONCORD_CHECK(ld_t >= C && ld_o >= C, "concord_embedding_fwd: leading dimension < C");
+  if (n == 0) return CONCORD_OK;
+  CONCORD_CHECK(tokens && out && (table || V == 0), "concord_embedding_fwd: NULL argument");
+  EmbArgs a{};
+  a.tokens = tokens, a.idx64 = index64, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
+  a.src = table, a.lds = ld_t, a.dst = out, a.ldd = ld_o;
+  emb_types(wdtype, dtype, [&](auto w, auto o) { emb_fwd<decltype(w), decltype(o)>(a, (hipStream_t)stream); });
+  return launch_status("embedding_fwd");
+}
+
+extern "C" size_t concord_embedding_workspace_bytes(int64_t n, int64_t V, int64_t C) {
+  if (!emb_sizes_ok(n, V, C) || n == 0 || V == 0) return 0;
+  return emb_workspace(n, C).bytes;
+}
+
+extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n, const void* dy, int64_t ld_dy, int dtype,
+                                     int64_t V, int64_t C, float scale, void* dtable, int64_t ld_dt, int wdtype,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  CONCORD_CHECK(emb_sizes_ok(n, V, C), "concord_embedding_bwd: bad size");
+  CONCORD_CHECK(emb_dtype_ok(dtype) && emb_dtype_ok(wdtype), "concord_embedding_bwd: bad type");
+  CONCORD_CHECK(ld_dy >= C && ld_dt >= C, "concord_embedding_bwd: leading dimension < C");
+  if (V == 0) return CONCORD_OK;
+  CONCORD_CHECK(dtable && (n == 0 || (tokens && dy)), "concord_embedding_bwd: NULL argument");
+  const EmbWorkspace w = emb_workspace(n, C);
+  if (n > 0 && (!workspace || workspace_bytes < w.bytes)) {
+    set_error("concord_embedding_bwd: workspace of %zu bytes needed", w.bytes);
+    return CONCORD_EWORKSPACE;
+  }
+  CONCORD_CHECK(((uintptr_t)workspace & 15) == 0, "concord_embedding_bwd: the workspace is not on 16 bytes");
+  const int piece = emb_piece(n, C);
+  CONCORD_CHECK(grid_fits(cdiv(n, 4 * piece) + cdiv(V, 4 * kFillRows), 256) && grid_fits(cdiv(n, piece), 256),
+                "concord_embedding_bwd: too many tokens or rows");
+  hipStream_t st = (hipStream_t)stream;
+  EmbArgs a{};
+  a.tokens = tokens, a.idx64 = index64, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
+  a.src = dy, a.lds = ld_dy, a.dst = dtable, a.ldd = ld_dt;
+  a.piece = piece, a.pieces = cdiv(n, piece);
+  uint32_t *keys[2] = {}, *pos[2] = {};
+  int at = 0;
+  if (n > 0) {
+    char* base = (char*)workspace;
+    for (int i = 0; i < 2; ++i) {
+      keys[i] = (uint32_t*)(base + w.keys[i]);
+      pos[i] = (uint32_t*)(base + w.pos[i]);
+    }
+    a.part = (float*)(base + w.part);
+    int bits = 1;
+    while (V >> bits) ++bits;   // (V itself stands for what is outside)
+    const int passes = (bits + kMaxBits - 1) / kMaxBits, each = (bits + passes - 1) / passes;
+    if (n <= kOneBlock) {
+      if (n <= 1024) hipLaunchKernelGGL((emb_sort_block_kernel<1>), dim3(1), dim3(1024), 0, st, a, passes, each, keys[0], pos[0]);
+      else hipLaunchKernelGGL((emb_sort_block_kernel<kOneBlock / 1024>), dim3(1), dim3(1024), 0, st, a, passes, each, keys[0], pos[0]);
+    } else {
+      const dim3 grid((unsigned)cdiv(n, kTile));
+      for (int p = 0; p < passes; ++p) {
+        SortPass s{};
+        if (p) s.keys = keys[at ^ 1], s.pos = pos[at ^ 1];
+        s.out_keys = keys[at], s.out_pos = pos[at], s.counts = (uint32_t*)(base + w.counts);
+        s.shift = p * each, s.bits = each;
+        hipLaunchKernelGGL(emb_count_kernel, grid, dim3(512), 0, st, a, s);
+        hipLaunchKernelGGL(emb_scatter_kernel, grid, dim3(512), 0, st, a, s);
+        at ^= 1;
+      }
+      at ^= 1;
+    }
+  }
+  a.keys = keys[at], a.pos = pos[at];
+  emb_types(dtype, wdtype, [&](auto g, auto t) { emb_bwd<decltype(g), decltype(t)>(a, st); });
+  return launch_status("embedding_bwd");
+}

@@ -1,0 +1,387 @@
+// qk_rope.hip -- the norm of each head's query and key with the rotation by
+// position in the same pass, forward and backward.
+//
+// A row x of D elements at position p, pairs i < R / 2 of its first R elements:
+//   r = 1 / sqrt(mean(x^2) + eps),  h = x r,  u = h w
+//   y = u with pair i (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = p base^(-2 i / R)
+// backward, from dy:
+//   du = dy rotated by -t,  g = du w,  dx = r (g - h mean(g h)),  dw = sum over rows of du h
+//
+// Bound by memory: every row is read once and written once, its statistics are
+// formed again in the backward rather than kept.  A row belongs to L adjacent
+// lanes, 8 elements each, that hold both elements of their pairs, so the rotation
+// exchanges nothing; a lane's angles depend on the token alone and serve all heads
+// that it takes.  Angles are formed in 64 bits (a far position times a frequency
+// loses its fraction in 32) and reduced to an eighth of a turn before the sine and
+// cosine, which are 32-bit polynomials.
+#include "elem.h"
+
+namespace concord {
+
+struct QkArgs {
+  const void* x[2];         // q and k; backward too
+  const void* dy[2];        // backward
+  void* out[2];             // y, or dx: [T][H][D], rows adjacent
+  int64_t x_t[2], x_h[2], dy_t[2], dy_h[2];
+  const void* w[2];         // NULL: ones
+  int wtype;
+  const void* pos;          // NULL: the token's place in its sequence
+  int pos64;
+  uint32_t T, seq, pos_seq; // tokens; tokens of a sequence; period of pos
+  int H[2];
+  int D, R, adjacent;
+  int heads, parts0;        // heads of a block's slice; slices of q
+  float eps;
+  double log2_base;
+  float* part[2];           // backward: [blocks of q's or k's slices][D] partial dw, or NULL
+};
+
+// the lane's four pairs: elements (a + j, b + j), or (a + 2 j, a + 2 j + 1) where pairs are adjacent
+struct QkLane {
+  int a, b;
+  bool in, turned;
+};
+CONCORD_DEV QkLane qk_lane(int l, int D, int R, bool adjacent) {
+  QkLane s;
+  s.in = l * 8 < D;
+  s.turned = l * 8 < R;
+  if (adjacent) s.a = l * 8, s.b = l * 8 + 4;
+  else if (s.turned) s.a = l * 4, s.b = R / 2 + l * 4;
+  else s.a = R + (l * 8 - R) / 2, s.b = s.a + (D - R) / 2;
+  return s;
+}
+
+// cosine and sine of pi/2 times a quarter-turn count given in 64 bits.  To the
+// nearest quarter turn, then Taylor polynomials of theta = pi/2 (turn - nearest),
+// |theta| <= pi/4: the first terms left out are below 2^-30 of 1 and of theta.
+CONCORD_DEV void sincos_quarters(double quarters, float& c, float& s) {
+  const double n = __builtin_rint(quarters);
+  const float th = (float)((quarters - n) * 1.5707963267948966);
+  const int q = (int)(int64_t)n & 3;
+  const float t = th * th;
+  float cs = __builtin_fmaf(t, -1.0f / 3628800.0f, 1.0f / 40320.0f);
+  cs = __builtin_fmaf(t, cs, -1.0f / 720.0f);
+  cs = __builtin_fmaf(t, cs, 1.0f / 24.0f);
+  cs = __builtin_fmaf(t, cs, -0.5f);
+  cs = __builtin_fmaf(t, cs, 1.0f);
+  float sn = __builtin_fmaf(t, 1.0f / 362880.0f, -1.0f / 5040.0f);
+  sn = __builtin_fmaf(t, sn, 1.0f / 120.0f);
+  sn = __builtin_fmaf(t, sn, -1.0f / 6.0f);
+  sn = __builtin_fmaf(t * th, sn, th);
+  const float u = q & 1 ? sn : cs, v = q & 1 ? cs : sn;
+  c = (q + 1) & 2 ? -u : u;
+  s = q & 2 ? -v : v;
+}
+
+// sum over the group of L lanes, to each
+template <int L>
+CONCORD_DEV float group_sum(float v) {
+#pragma unroll
+  for (int h = 1; h < L; h <<= 1) v += __shfl_xor(v, h, 64);
+  return v;
+}
+
+template <class T>
+struct QkRow {
+  typedef Chunk<T, 4> V;
+  V a, b;
+  CONCORD_DEV void load(const void* p, int64_t at, const QkLane& s) {
+    a = {}, b = {};
+    if (s.in) {
+      a = *(const V*)((const T*)p + at + s.a);
+      b = *(const V*)((const T*)p + at + s.b);
+    }
+  }
+  CONCORD_DEV void get(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = to_f32(a.v[j]), v[4 + j] = to_f32(b.v[j]);
+  }
+  CONCORD_DEV void put(const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a.v[j] = from_f32<T>(v[j]), b.v[j] = from_f32<T>(v[4 + j]);
+  }
+  CONCORD_DEV void store(void* p, int64_t at, const QkLane& s) const {
+    if (s.in) {
+      *(V*)((T*)p + at + s.a) = a;
+      *(V*)((T*)p + at + s.b) = b;
+    }
+  }
+};
+
+// v's pairs turned by +t (dir = 1) or -t (dir = -1)
+template <bool ADJ>
+CONCORD_DEV void turn(float (&v)[8], const float (&c)[4], const float (&s)[4], float dir) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int ia = ADJ ? 2 * j : j, ib = ADJ ? 2 * j + 1 : 4 + j;
+    const float a = v[ia], b = v[ib], sn = s[j] * dir;
+    v[ia] = __builtin_fmaf(a, c[j], -(b * sn));
+    v[ib] = __builtin_fmaf(a, sn, b * c[j]);
+  }
+}
+
+// Block (x, y): tokens of groups x, x + gridDim.x, ...; slice y of the heads,
+// q's slices before k's.
+template <class T, int L, bool ADJ, bool BWD>
+__global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
+  constexpr int G = 256 / L, U = BWD ? 2 : 4;
+  __shared__ float sums[BWD ? G : 1][BWD ? L * 8 : 1];
+  const int l = threadIdx.x & (L - 1), g = threadIdx.x / L;
+  const int which = (int)blockIdx.y >= a.parts0;
+  const int h0 = ((int)blockIdx.y - (which ? a.parts0 : 0)) * a.heads, H = a.H[which], h1 = min(h0 + a.heads, H);
+  const QkLane s = qk_lane(l, a.D, a.R, ADJ);
+  float w[8], dw[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    dw[j] = 0.0f;
+    w[j] = 1.0f;
+    if (a.w[which] && s.in) w[j] = load_any(a.w[which], a.wtype, (j < 4 ? s.a : s.b) + (j & 3));
+  }
+  // the lane's first frequency, in quarter turns a position, and the step from pair to pair
+  const double each = a.R ? -2.0 * a.log2_base / a.R : 0.0;
+  const double freq0 = exp2(each * (l * 4)) * 0.63661977236758134, ratio = exp2(each);
+  const float inv_d = 1.0f / (float)a.D;
+  for (uint32_t t = blockIdx.x * G + g; t < a.T; t += gridDim.x * G) {
+    float c[4], sn[4];
+    {
+      const uint32_t at = a.pos ? t % a.pos_seq : t % a.seq;
+      const int64_t p = !a.pos ? (int64_t)at : a.pos64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
+      double f = freq0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sincos_quarters((double)p * f, c[j], sn[j]);
+        if (!s.turned) c[j] = 1.0f, sn[j] = 0.0f;
+        f *= ratio;
+      }
+    }
+    const int64_t xt = t * a.x_t[which], ot = ((int64_t)t * H) * a.D, dt = BWD ? t * a.dy_t[which] : 0;
+    for (int h = h0; h < h1; h += U) {
+      QkRow<T> x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int hu = min(h + u, h1 - 1);
+        x[u].load(a.x[which], xt + hu * a.x_h[which], s);
+        if (BWD) y[u].load(a.dy[which], dt + hu * a.dy_h[which], s);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u >= h1) continue;
+        float v[8];
+        x[u].get(v);
+        float q = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q = __builtin_fmaf(v[j], v[j], q);
+        const float r = 1.0f / __builtin_sqrtf(group_sum<L>(q) * inv_d + a.eps);
+        if (!BWD) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[j];
+          turn<ADJ>(v, c, sn, 1.0f);
+        } else {
+          float d[8];
+          y[u].get(d);
+          turn<ADJ>(d, c, sn, -1.0f);
+          float along = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] *= r;
+            dw[j] = __builtin_fmaf(d[j], v[j], dw[j]);
+            d[j] *= w[j];
+            along = __builtin_fmaf(d[j], v[j], along);
+          }
+          along = group_sum<L>(along) * inv_d;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = r * __builtin_fmaf(-v[j], along, d[j]);
+        }
+        x[u].put(v);
+        x[u].store(a.out[which], ot + (int64_t)(h + u) * a.D, s);
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (!a.part[which]) return;
+    // the block's groups in order
+    if (s.in) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[g][(j < 4 ? s.a : s.b) + (j & 3)] = dw[j];
+    }
+    __syncthreads();
+    const int64_t row = (int64_t)((int)blockIdx.y - (which ? a.parts0 : 0)) * gridDim.x + blockIdx.x;
+    for (int i = threadIdx.x; i < a.D; i += 256) {
+      float v = sums[0][i];
+#pragma unroll
+      for (int k = 1; k < G; ++k) v += sums[k][i];
+      a.part[which][row * a.D + i] = v;
+    }
+  }
+}
+
+// dw from the blocks' partials: 64 columns a block, each wave a sixteenth of the
+// rows in order, then the waves' sums in order
+__global__ __launch_bounds__(1024) void qk_dw_kernel(const float* p0, const float* p1, int rows0, int rows1, int D,
+                                                     void* dw0, void* dw1, int wtype) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane, nb = blockIdx.y ? rows1 : rows0;
+  const float* p = blockIdx.y ? p1 : p0;
+  void* dw = blockIdx.y ? dw1 : dw0;
+  if (!dw) return;
+  float v = 0.0f;
+  if (c < D) {
+    const int per = (nb + 15) / 16, end = min(nb, (wave + 1) * per);
+    int r = wave * per;
+    for (; r + 8 <= end; r += 8) {
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = p[(int64_t)(r + i) * D + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += t[i];
+    }
+    for (; r < end; ++r) v += p[(int64_t)r * D + c];
+  }
+  sums[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0 && c < D) {
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v += sums[k][lane];
+    store_any(dw, wtype, c, v);
+  }
+}
+
+// ---- host -------------------------------------------------------------------
+struct QkPlan {
+  int lanes;        // of a row
+  int heads;        // a slice
+  int parts[2];     // slices of q and of k
+  unsigned blocks;  // of tokens
+};
+static QkPlan qk_plan(int64_t T, int H, int HK, int D, bool bwd) {
+  QkPlan p{};
+  p.lanes = 1;
+  while (p.lanes * 8 < D) p.lanes *= 2;
+  const int64_t groups = 256 / p.lanes;
+  // as many heads a slice as leave 256 blocks twice over: the angles are formed once a slice
+  p.heads = 16;
+  while (p.heads > 1 && cdiv(T, groups) * (cdiv(H, p.heads) + cdiv(HK, p.heads)) < 512) p.heads /= 2;
+  p.parts[0] = (int)cdiv(H, p.heads), p.parts[1] = (int)cdiv(HK, p.heads);
+  const int64_t most = std::max<int64_t>(1, (bwd ? 1024 : 4096) / (p.parts[0] + p.parts[1]));
+  p.blocks = (unsigned)std::min<int64_t>(cdiv(T, groups), most);
+  return p;
+}
+
+template <class T, int L>
+static void qk_launch(const QkArgs& a, const QkPlan& p, bool bwd, hipStream_t st) {
+  const dim3 grid(p.blocks, p.parts[0] + p.parts[1]);
+  if (bwd) {
+    if (a.adjacent) hipLaunchKernelGGL((qk_kernel<T, L, true, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((qk_kernel<T, L, false, true>), grid, dim3(256), 0, st, a);
+  } else {
+    if (a.adjacent) hipLaunchKernelGGL((qk_kernel<T, L, true, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((qk_kernel<T, L, false, false>), grid, dim3(256), 0, st, a);
+  }
+}
+template <class T>
+static void qk_lanes(const QkArgs& a, const QkPlan& p, bool bwd, hipStream_t st) {
+  switch (p.lanes) {
+    case 1: return qk_launch<T, 1>(a, p, bwd, st);
+    case 2: return qk_launch<T, 2>(a, p, bwd, st);
+    case 4: return qk_launch<T, 4>(a, p, bwd, st);
+    case 8: return qk_launch<T, 8>(a, p, bwd, st);
+    case 16: return qk_launch<T, 16>(a, p, bwd, st);
+    default: return qk_launch<T, 32>(a, p, bwd, st);
+  }
+}
+static void qk_run(const QkArgs& a, const QkPlan& p, int dtype, bool bwd, hipStream_t st) {
+  if (dtype == CONCORD_F32) qk_lanes<float>(a, p, bwd, st);
+  else if (dtype == CONCORD_BF16) qk_lanes<BF16>(a, p, bwd, st);
+  else qk_lanes<_Float16>(a, p, bwd, st);
+}
+
+static bool qk_aligned(const void* p, int64_t t, int64_t h) {
+  return ((uintptr_t)p & 15) == 0 && t % 8 == 0 && h % 8 == 0;
+}
+
+static bool qk_sizes_ok(const concord_qk_args& g) {
+  return g.T >= 0 && g.T < (1LL << 31) && g.H >= 0 && g.HK >= 0 && g.H < (1 << 14) && g.HK < (1 << 14) && g.H + g.HK > 0 &&
+         g.D >= 8 && g.D <= 256 && g.D % 8 == 0 && g.R >= 0 && g.R <= g.D && g.R % 8 == 0;
+}
+
+// checks that both passes share, and their arguments
+static int qk_args(const concord_qk_args* args, const char* name, bool bwd, QkArgs& a) {
+  CONCORD_CHECK(args, "%s: NULL argument", name);
+  const concord_qk_args& g = *args;
+  CONCORD_CHECK(qk_sizes_ok(g), "%s: bad size", name);
+  for (int t : {g.dtype, g.wtype})
+    CONCORD_CHECK(t == CONCORD_F32 || t == CONCORD_BF16 || t == CONCORD_F16, "%s: bad type", name);
+  CONCORD_CHECK(g.base > 0 && g.base < 1e300 && g.eps >= 0, "%s: bad base or eps", name);
+  if (g.T == 0) return CONCORD_OK;
+  CONCORD_CHECK(g.seq >= 1 && g.seq <= g.T && (!g.positions || (g.pos_seq >= 1 && g.pos_seq <= g.T)), "%s: bad sequence length",
+                name);
+  CONCORD_CHECK((g.H == 0 || g.q) && (g.HK == 0 || g.k), "%s: NULL argument", name);
+  CONCORD_CHECK((g.H == 0 || qk_aligned(g.q, g.q_t, g.q_h)) && (g.HK == 0 || qk_aligned(g.k, g.k_t, g.k_h)),
+                "%s: rows must lie on 16 bytes, strides in multiples of 8", name);
+  void* const out[2] = {bwd ? g.dq : g.q_out, bwd ? g.dk : g.k_out};
+  CONCORD_CHECK((g.H == 0 || out[0]) && (g.HK == 0 || out[1]), "%s: NULL result", name);
+  CONCORD_CHECK((((uintptr_t)out[0] | (uintptr_t)out[1]) & 15) == 0, "%s: results must lie on 16 bytes", name);
+  if (bwd) {
+    CONCORD_CHECK((g.H == 0 || g.dq_out) && (g.HK == 0 || g.dk_out), "%s: NULL gradient", name);
+    CONCORD_CHECK((g.H == 0 || qk_aligned(g.dq_out, g.dq_t, g.dq_h)) && (g.HK == 0 || qk_aligned(g.dk_out, g.dk_t, g.dk_h)),
+                  "%s: rows must lie on 16 bytes, strides in multiples of 8", name);
+  }
+  a.x[0] = g.q, a.x[1] = g.k, a.x_t[0] = g.q_t, a.x_h[0] = g.q_h, a.x_t[1] = g.k_t, a.x_h[1] = g.k_h;
+  a.dy[0] = g.dq_out, a.dy[1] = g.dk_out, a.dy_t[0] = g.dq_t, a.dy_h[0] = g.dq_h, a.dy_t[1] = g.dk_t, a.dy_h[1] = g.dk_h;
+  a.out[0] = out[0], a.out[1] = out[1];
+  a.w[0] = g.q_weight, a.w[1] = g.k_weight, a.wtype = g.wtype;
+  a.pos = g.positions, a.pos64 = g.pos64;
+  a.T = (uint32_t)g.T, a.seq = (uint32_t)g.seq, a.pos_seq = (uint32_t)(g.positions ? g.pos_seq : 1);
+  a.H[0] = g.H, a.H[1] = g.HK, a.D = g.D, a.R = g.R, a.adjacent = g.adjacent != 0, a.eps = g.eps;
+  a.log2_base = __builtin_log2(g.base);
+  return CONCORD_OK;
+}
+
+static size_t qk_workspace(const concord_qk_args& g, const QkPlan& p) {
+  return (size_t)p.blocks * (p.parts[0] + p.parts[1]) * g.D * sizeof(float);
+}
+
+}  // namespace concord
+
+using namespace concord;
+
+extern "C" int concord_qk_norm_rope_fwd(const concord_qk_args* args, void* stream) {
+  QkArgs a{};
+  if (const int rc = qk_args(args, "concord_qk_norm_rope_fwd", false, a)) return rc;
+  if (args->T == 0) return CONCORD_OK;
+  const QkPlan p = qk_plan(args->T, args->H, args->HK, args->D, false);
+  a.heads = p.heads, a.parts0 = p.parts[0];
+  qk_run(a, p, args->dtype, false, (hipStream_t)stream);
+  return launch_status("qk_norm_rope_fwd");
+}
+
+extern "C" size_t concord_qk_norm_rope_workspace_bytes(const concord_qk_args* args) {
+  if (!args || !qk_sizes_ok(*args) || args->T == 0) return 0;
+  return qk_workspace(*args, qk_plan(args->T, args->H, args->HK, args->D, true));
+}
+
+extern "C" int concord_qk_norm_rope_bwd(const concord_qk_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  QkArgs a{};
+  if (const int rc = qk_args(args, "concord_qk_norm_rope_bwd", true, a)) return rc;
+  const concord_qk_args& g = *args;
+  hipStream_t st = (hipStream_t)stream;
+  int rows[2] = {};
+  if (g.T > 0) {
+    const QkPlan p = qk_plan(g.T, g.H, g.HK, g.D, true);
+    if ((g.dq_weight || g.dk_weight) && (!workspace || workspace_bytes < qk_workspace(g, p))) {
+      set_error("concord_qk_norm_rope_bwd: workspace of %zu bytes needed", qk_workspace(g, p));
+      return CONCORD_EWORKSPACE;
+    }
+    a.heads = p.heads, a.parts0 = p.parts[0];
+    for (int i = 0; i < 2; ++i) rows[i] = (int)p.blocks * p.parts[i];
+    a.part[0] = g.dq_weight ? (float*)workspace : nullptr;
+    a.part[1] = g.dk_weight ? (float*)workspace + (int64_t)rows[0] * g.D : nullptr;
+    qk_run(a, p, g.dtype, true, st);
+  }
+  if (g.dq_weight || g.dk_weight)   // (no token: sums over no partials, zero)
+    hipLaunchKernelGGL(qk_dw_kernel, dim3((unsigned)cdiv(g.D, 64), 2), dim3(1024), 0, st, (const float*)a.part[0],
+                       (const float*)a.part[1], rows[0], rows[1], g.D, g.dq_weight, g.dk_weight, g.wtype);
+  return launch_status("qk_norm_rope_bwd");
+}

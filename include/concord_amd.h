@@ -1,7 +1,8 @@
 /*
  * concord_amd.h -- C ABI of the MI355X (gfx950) packed-weight linear path, and
  * of the operators that stand between such layers in a training step (layer
- * norm, attention, distillation; at the end).
+ * norm, attention, distillation; embedding, norms of queries and keys with the
+ * position rotation, activations kept in 8 bits; at the end).
  *
  * Every entry point takes raw device pointers, sizes and leading dimensions,
  * plus the hipStream_t (passed as void*) to enqueue on.  No entry point
@@ -598,6 +599,78 @@ int concord_attention_fwd(const concord_attn_args* args, void* workspace, size_t
  * concord_attention_workspace_bytes(args) bytes on 16; it need not be zeroed. */
 size_t concord_attention_workspace_bytes(const concord_attn_args* args);
 int concord_attention_bwd(const concord_attn_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- From tokens to the feed-forward: embedding, norms of queries and keys with
+ * the position rotation, activations kept in 8 bits (no counterpart in the
+ * reference) ---- */
+
+/* y[i] = scale table[tokens[i]] for n tokens (int64 where index64, else int32,
+ * one after another), table [V, ld_t] of type wdtype, y [n, ld_o] of type dtype.
+ * A token outside [0, V) gives a row of zeros. */
+int concord_embedding_fwd(const void* tokens, int index64, int64_t n, const void* table, int64_t ld_t, int wdtype,
+                          int64_t V, int64_t C, float scale, void* out, int64_t ld_o, int dtype, void* stream);
+/* dtable[v] = scale sum of dy[i] over the tokens i that name v, all V rows
+ * (zeros where none does), summed in fp32 in a fixed order.  workspace:
+ * concord_embedding_workspace_bytes(n, V, C) bytes on 16; it need not be zeroed.
+ * n < 2^31, V < 2^31 - 1, C < 2^21 (the size query gives 0 for other sizes). */
+size_t concord_embedding_workspace_bytes(int64_t n, int64_t V, int64_t C);
+int concord_embedding_bwd(const void* tokens, int index64, int64_t n, const void* dy, int64_t ld_dy, int dtype, int64_t V,
+                          int64_t C, float scale, void* dtable, int64_t ld_dt, int wdtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The norm of each head's query and key, then the rotation by position: a row x
+ * of D elements (a multiple of 8 up to 256) at position p gives u = x weight /
+ * sqrt(mean(x^2) + eps), and pair i < R / 2 of u's first R elements (R a multiple
+ * of 8, 0: none) turns by p base^(-2 i / R).  Pair i is elements i and i + R / 2,
+ * or 2 i and 2 i + 1 where `adjacent`.
+ *
+ * Element (token, head, d) of q lies at token * q_t + head * q_h + d (strides in
+ * elements, multiples of 8; 16-byte aligned), likewise the others; results are
+ * [T][H][D] and [T][HK][D] without gaps, 16-byte aligned.  Weights [D] of type
+ * wdtype, NULL: ones.  Token t has position positions[t % pos_seq] (int64 where
+ * pos64, else int32), or t % seq where positions is NULL. */
+typedef struct concord_qk_args {
+  const void *q, *k;
+  int64_t q_t, q_h, k_t, k_h;
+  void *q_out, *k_out;              /* forward */
+  const void *q_weight, *k_weight;
+  const void* positions;
+  int64_t T, seq, pos_seq;
+  int32_t H, HK, D, R, adjacent, pos64, dtype, wtype;
+  float eps;
+  double base;
+  /* backward: upstream gradients, results */
+  const void *dq_out, *dk_out;
+  int64_t dq_t, dq_h, dk_t, dk_h;   /* strides of dq_out and dk_out */
+  void *dq, *dk;
+  void *dq_weight, *dk_weight;      /* of type wdtype; NULL: not wanted */
+} concord_qk_args;
+int concord_qk_norm_rope_fwd(const concord_qk_args* args, void* stream);
+/* dq and dk from the inputs and the upstream gradients (nothing else is kept),
+ * and the weights' gradients, summed over tokens and heads in fp32 in a fixed
+ * order.  workspace: concord_qk_norm_rope_workspace_bytes(args) bytes, only where
+ * a weight's gradient is wanted; it need not be zeroed. */
+size_t concord_qk_norm_rope_workspace_bytes(const concord_qk_args* args);
+int concord_qk_norm_rope_bwd(const concord_qk_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Activations in 8 bits.  32 adjacent values of a row (the row's last block may be
+ * shorter) share a step 2^e, the smallest power of two with max|x| <= 127 2^e, e >=
+ * -126: codes [rows][C] = x 2^-e rounded half to even, exponents [rows][ceil(C /
+ * 32)] = e + 127.  A block with an infinity or NaN has exponent 255 and reads back as
+ * NaN.  concord_unpack8 gives code 2^e, limited to the type's largest finite number. */
+int concord_pack8(const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t C, int8_t* codes, uint8_t* exponents,
+                  void* stream);
+int concord_unpack8(const int8_t* codes, const uint8_t* exponents, int64_t rows, int64_t C, void* x, int64_t ld_x,
+                    int dtype, void* stream);
+/* y = f(x), f(x) = x Phi(x) or its tanh form, for rows of C values; gated: y = a
+ * f(g) for rows [a | g] of 2 C values.  codes and exponents (both or neither): x in 8
+ * bits, each half of a gated row in blocks of its own ([rows][2 C] and [rows][2][
+ * ceil(C / 32)]). */
+int concord_gelu8_fwd(const void* x, int64_t ld_x, int dtype, int64_t rows, int64_t C, int gated, int tanh_form, void* y,
+                      int64_t ld_y, int8_t* codes, uint8_t* exponents, void* stream);
+/* dx = dy f'(z), z what the codes stand for; gated: [dy f(g) | dy a f'(g)]. */
+int concord_gelu8_bwd(const void* dy, int64_t ld_dy, const int8_t* codes, const uint8_t* exponents, int dtype, int64_t rows,
+                      int64_t C, int gated, int tanh_form, void* dx, int64_t ld_dx, void* stream);
 
 #ifdef __cplusplus
 }

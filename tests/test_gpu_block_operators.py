@@ -1,0 +1,560 @@
+"""Embedding, norms of queries and keys with the position rotation, and activations
+kept in 8 bits, forward and backward, against plain implementations in 64 bits.
+
+Tolerances count roundings: u = 2^-24 for each one of fp32 arithmetic, half a step
+(finfo.eps / 2 of the value) for the result's type, and half the smallest subnormal
+where fp16 underflows."""
+import math
+
+import pytest
+import torch
+
+from gpu_util import DEV
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+def _gen(*key):
+    return torch.Generator(device=DEV).manual_seed(sum(ord(c) * (i + 1) for i, c in enumerate(repr(key))))
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2 if dtype != F32 else 0.0
+
+
+def _tiny(dtype):
+    return 2.0 ** -25 if dtype == F16 else 2.0 ** -126
+
+
+def _close(got, want, bound, dtype, what=""):
+    """|got - want| <= bound (fp32 roundings) and the result's own rounding"""
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, (got.shape, want.shape)
+    limit = bound * (1 + _half(dtype)) + want.abs() * _half(dtype) + _tiny(dtype)
+    over = ((got - want).abs() - limit).detach()
+    assert not torch.isnan(got).any(), what
+    assert not over.numel() or float(over.max()) <= 0, (what, float(over.max()), int(over.argmax()))
+
+
+# ---- embedding ----------------------------------------------------------------
+def _embedding_reference(tokens, w, scale, dy):
+    t = tokens.reshape(-1).long()
+    there = (t >= 0) & (t < w.shape[0])
+    at = torch.where(there, t, 0)
+    y = w.double()[at] * there[:, None] * scale
+    dw = torch.zeros(w.shape, dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(dw)   # sums of magnitudes
+    g = dy.double().reshape(-1, w.shape[1]) * there[:, None]
+    dw.index_add_(0, at, g)
+    size.index_add_(0, at, g.abs())
+    count = torch.zeros(w.shape[0], dtype=torch.float64, device=DEV).index_add_(0, at, there.double())
+    return y.reshape(*tokens.shape, -1), dw * scale, size * abs(scale), count
+
+
+def _check_embedding(tokens, w, scale, dtype, dy):
+    import concord_amd as ca
+    y = ca.embedding(tokens, w, scale=scale, dtype=dtype)
+    dw, = torch.autograd.grad(y, (w,), dy)
+    ry, rdw, size, count = _embedding_reference(tokens, w.detach(), scale, dy)
+    out = dtype or w.dtype
+    assert y.dtype == out and dw.dtype == w.dtype and dw.shape == w.shape
+    _close(y.detach(), ry, ry.abs() * U, out, "y")
+    # count - 1 additions, the scale
+    _close(dw, rdw, size * (count[:, None] + 1) * U, w.dtype, "dw")
+    with torch.no_grad():
+        assert torch.equal(ca.embedding(tokens, w, scale=scale, dtype=dtype), y.detach())
+    again, = torch.autograd.grad(ca.embedding(tokens, w, scale=scale, dtype=dtype), (w,), dy)
+    assert torch.equal(again, dw)   # a fixed order
+    return y.detach(), dw
+
+
+@pytest.mark.parametrize("n,vocab,width", [
+    (1, 1, 1), (1, 7, 8), (3, 2, 5), (63, 65, 64), (64, 511, 40), (65, 512, 384), (1000, 3, 33), (1024, 1000, 256),
+    (1025, 70000, 16), (4096, 50257, 24), (4097, 300000, 8), (5000, 65, 384), (8192, 8192, 128), (20000, 1, 72),
+    (33333, 50257, 100), (131073, 513, 8)])
+@pytest.mark.parametrize("table,dtype", [(F32, None), (F32, BF16), (BF16, None), (F16, F32)])
+def test_embedding(n, vocab, width, table, dtype):
+    g = _gen("embedding", n, vocab, width, table)
+    # some tokens far commoner than the rest
+    tokens = (torch.rand(n, generator=g, device=DEV) ** 4 * vocab).long().clamp_max_(vocab - 1)
+    w = torch.randn(vocab, width, generator=g, device=DEV).to(table).requires_grad_(True)
+    dy = torch.randn(n, width, generator=g, device=DEV).to(dtype or table)
+    _check_embedding(tokens, w, 1.5, dtype, dy)
+
+
+@pytest.mark.parametrize("case", ["all", "none", "some", "huge"])
+@pytest.mark.parametrize("index", [torch.int64, torch.int32])
+def test_embedding_tokens_outside(case, index):
+    g = _gen("outside", case)
+    n, vocab, width = 3000, 500, 72
+    tokens = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    if case == "all":
+        tokens[:] = -1
+    elif case == "some":
+        tokens[torch.rand(n, generator=g, device=DEV) < 0.4] = -1
+        tokens[7], tokens[-1] = vocab, vocab + 1
+    elif case == "huge":
+        tokens[::3] = -2 ** 31
+        tokens[1::3] = 2 ** 31 - 1
+    w = torch.randn(vocab, width, generator=g, device=DEV).requires_grad_(True)
+    y, dw = _check_embedding(tokens.to(index), w, 1.0, None, torch.randn(n, width, generator=g, device=DEV))
+    if case == "all":
+        assert not y.any() and not dw.any()
+    if case == "huge" and index == torch.int64:
+        import concord_amd as ca
+        far = tokens.clone()
+        far[::3] = 2 ** 32 + 5   # its low word is a token
+        assert not ca.embedding(far, w)[::3].any()
+
+
+@pytest.mark.parametrize("n", [0, 1, 5])
+def test_embedding_of_no_token_and_no_row(n):
+    import concord_amd as ca
+    w = torch.randn(9, 24, device=DEV, requires_grad=True)
+    y = ca.embedding(torch.full((n, 0), 1, dtype=torch.int64, device=DEV), w)
+    assert y.shape == (n, 0, 24)
+    dw, = torch.autograd.grad(y, (w,), torch.zeros_like(y))
+    assert dw.shape == w.shape and not dw.any()
+    none = torch.empty(0, 24, device=DEV, requires_grad=True)
+    y = ca.embedding(torch.zeros(n, dtype=torch.int64, device=DEV), none)
+    assert y.shape == (n, 24) and not y.any()
+    assert torch.autograd.grad(y, (none,), torch.ones_like(y))[0].shape == (0, 24)
+
+
+def test_embedding_layouts():
+    """Tokens and tables in other strides, an upstream gradient that is expanded or transposed."""
+    import concord_amd as ca
+    g = _gen("layouts")
+    tokens = torch.randint(0, 50, (40, 30), generator=g, device=DEV).t()
+    big = torch.randn(50, 100, generator=g, device=DEV)
+    for w in (big[:, 3:80], big[:, :64], torch.randn(64, 50, generator=g, device=DEV).t()):
+        w = w.detach().requires_grad_(True)
+        dy = torch.randn(w.shape[1], 30, 40, generator=g, device=DEV).permute(1, 2, 0)
+        _check_embedding(tokens, w, 2.0, None, dy)
+    w = big[:, :64].detach().requires_grad_(True)
+    dw, = torch.autograd.grad(ca.embedding(tokens, w).sum(), (w,))
+    count = torch.bincount(tokens.reshape(-1), minlength=50).float()
+    assert torch.equal(dw, count[:, None].expand(50, 64))
+
+
+def test_embedding_rows_of_infinities_stay_apart():
+    import concord_amd as ca
+    w = torch.ones(6, 40, device=DEV)
+    w[2] = math.inf
+    w[3] = math.nan
+    w.requires_grad_(True)
+    tokens = torch.tensor([0, 2, 3, -1, 5], device=DEV)
+    y = ca.embedding(tokens, w)
+    assert torch.equal(y[[0, 3, 4]].detach(), torch.tensor([1.0, 0.0, 1.0], device=DEV)[:, None].expand(3, 40))
+    dy = torch.ones(5, 40, device=DEV)
+    dy[3] = math.nan   # of a token that stands for nothing
+    dw, = torch.autograd.grad(y, (w,), dy)
+    assert torch.equal(dw[:, 0], torch.tensor([1.0, 0, 1, 1, 0, 1], device=DEV))
+
+
+# ---- norms of queries and keys with the rotation --------------------------------
+def _rotated(x, angle, rotary, adjacent):
+    """x's first `rotary` elements turned, and the sums of magnitudes that each result came from"""
+    a, b = (x[..., 0:rotary:2], x[..., 1:rotary:2]) if adjacent else (x[..., :rotary // 2], x[..., rotary // 2:rotary])
+    c, s = angle.cos(), angle.sin()
+    u, v, m = a * c - b * s, a * s + b * c, a.abs() + b.abs()
+    if adjacent:
+        turned, size = torch.stack((u, v), -1).flatten(-2), torch.stack((m, m), -1).flatten(-2)
+    else:
+        turned, size = torch.cat((u, v), -1), torch.cat((m, m), -1)
+    return torch.cat((turned, x[..., rotary:]), -1), torch.cat((size, x[..., rotary:].abs()), -1)
+
+
+def _qk_reference(x, w, positions, base, rotary, adjacent, eps, dy):
+    """(y, its bound, dx, its bound, dw, its bound); bounds count fp32 roundings: 13 in the sum of
+    squares (half of them in r) and 5 to the norm, 4 in each sine and cosine, 3 in the turn"""
+    d = x.shape[-1]
+    x, dy = x.double(), dy.double()
+    wd = w.double() if w is not None else torch.ones(d, dtype=torch.float64, device=DEV)
+    freq = base ** (-2.0 * torch.arange(rotary // 2, device=DEV, dtype=torch.float64) / max(rotary, 1))
+    angle = positions.double()[..., None, None] * freq
+    r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    h = x * r
+    y, size = _rotated(h * wd, angle, rotary, adjacent)
+    du, du_size = _rotated(dy, -angle, rotary, adjacent)
+    g, g_size = du * wd, du_size * wd.abs()
+    dx = r * (g - h * (g * h).mean(-1, keepdim=True))
+    dx_size = r * (g_size + h.abs() * (g_size * h.abs()).mean(-1, keepdim=True))
+    over = tuple(range(x.dim() - 1))
+    rows = x.numel() // d
+    dw, dw_size = (du * h).sum(over), (du_size * h.abs()).sum(over)
+    return y, 24 * U * size, dx, 64 * U * dx_size, dw, (32 + rows) * U * dw_size
+
+
+def _check_qk(q, k, wq, wk, positions, real_positions, base=10000.0, rotary=None, adjacent=False, eps=1e-6, gen=None):
+    import concord_amd as ca
+    leaves = [t.detach().requires_grad_(True) for t in (q, k)] + [w for w in (wq, wk) if w is not None]
+    yq, yk = ca.qk_norm_rope(leaves[0], leaves[1], wq, wk, positions=positions, base=base, rotary_dim=rotary,
+                             interleaved=adjacent, eps=eps)
+    dq, dk = (torch.randn(t.shape, generator=gen, device=DEV).to(t.dtype) for t in (q, k))
+    grads = list(torch.autograd.grad((yq, yk), leaves, (dq, dk)))
+    rot = q.shape[-1] if rotary is None else rotary
+    dws = grads[2:]
+    for name, x, w, y, dy, dx in (("q", q, wq, yq, dq, grads[0]), ("k", k, wk, yk, dk, grads[1])):
+        ry, by, rdx, bdx, rdw, bdw = _qk_reference(x, w, real_positions, base, rot, adjacent, eps, dy)
+        assert y.dtype == x.dtype and dx.dtype == x.dtype
+        _close(y.detach(), ry, by, x.dtype, name)
+        _close(dx, rdx, bdx, x.dtype, "d" + name)
+        if w is not None:
+            dw = dws.pop(0)
+            assert dw.dtype == w.dtype
+            _close(dw, rdw, bdw, w.dtype, "dw" + name)
+    with torch.no_grad():
+        plain = ca.qk_norm_rope(q, k, wq, wk, positions=positions, base=base, rotary_dim=rotary, interleaved=adjacent,
+                                eps=eps)
+    assert torch.equal(plain[0], yq.detach()) and torch.equal(plain[1], yk.detach())
+
+
+@pytest.mark.parametrize("batch,tokens,heads,kv,dim", [
+    (1, 1, 1, 1, 8), (1, 1, 32, 8, 128), (3, 1, 5, 5, 64), (2, 7, 6, 3, 40), (1, 63, 4, 1, 16), (2, 129, 20, 5, 80),
+    (1, 1000, 17, 1, 96), (4, 257, 3, 3, 256), (1, 2049, 8, 2, 200), (2, 3000, 1, 1, 24)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_qk_norm_rope(batch, tokens, heads, kv, dim, dtype):
+    g = _gen("qk", batch, tokens, heads, kv, dim, dtype)
+    q = (2 * torch.randn(batch, tokens, heads, dim, generator=g, device=DEV)).to(dtype)
+    k = (2 * torch.randn(batch, tokens, kv, dim, generator=g, device=DEV)).to(dtype)
+    wq, wk = ((1 + 0.3 * torch.randn(dim, generator=g, device=DEV)).requires_grad_(True) for _ in range(2))
+    pos = torch.arange(tokens, device=DEV).expand(batch, -1)
+    _check_qk(q, k, wq, wk, None, pos, gen=g)
+
+
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize("dim,rotary", [(64, 64), (64, 32), (64, 8), (64, 0), (80, 40), (80, 72), (128, 64), (256, 248),
+                                        (8, 8), (8, 0)])
+def test_qk_rotary_dims(dim, rotary, adjacent):
+    g = _gen("rotary", dim, rotary, adjacent)
+    q, k = (torch.randn(2, 33, h, dim, generator=g, device=DEV) for h in (5, 2))
+    pos = torch.randint(-100, 5000, (2, 33), generator=g, device=DEV)
+    w = (1 + 0.3 * torch.randn(dim, generator=g, device=DEV)).requires_grad_(True)
+    _check_qk(q, k, w, None, pos, pos, base=500.0, rotary=rotary, adjacent=adjacent, gen=g)
+    _check_qk(q, k, None, w, pos.int(), pos, base=5e5, rotary=rotary, adjacent=adjacent, gen=g)
+    _check_qk(q, k, None, None, pos[1], pos[1].expand(2, -1), rotary=rotary, adjacent=adjacent, gen=g)
+
+
+@pytest.mark.parametrize("far", [1 << 20, 1 << 24, (1 << 31) - 1, 1 << 40])
+def test_qk_far_positions(far):
+    """The angle of a far position keeps its fraction: 64 bits lose 2^-52 of far / 2 pi turns, which
+    is below a rounding of fp32 up to far = 2^28; past that the reference itself loses it, so both
+    get an allowance of far 2^-51."""
+    import concord_amd as ca
+    g = _gen("far", far)
+    q = torch.randn(40, 2, 64, generator=g, device=DEV)
+    pos = far - torch.arange(40, device=DEV)
+    got = ca.qk_norm_rope(q, q, positions=pos)[0]
+    y, bound, *_ = _qk_reference(q, None, pos, 10000.0, 64, False, 1e-6, q)
+    size = bound / (24 * U)
+    _close(got, y, bound + size * far * 2.0 ** -51, F32)
+
+
+@pytest.mark.parametrize("wtype", TYPES)
+def test_qk_weights_of_other_types(wtype):
+    g = _gen("wtype", wtype)
+    q, k = (torch.randn(300, h, 64, generator=g, device=DEV).to(BF16) for h in (4, 2))
+    wq, wk = ((1 + 0.3 * torch.randn(64, generator=g, device=DEV)).to(wtype).requires_grad_(True) for _ in range(2))
+    _check_qk(q, k, wq, wk, None, torch.arange(300, device=DEV), gen=g)
+
+
+def test_qk_layouts():
+    """The split of one projection's output, head-major tensors, broadcast heads, rows off 16 bytes."""
+    g = _gen("qk layouts")
+    qkv = torch.randn(2, 50, 8, 64, generator=g, device=DEV).to(BF16)
+    pos = torch.arange(50, device=DEV).expand(2, -1)
+    q, k, _ = qkv.split([4, 2, 2], dim=2)
+    head_major = torch.randn(2, 4, 50, 64, generator=g, device=DEV).to(BF16).transpose(1, 2)
+    off = torch.randn(2, 50, 4, 65, generator=g, device=DEV).to(BF16)[..., 1:]
+    one = torch.randn(2, 50, 1, 64, generator=g, device=DEV).to(BF16).expand(2, 50, 4, 64)
+    dims = torch.randn(2, 50, 64, 4, generator=g, device=DEV).to(BF16).transpose(2, 3)
+    w = torch.randn(128, generator=g, device=DEV)[::2].requires_grad_(True)
+    for x in (q, head_major, off, one, dims, qkv[:, :, ::2]):
+        _check_qk(x, k, w, None, None, pos, gen=g)
+    _check_qk(q, head_major, None, w, pos.t().contiguous().t(), pos, gen=g)
+
+
+def test_qk_no_tokens_and_rows_of_zeros():
+    import concord_amd as ca
+    q = torch.zeros(0, 4, 64, device=DEV, dtype=BF16, requires_grad=True)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    y = ca.qk_norm_rope(q, q, w, w)
+    dq, dw = torch.autograd.grad(y, (q, w), [torch.zeros_like(t) for t in y])
+    assert y[0].shape == q.shape and dq.shape == q.shape and not dw.any()
+    x = torch.zeros(5, 2, 64, device=DEV, requires_grad=True)   # eps alone under the root
+    y = ca.qk_norm_rope(x, x, w, w)
+    dx, dw = torch.autograd.grad(y, (x, w), [torch.ones_like(t) for t in y])
+    assert not y[0].any() and not dw.any() and torch.isfinite(dx).all()
+
+
+def test_qk_rows_of_nan_stay_apart():
+    import concord_amd as ca
+    g = _gen("nan rows")
+    q = torch.randn(70, 3, 80, generator=g, device=DEV)
+    clean = ca.qk_norm_rope(q, q)[0]
+    bad = q.clone()
+    bad[5, 1], bad[64, 0, 3] = math.nan, math.inf
+    got = ca.qk_norm_rope(bad, q)[0]
+    rows = torch.ones(70, 3, dtype=torch.bool, device=DEV)
+    rows[5, 1] = rows[64, 0] = False
+    assert torch.equal(got[rows], clean[rows]) and torch.isnan(got[5, 1]).all()
+
+
+def test_qk_one_result_unused():
+    import concord_amd as ca
+    g = _gen("unused")
+    q, k = (torch.randn(20, 2, 64, generator=g, device=DEV).requires_grad_(True) for _ in range(2))
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    yq, _ = ca.qk_norm_rope(q, k, w, w)
+    dq, dk = torch.autograd.grad(yq.sum(), (q, k))
+    both = torch.autograd.grad([t.sum() for t in ca.qk_norm_rope(q, k, w, w)], (q, k))
+    assert torch.equal(dq, both[0]) and not dk.any()
+
+
+def test_qk_gradients_against_differences():
+    """Central differences in 64 bits of the formula at random directions; fp32 gradients."""
+    import concord_amd as ca
+    g = _gen("differences")
+    q, k = (torch.randn(6, h, 32, generator=g, device=DEV).requires_grad_(True) for h in (3, 1))
+    w = (1 + 0.2 * torch.randn(32, generator=g, device=DEV)).requires_grad_(True)
+    pos = torch.randint(0, 1000, (6,), generator=g, device=DEV)
+    ups = [torch.randn(t.shape, generator=g, device=DEV) for t in (q, k)]
+    grads = torch.autograd.grad(ca.qk_norm_rope(q, k, w, w, positions=pos), (q, k, w), ups)
+    dirs = [torch.randn(t.shape, generator=g, device=DEV).double() for t in (q, k, w)]
+
+    def f(t):
+        ws = w.detach().double() + t * dirs[2]
+        total = 0.0
+        for x, d, up in ((q, dirs[0], ups[0]), (k, dirs[1], ups[1])):
+            y, *_ = _qk_reference(x.detach().double() + t * d, ws, pos, 10000.0, 32, False, 1e-6, up)
+            total = total + float((y * up.double()).sum())
+        return total
+    step = 1e-4
+    slope = (f(step) - f(-step)) / (2 * step)
+    got = sum(float((a.double() * b).sum()) for a, b in zip(grads, dirs))
+    size = sum(float((a.double() * b).abs().sum()) for a, b in zip(grads, dirs))
+    # fp32 gradients (64 u), and the differences' own error: step^2 of a third derivative of order 10 here
+    assert abs(got - slope) <= 64 * U * size + 10 * step ** 2 * size
+
+
+# ---- activations in 8 bits ---------------------------------------------------------
+def _kept(x):
+    """(codes, exponents, values) of the 8-bit form, in exact arithmetic: blocks of 32, the smallest
+    power of two that takes the largest value to 127 or less"""
+    c = x.shape[-1]
+    b = torch.nn.functional.pad(x.double(), (0, -c % 32)).unflatten(-1, (-1, 32))
+    top = b.abs().amax(-1)
+    powers = (torch.arange(-126, 123, device=x.device) + 1023 << 52).view(torch.float64)
+    at = torch.searchsorted(127.0 * powers, torch.nan_to_num(top, nan=0.0, posinf=0.0))
+    step = powers[at]
+    bad = ~torch.isfinite(b).all(-1)
+    codes = (b / step[..., None]).round().masked_fill(bad[..., None], 0.0)
+    most = torch.finfo(x.dtype).max
+    values = (codes * step[..., None]).clamp(-most, most).masked_fill(bad[..., None], math.nan)
+    exps = torch.where(bad, 255, at + 1)
+    return codes.flatten(-2)[..., :c].to(torch.int8), exps.to(torch.uint8), values.flatten(-2)[..., :c]
+
+
+def _same(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=-77.0), torch.nan_to_num(b, nan=-77.0)) and \
+        torch.equal(torch.isnan(a), torch.isnan(b))
+
+
+def _spread(shape, dtype, g):
+    """values of many magnitudes: blocks from the type's smallest to its largest"""
+    x = torch.randn(shape, generator=g, device=DEV)
+    mag = torch.rand(*shape[:-1], 1, generator=g, device=DEV)
+    lo, hi = (-24.0, 15.0) if dtype == F16 else (-120.0, 125.0)
+    x = x * torch.exp2(lo + (hi - lo) * mag)
+    most = torch.finfo(dtype).max
+    return x.clamp(-most, most).to(dtype)
+
+
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 31), (1, 32), (3, 33), (2, 64), (5, 7), (7, 40), (1000, 96), (33, 1283),
+                                        (129, 2051), (64, 5120), (4099, 65)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pack8_is_exact(rows, width, dtype):
+    import concord_amd as ca
+    g = _gen("pack", rows, width, dtype)
+    for x in (torch.randn(rows, width, generator=g, device=DEV).to(dtype), _spread((rows, width), dtype, g)):
+        codes, exps = ca.pack8(x)
+        rc, re, rv = _kept(x)
+        assert codes.dtype == torch.int8 and exps.dtype == torch.uint8
+        assert torch.equal(exps, re) and torch.equal(codes, rc)
+        back = ca.unpack8(codes, exps, dtype)
+        assert back.dtype == dtype and torch.equal(back.double(), rv)
+        step = torch.exp2(exps.double() - 127).repeat_interleave(32, -1)[..., :width]
+        assert ((back.double() - x.double()).abs() <= step / 2).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pack8_edges(dtype):
+    """Ties, mantissas around 127 / 64, the largest and smallest numbers, zeros, infinities and NaN."""
+    import concord_amd as ca
+    info = torch.finfo(dtype)
+    x = torch.zeros(12, 70, device=DEV, dtype=dtype)
+    x[0, :4] = torch.tensor([127.0, 0.5, 1.5, -2.5], device=DEV)   # step 1: ties to even
+    x[1, :3] = torch.tensor([127.5, 1.0, 3.0], device=DEV)         # step 2
+    x[2, 0], x[2, 33], x[2, 69] = info.max, -info.max, info.max
+    x[3, :2] = torch.tensor([info.smallest_normal, -info.tiny], device=DEV)
+    x[4, 0] = 2.0 ** -24 if dtype == F16 else info.tiny * 2.0 ** -7   # subnormal
+    x[5, 5] = math.inf
+    x[6, 40] = -math.inf
+    x[7, 69] = math.nan
+    x[8, 3], x[8, 4] = math.nan, math.inf
+    x[9, :] = -1.0
+    x[10, ::2] = 1.9921875   # 255 / 128: above 127 / 64
+    x[11, ::2] = 1.984375    # 127 / 64
+    codes, exps = ca.pack8(x)
+    rc, re, rv = _kept(x)
+    assert torch.equal(exps, re) and torch.equal(codes, rc)
+    assert _same(ca.unpack8(codes, exps, dtype).double(), rv)
+    assert int(exps[5, 0]) == 255 and int(exps[5, 1]) != 255
+    # another type than it came from: limited to its largest number
+    if dtype != F16:
+        half = ca.unpack8(codes[2:3], exps[2:3], F16)
+        assert float(half.max()) == 65504.0 == -float(half.min())
+
+
+def test_pack8_layouts():
+    import concord_amd as ca
+    g = _gen("pack layouts")
+    big = torch.randn(6, 50, 200, generator=g, device=DEV).to(BF16)
+    for x in (big[:, :, 5:101], big[:, :, 8:104], big[:, ::2], big.transpose(1, 2), big[:, :, ::3], big[:0], big[0, 0],
+              big[0, 0, 0:1].expand(70)):
+        codes, exps = ca.pack8(x)
+        rc, re, rv = _kept(x.contiguous())
+        assert torch.equal(codes, rc) and torch.equal(exps, re) and codes.shape == x.shape
+        assert torch.equal(ca.unpack8(codes, exps, BF16).double(), rv)
+    codes, exps = ca.pack8(big)
+    wide = codes.new_zeros(6, 50, 201)
+    wide[..., 1:] = codes
+    assert torch.equal(ca.unpack8(wide[..., 1:], exps.transpose(0, 1).contiguous().transpose(0, 1), BF16),
+                       ca.unpack8(codes, exps, BF16))
+
+
+def _gelu64(x, tanh):
+    """gelu, its derivative, and the share of each that fp32 roundings may take: an exponent y rounded
+    at each of three steps is 3 |y| ln 2 u of its power; 16 u cover the polynomial's error (3.2e-8 of
+    Phi, half a u) and its evaluation, the reciprocal and the products"""
+    if tanh:
+        c, a = math.sqrt(2 / math.pi), 0.044715
+        u = c * (x + a * x ** 3)
+        sig = torch.sigmoid(2 * u)
+        rel = (16 + 3 * 2 * u.abs()) * U
+        du = 2 * c * (1 + 3 * a * x ** 2)
+        d = sig + x * sig * torch.sigmoid(-2 * u) * du
+        return x * sig, d, rel, rel * (sig + 2 * (x * sig * torch.sigmoid(-2 * u) * du).abs())
+    cdf = torch.special.erfc(-x / math.sqrt(2)) / 2   # (special.ndtr loses the left tail's digits on the GPU)
+    pdf = torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+    rel = torch.full_like(x, 16 * U)
+    return x * cdf, cdf + x * pdf, rel, rel * (cdf + (x * pdf).abs())
+
+
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 8), (3, 31), (5, 64), (129, 333), (64, 1536), (2, 4099)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tanh", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+def test_gelu8(rows, width, dtype, tanh, gated):
+    import concord_amd as ca
+    g = _gen("gelu", rows, width, dtype, tanh, gated)
+    # the whole range in which the normal distribution is neither 0 nor 1
+    x = (torch.randn(rows, width * (2 if gated else 1), generator=g, device=DEV) * 4).to(dtype).requires_grad_(True)
+    dy = torch.randn(rows, width, generator=g, device=DEV).to(dtype)
+    f = ca.geglu8 if gated else ca.gelu8
+    y = f(x, approximate="tanh" if tanh else "none")
+    dx, = torch.autograd.grad(y, (x,), dy)
+    assert y.dtype == dtype == dx.dtype and dx.shape == x.shape and y.shape == dy.shape
+    d = dy.double()
+    if gated:
+        a, b = x.detach().double().chunk(2, -1)
+        v, _, rel, _ = _gelu64(b, tanh)
+        _close(y.detach(), a * v, (a * v).abs() * (rel + U) + a.abs() * 2.0 ** -120, dtype, "y")
+        ka, kb = (_kept(t)[2] for t in x.detach().chunk(2, -1))
+        v, dv, rel, bound = _gelu64(kb, tanh)
+        _close(dx[:, :width], d * v, (d * v).abs() * (rel + U) + d.abs() * 2.0 ** -120, dtype, "da")
+        _close(dx[:, width:], d * ka * dv, (d * ka).abs() * (bound + 2 * U * dv.abs() + 2.0 ** -120), dtype, "dg")
+    else:
+        v, _, rel, _ = _gelu64(x.detach().double(), tanh)
+        _close(y.detach(), v, v.abs() * rel + 2.0 ** -120, dtype, "y")
+        _, dv, _, bound = _gelu64(_kept(x.detach())[2], tanh)
+        _close(dx, d * dv, d.abs() * (bound + U * dv.abs() + 2.0 ** -120), dtype, "dx")
+    with torch.no_grad():
+        assert torch.equal(f(x, approximate="tanh" if tanh else "none"), y.detach())
+
+
+@pytest.mark.parametrize("tanh", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gelu8_far_out(dtype, tanh):
+    """Past |x| = 16 the result is x or 0 and the derivative 1 or 0, up to the type's largest number."""
+    import concord_amd as ca
+    most = torch.finfo(dtype).max
+    x = torch.tensor([most, -most, 1e4, -1e4, 17.0, -17.0, 0.0, -0.0], device=DEV).to(dtype)
+    x = x[:, None].repeat(1, 32).requires_grad_(True)   # a block of each
+    y = ca.gelu8(x, approximate="tanh" if tanh else "none")
+    dx, = torch.autograd.grad(y, (x,), torch.ones_like(y))
+    want = x.detach().clamp_min(0)
+    assert torch.equal(y.detach(), want)
+    slope = torch.tensor([1.0, 0, 1, 0, 1, 0, 0.5, 0.5], device=DEV)[:, None].expand(8, 32)
+    _close(dx, slope.double(), slope.double() * 16 * U + 2.0 ** -100, dtype)
+
+
+def test_gelu8_infinities_and_nan_stay_in_their_block():
+    import concord_amd as ca
+    g = _gen("gelu nan")
+    x = torch.randn(4, 128, generator=g, device=DEV)
+    bad = x.clone()
+    bad[1, 40] = math.nan
+    bad[2, 3] = math.inf
+    x.requires_grad_(True), bad.requires_grad_(True)
+    y, z = ca.gelu8(x), ca.gelu8(bad)
+    up = torch.ones_like(x)
+    (dx,), (dz,) = torch.autograd.grad(y, (x,), up), torch.autograd.grad(z, (bad,), up)
+    rest = torch.ones(4, 128, dtype=torch.bool, device=DEV)
+    rest[1, 40] = rest[2, 3] = False
+    assert torch.equal(y[rest], z[rest]) and torch.isnan(z[1, 40]) and float(z[2, 3].detach()) == math.inf
+    rest[1, 32:64] = rest[2, :32] = False
+    assert torch.equal(dx[rest], dz[rest]) and torch.isnan(dz[~rest]).all()
+
+
+def test_gelu8_layouts():
+    import concord_amd as ca
+    g = _gen("gelu layouts")
+    big = torch.randn(6, 50, 208, generator=g, device=DEV).to(BF16)
+    for x in (big[:, :, 5:101], big[:, :, 8:104], big[:, ::2], big.transpose(1, 2), big[:0], big[0, 0]):
+        for f in (ca.gelu8, ca.geglu8):
+            a = x.detach().requires_grad_(True)
+            b = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
+            ya, yb = f(a), f(b)
+            up = torch.randn(ya.shape, generator=g, device=DEV).to(BF16)
+            wide = torch.zeros(*up.shape[:-1], up.shape[-1] + 3, device=DEV, dtype=BF16)
+            wide[..., 1:-2] = up
+            da, = torch.autograd.grad(ya, (a,), wide[..., 1:-2])
+            db, = torch.autograd.grad(yb, (b,), up)
+            assert torch.equal(ya, yb) and torch.equal(da, db)
+
+
+def test_gelu8_gradient_against_differences():
+    """x on a grid that the 8-bit form holds exactly, so the gradient is gelu's own."""
+    import concord_amd as ca
+    g = _gen("gelu differences")
+    x = (torch.randint(-64, 64, (8, 64), generator=g, device=DEV) / 32.0).requires_grad_(True)
+    for f, tanh in ((ca.gelu8, False), (ca.gelu8, True), (ca.geglu8, False)):
+        y = f(x, approximate="tanh" if tanh else "none")
+        up = torch.randn(y.shape, generator=g, device=DEV)
+        dx, = torch.autograd.grad(y, (x,), up)
+        direction = torch.randn(x.shape, generator=g, device=DEV).double()
+
+        def value(t):
+            z = x.detach().double() + t * direction
+            if f is ca.geglu8:
+                a, b = z.chunk(2, -1)
+                return float((a * _gelu64(b, tanh)[0] * up.double()).sum())
+            return float((_gelu64(z, tanh)[0] * up.double()).sum())
+        slope = (value(1e-4) - value(-1e-4)) / 2e-4
+        size = float((dx.double() * direction).abs().sum())
+        assert abs(float((dx.double() * direction).sum()) - slope) <= (64 * U + 10 * 1e-8) * size
