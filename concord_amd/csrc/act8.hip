@@ -7,11 +7,11 @@
 //   gated:  y = a f(g), a and g the halves of a row;   da = dy f(gz), dg = dy az f'(gz)
 // z, az, gz: the values that the codes stand for.
 //
-// Bound by memory.  A thread takes 8 adjacent values; the four threads of a quad
-// hold a block of the 8-bit form, so its largest magnitude is two lane exchanges
-// away.  Rows that begin on no 16-byte boundary (odd widths) are read and written
+// Bound by memory and instructions alike.  A thread takes 16 bytes of adjacent values at
+// a time; four adjacent threads (fp32: eight) hold a block of the 8-bit form, so its
+// largest magnitude is two or three lane exchanges away.  Rows that begin on no 16-byte boundary (odd widths) are read and written
 // with the same wide accesses at the alignment of one element, which this GPU
-// takes; a row's last 1 to 7 values go one by one.
+// takes; what is left at a row's end goes one by one.
 #include "act8.h"
 
 namespace concord {
@@ -29,197 +29,276 @@ struct Act8Args {
   uint32_t nb;          // blocks of C columns
 };
 
-template <class T, bool ALIGNED>
-struct alignas(ALIGNED ? sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16 : sizeof(T)) Eight {
-  T v[8];
+// N adjacent elements, on 16 bytes (or their own size) or wherever an element may begin
+template <class T, int N, bool ALIGNED>
+struct alignas(ALIGNED ? (sizeof(T) * N < 16 ? sizeof(T) * N : 16) : sizeof(T)) Run {
+  T v[N];
 };
 
-template <class T, bool ALIGNED>
-CONCORD_DEV void load8(float (&v)[8], const T* p, int64_t n) {
-  typedef Eight<T, ALIGNED> E;
-  E r = {};
-  if (n >= 8) {
-    r = *(const E*)p;
-  } else if (!ALIGNED) {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) r.v[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(r.v[i]);
-}
-template <class T, bool ALIGNED>
-CONCORD_DEV void store8(T* p, int64_t n, const float (&v)[8]) {
-  typedef Eight<T, ALIGNED> E;
-  E r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = from_f32<T>(v[i]);
-  if (n >= 8) {
-    *(E*)p = r;
-  } else if (!ALIGNED) {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) p[i] = r.v[i];
-  }
-}
-template <bool ALIGNED>
-CONCORD_DEV void store_codes(uint8_t* p, int64_t n, uint32_t lo, uint32_t hi) {
-  typedef Eight<uint8_t, ALIGNED> E;
-  if (n >= 8) {
-    *(E*)p = __builtin_bit_cast(E, (uint64_t)hi << 32 | lo);
-  } else if (!ALIGNED) {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) p[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
-  }
-}
-template <bool ALIGNED>
-CONCORD_DEV void load_codes(const uint8_t* p, int64_t n, uint32_t& lo, uint32_t& hi) {
-  typedef Eight<uint8_t, ALIGNED> E;
-  lo = hi = 0;
-  if (n >= 8) {
-    const uint64_t w = __builtin_bit_cast(uint64_t, *(const E*)p);
-    lo = (uint32_t)w, hi = (uint32_t)(w >> 32);
-  } else if (!ALIGNED) {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < n) (i < 4 ? lo : hi) |= (uint32_t)p[i] << (8 * (i & 3));
+// a result that this kernel does not read again: past the caches, where it lies on its size
+template <bool ALIGNED, class V>
+CONCORD_DEV void store_wide(void* p, const V& v) {
+  if constexpr (!ALIGNED) {
+    *(V*)p = v;
+  } else if constexpr (sizeof(V) == 4) {
+    __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, v), (uint32_t*)p);
+  } else if constexpr (sizeof(V) == 8) {
+    __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, v), (uint64_t*)p);
+  } else {
+    store_stream((V*)p, v);
   }
 }
 
-// the thread's place: eight columns from c of a row
-struct Place8 {
-  int64_t row, c, n;   // n: columns that the row still has (0 or less: none)
+// Values that a thread takes at a time: 16 bytes of them, so that a wave's accesses
+// leave no gaps (fp32: 4, unpacking 4099 x 1283 took 9.7 us by 8, by 4 it takes 8.0)
+template <class T>
+constexpr int kWide = 16 / (int)sizeof(T);
+
+// V values of a row as they lie in memory, zeros past its end
+template <class T, bool ALIGNED>
+struct Values {
+  static constexpr int V = kWide<T>;
+  typedef Run<T, V, ALIGNED> All;
+  All r;
+  CONCORD_DEV void load(const T* p, int n) {
+    r = All{};
+    if (n >= V) {
+      r = *(const All*)p;
+    } else if (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i)
+        if (i < n) r.v[i] = p[i];
+    }
+  }
+  CONCORD_DEV void get(float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32(r.v[i]);
+  }
+  // bits of the largest magnitude as an fp32 number (above infinity's where there is a NaN)
+  CONCORD_DEV uint32_t top() const {
+    struct Words {
+      uint32_t w[4];
+    };
+    const Words w = __builtin_bit_cast(Words, r);
+    if constexpr (sizeof(T) == 4) {
+      return max(max(w.w[0] & 0x7FFFFFFFu, w.w[1] & 0x7FFFFFFFu), max(w.w[2] & 0x7FFFFFFFu, w.w[3] & 0x7FFFFFFFu));
+    } else {
+      // two values a word: 16-bit numbers without their signs are in order as integers
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 m = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w.w[i] & 0x7FFF7FFFu));
+      return __float_as_uint(to_f32(__builtin_bit_cast(T, max(m.x, m.y))));
+    }
+  }
+  CONCORD_DEV void store(T* p, int n, const float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_f32<T>(v[i]);
+    if (n >= V) {
+      store_wide<ALIGNED>(p, r);
+    } else if (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i)
+        if (i < n) p[i] = r.v[i];
+    }
+  }
+};
+
+// their codes
+template <class T, bool ALIGNED>
+struct Codes {
+  static constexpr int V = kWide<T>;
+  typedef Run<uint8_t, V, ALIGNED> All;
+  struct Words {
+    uint32_t w[V / 4];
+  } c;
+  CONCORD_DEV void load(const uint8_t* p, int n) {
+    c = {};
+    if (n >= V) {
+      c = __builtin_bit_cast(Words, *(const All*)p);
+    } else if (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i)
+        if (i < n) c.w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
+    }
+  }
+  CONCORD_DEV void store(uint8_t* p, int n) const {
+    if (n >= V) {
+      store_wide<ALIGNED>(p, __builtin_bit_cast(All, c));
+    } else if (!ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i)
+        if (i < n) p[i] = (uint8_t)(c.w[i >> 2] >> (8 * (i & 3)));
+    }
+  }
+};
+
+// a thread's place: V columns from c of a row
+struct Place {
+  int64_t row, c;
+  int n;            // columns that the row still has, V for more (0 or less: none)
   uint32_t block;
 };
-template <class T>
-CONCORD_DEV Place8 place8(const Act8Args& a, uint32_t id) {
-  Place8 p;
-  const uint32_t per = a.nb * 4, row = id / per, in = id - row * per;
+template <int V>
+CONCORD_DEV Place place(const Act8Args& a, uint32_t id) {
+  constexpr uint32_t EACH = kBlock8 / V;   // threads of a block
+  Place p;
+  const uint32_t per = a.nb * EACH, row = a.rows == 1 ? 0 : id / per, in = id - row * per;
   p.row = row;
-  p.c = (int64_t)in * 8;
-  p.n = a.C - p.c;
-  p.block = in >> 2;
+  p.c = (int64_t)in * V;
+  p.n = (int)min(a.C - p.c, (int64_t)V);
+  p.block = in / EACH;
   return p;
 }
 
-// encode the thread's eight values; the quad's first thread writes the exponent
-template <bool ALIGNED>
-CONCORD_DEV void keep8(const float (&v)[8], const Place8& p, uint8_t* codes, uint8_t* exps) {
-  uint32_t top = 0;
+// A block of 256 threads takes K * 256 places, a thread every 256th of them: what a wave
+// loads or stores at once lies side by side, and its loads are all out before it waits for
+// the first.  f(place) for each place there is.
+template <int K, int V, class F>
+CONCORD_DEV void each_place(const Act8Args& a, uint32_t count, F&& f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[i]));
+  for (int k = 0; k < K; ++k) {
+    const uint32_t id = (blockIdx.x * K + k) * 256 + threadIdx.x;
+    if (id < count) f(k, place<V>(a, id));
+  }
+}
+
+// one place where its loads are many already (a gated row's two halves) or its rows do
+// not begin on 16 bytes
+constexpr int places(bool gated, bool aligned) { return gated || !aligned ? 1 : 2; }
+
+// encode the thread's values; the first thread of a block's four or eight writes the exponent
+template <class T, bool ALIGNED>
+CONCORD_DEV void keep8(const Values<T, ALIGNED>& x, const float (&v)[kWide<T>], const Place& p, uint8_t* codes,
+                       uint8_t* exps) {
+  constexpr int V = kWide<T>, EACH = kBlock8 / V;
+  uint32_t top = x.top();
   top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));   // quad_perm 1, 0, 3, 2
   top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));   // quad_perm 2, 3, 0, 1
+  if (EACH == 8) top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, true));   // row_half_mirror
   const uint32_t e8 = exponent8(top);
   const float inv = inverse_step8(e8);
-  store_codes<ALIGNED>(codes + p.c, p.n, codes8(v, inv, e8 == kBad8), codes8(v + 4, inv, e8 == kBad8));
-  if ((threadIdx.x & 3) == 0) exps[p.block] = (uint8_t)e8;
+  Codes<T, ALIGNED> c;
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) c.c.w[i] = e8 == kBad8 ? 0 : codes8(v + 4 * i, inv);
+  c.store(codes + p.c, p.n);
+  if ((threadIdx.x & (EACH - 1)) == 0) exps[p.block] = (uint8_t)e8;
 }
 template <class T, bool ALIGNED>
-CONCORD_DEV void kept8(float (&v)[8], const Place8& p, const uint8_t* codes, const uint8_t* exps) {
-  uint32_t lo, hi;
-  load_codes<ALIGNED>(codes + p.c, p.n, lo, hi);
-  const uint32_t e8 = exps[p.block];
-  const float step = step8(e8);
-  const bool large = e8 >= Largest<T>::e8;
+CONCORD_DEV void kept8(float (&v)[kWide<T>], const Codes<T, ALIGNED>& c, uint32_t e8) {
+  const float step = step8(e8), less = -128.0f * step;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = value8<T>(__builtin_amdgcn_sbfe((int)(i < 4 ? lo : hi), 8 * (i & 3), 8), step, large);
+  for (int i = 0; i < kWide<T> / 4; ++i) values8<T>(v + 4 * i, c.c.w[i], step, less, e8 >= Largest<T>::e8);
 }
 
 template <class T, bool ALIGNED>
 __global__ __launch_bounds__(256) void pack8_kernel(Act8Args a, uint32_t count) {
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
-  if (id >= count) return;
-  const Place8 p = place8<T>(a, id);
-  float v[8];
-  load8<T, ALIGNED>(v, (const T*)a.x + p.row * a.ldx + p.c, p.n);
-  keep8<ALIGNED>(v, p, a.codes + p.row * a.C, a.exps + p.row * a.nb);
+  constexpr int V = kWide<T>, K = places(false, ALIGNED);
+  Values<T, ALIGNED> x[K];
+  each_place<K, V>(a, count, [&](int k, const Place& p) { x[k].load((const T*)a.x + p.row * a.ldx + p.c, p.n); });
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    float v[V];
+    x[k].get(v);
+    keep8(x[k], v, p, a.codes + p.row * a.C, a.exps + p.row * a.nb);
+  });
 }
 
 template <class T, bool ALIGNED>
 __global__ __launch_bounds__(256) void unpack8_kernel(Act8Args a, uint32_t count) {
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
-  if (id >= count) return;
-  const Place8 p = place8<T>(a, id);
-  float v[8];
-  kept8<T, ALIGNED>(v, p, a.codes + p.row * a.C, a.exps + p.row * a.nb);
-  store8<T, ALIGNED>((T*)a.out + p.row * a.ldo + p.c, p.n, v);
+  constexpr int V = kWide<T>, K = places(false, ALIGNED);
+  Codes<T, ALIGNED> c[K];
+  uint32_t e8[K];
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    c[k].load(a.codes + p.row * a.C + p.c, p.n);
+    e8[k] = a.exps[p.row * a.nb + p.block];
+  });
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    float v[V];
+    kept8(v, c[k], e8[k]);
+    Values<T, ALIGNED> x;
+    x.store((T*)a.out + p.row * a.ldo + p.c, p.n, v);
+  });
 }
 
 template <class T, class F, bool GATED, bool ALIGNED>
 __global__ __launch_bounds__(256) void gelu8_fwd_kernel(Act8Args a, uint32_t count) {
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
-  if (id >= count) return;
-  const Place8 p = place8<T>(a, id);
-  const T* x = (const T*)a.x + p.row * a.ldx + p.c;
-  float v[8], y[8];
-  if (GATED) {
-    float g[8];
-    load8<T, ALIGNED>(v, x, p.n);
-    load8<T, ALIGNED>(g, x + a.C, p.n);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[i] * F::value(g[i]);
-    if (a.codes) {
-      uint8_t *codes = a.codes + p.row * 2 * a.C, *exps = a.exps + p.row * 2 * a.nb;
-      keep8<ALIGNED>(v, p, codes, exps);
-      keep8<ALIGNED>(g, p, codes + a.C, exps + a.nb);
+  constexpr int V = kWide<T>, K = places(GATED, ALIGNED);
+  Values<T, ALIGNED> x[K], g[K];
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    const T* at = (const T*)a.x + p.row * a.ldx + p.c;
+    x[k].load(at, p.n);
+    if (GATED) g[k].load(at + a.C, p.n);
+  });
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    float v[V], w[V], y[V];
+    x[k].get(v);
+    const int wide = GATED ? 2 : 1;
+    uint8_t *codes = a.codes + p.row * wide * a.C, *exps = a.exps + p.row * wide * a.nb;
+    if (a.codes) keep8(x[k], v, p, codes, exps);
+    if (GATED) {
+      g[k].get(w);
+      if (a.codes) keep8(g[k], w, p, codes + a.C, exps + a.nb);
     }
-  } else {
-    load8<T, ALIGNED>(v, x, p.n);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = F::value(v[i]);
-    if (a.codes) keep8<ALIGNED>(v, p, a.codes + p.row * a.C, a.exps + p.row * a.nb);
-  }
-  store8<T, ALIGNED>((T*)a.out + p.row * a.ldo + p.c, p.n, y);
+    for (int i = 0; i < V; ++i) y[i] = GATED ? v[i] * F::value(w[i]) : F::value(v[i]);
+    x[k].store((T*)a.out + p.row * a.ldo + p.c, p.n, y);
+  });
 }
 
 template <class T, class F, bool GATED, bool ALIGNED>
 __global__ __launch_bounds__(256) void gelu8_bwd_kernel(Act8Args a, uint32_t count) {
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
-  if (id >= count) return;
-  const Place8 p = place8<T>(a, id);
-  float dy[8], z[8];
-  load8<T, ALIGNED>(dy, (const T*)a.dy + p.row * a.lddy + p.c, p.n);
-  T* out = (T*)a.out + p.row * a.ldo + p.c;
-  if (GATED) {
-    const uint8_t *codes = a.codes + p.row * 2 * a.C, *exps = a.exps + p.row * 2 * a.nb;
-    float g[8];
-    kept8<T, ALIGNED>(z, p, codes, exps);
-    kept8<T, ALIGNED>(g, p, codes + a.C, exps + a.nb);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v, d;
-      F::both(g[i], v, d);
-      g[i] = dy[i] * z[i] * d;
-      z[i] = dy[i] * v;
+  constexpr int V = kWide<T>, K = places(GATED, ALIGNED);
+  Values<T, ALIGNED> r[K];
+  Codes<T, ALIGNED> c[K], cg[K];
+  uint32_t e8[K], eg[K];
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    const int wide = GATED ? 2 : 1;
+    const uint8_t *codes = a.codes + p.row * wide * a.C + p.c, *exps = a.exps + p.row * wide * a.nb + p.block;
+    r[k].load((const T*)a.dy + p.row * a.lddy + p.c, p.n);
+    c[k].load(codes, p.n);
+    e8[k] = exps[0];
+    if (GATED) {
+      cg[k].load(codes + a.C, p.n);
+      eg[k] = exps[a.nb];
     }
-    store8<T, ALIGNED>(out, p.n, z);
-    store8<T, ALIGNED>(out + a.C, p.n, g);
-  } else {
-    kept8<T, ALIGNED>(z, p, a.codes + p.row * a.C, a.exps + p.row * a.nb);
+  });
+  each_place<K, V>(a, count, [&](int k, const Place& p) {
+    float dy[V], z[V];
+    T* out = (T*)a.out + p.row * a.ldo + p.c;
+    r[k].get(dy);
+    kept8(z, c[k], e8[k]);
+    if (GATED) {
+      float g[V];
+      kept8(g, cg[k], eg[k]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v, d;
-      F::both(z[i], v, d);
-      z[i] = dy[i] * d;
+      for (int i = 0; i < V; ++i) {
+        float v, d;
+        F::both(g[i], v, d);
+        g[i] = dy[i] * z[i] * d;
+        z[i] = dy[i] * v;
+      }
+      r[k].store(out, p.n, z);
+      r[k].store(out + a.C, p.n, g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = dy[i] * F::slope(z[i]);
+      r[k].store(out, p.n, z);
     }
-    store8<T, ALIGNED>(out, p.n, z);
-  }
+  });
 }
 
 // ---- host -------------------------------------------------------------------
 enum Act8Pass { kPack8, kUnpack8, kFwd8, kBwd8 };
 
-// eight-value places, those behind a row's end included; -1: too many for a launch
-static int64_t act8_count(int64_t rows, int64_t C) {
-  const int64_t nb = cdiv(C, kBlock8);
-  return rows > ((1LL << 32) - 256) / 4 / nb ? -1 : rows * nb * 4;
+// threads' places, those behind a row's end included; -1: too many for a launch
+static int64_t act8_count(int dtype, int64_t rows, int64_t C) {
+  const int64_t nb = cdiv(C, kBlock8), each = dtype == CONCORD_F32 ? 8 : 4;
+  return rows > ((1LL << 32) - 4096) / each / nb ? -1 : rows * nb * each;
 }
 
 template <class T, class F, bool GATED, bool ALIGNED>
 static void act8_launch(Act8Pass pass, const Act8Args& a, uint32_t count, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv(count, 256)), th(256);
+  const dim3 grid((unsigned)cdiv(count, 256 * places(GATED, ALIGNED))), th(256);
   if (pass == kPack8) hipLaunchKernelGGL((pack8_kernel<T, ALIGNED>), grid, th, 0, st, a, count);
   else if (pass == kUnpack8) hipLaunchKernelGGL((unpack8_kernel<T, ALIGNED>), grid, th, 0, st, a, count);
   else if (pass == kFwd8) hipLaunchKernelGGL((gelu8_fwd_kernel<T, F, GATED, ALIGNED>), grid, th, 0, st, a, count);
@@ -231,19 +310,20 @@ static bool act8_on16(const void* p, int64_t ld, size_t es) { return ((uintptr_t
 template <class T, class F, bool GATED>
 static void act8_rows(Act8Pass pass, const Act8Args& a, uint32_t count, hipStream_t st) {
   const size_t es = sizeof(T);
-  const bool aligned = a.C % 8 == 0 && (!a.x || act8_on16(a.x, a.ldx, es)) && (!a.dy || act8_on16(a.dy, a.lddy, es)) &&
-                       (!a.out || act8_on16(a.out, a.ldo, es)) && ((uintptr_t)a.codes & 7) == 0;
+  const bool aligned = a.C % kWide<T> == 0 && (!a.x || act8_on16(a.x, a.ldx, es)) && (!a.dy || act8_on16(a.dy, a.lddy, es)) &&
+                       (!a.out || act8_on16(a.out, a.ldo, es)) && ((uintptr_t)a.codes & (kWide<T> - 1)) == 0;
   if (aligned) act8_launch<T, F, GATED, true>(pass, a, count, st);
   else act8_launch<T, F, GATED, false>(pass, a, count, st);
 }
 template <class T>
 static void act8_form(Act8Pass pass, const Act8Args& a, uint32_t count, bool tanh, bool gated, hipStream_t st) {
+  constexpr bool FINE = sizeof(T) == 4;
   if (gated) {
-    if (tanh) act8_rows<T, GeluTanh, true>(pass, a, count, st);
-    else act8_rows<T, Gelu, true>(pass, a, count, st);
+    if (tanh) act8_rows<T, GeluTanh<FINE>, true>(pass, a, count, st);
+    else act8_rows<T, Gelu<FINE>, true>(pass, a, count, st);
   } else {
-    if (tanh) act8_rows<T, GeluTanh, false>(pass, a, count, st);
-    else act8_rows<T, Gelu, false>(pass, a, count, st);
+    if (tanh) act8_rows<T, GeluTanh<FINE>, false>(pass, a, count, st);
+    else act8_rows<T, Gelu<FINE>, false>(pass, a, count, st);
   }
 }
 static void act8_run(Act8Pass pass, int dtype, Act8Args a, bool tanh, bool gated, hipStream_t st) {
@@ -254,7 +334,7 @@ static void act8_run(Act8Pass pass, int dtype, Act8Args a, bool tanh, bool gated
     a.ldx = a.lddy = a.ldo = a.C;
   }
   a.nb = (uint32_t)cdiv(a.C, kBlock8);
-  const uint32_t count = (uint32_t)act8_count(a.rows, a.C);
+  const uint32_t count = (uint32_t)act8_count(dtype, a.rows, a.C);
   if (dtype == CONCORD_F32) act8_form<float>(pass, a, count, tanh, gated, st);
   else if (dtype == CONCORD_BF16) act8_form<BF16>(pass, a, count, tanh, gated, st);
   else act8_form<_Float16>(pass, a, count, tanh, gated, st);
@@ -263,7 +343,7 @@ static void act8_run(Act8Pass pass, int dtype, Act8Args a, bool tanh, bool gated
 static int act8_check(const char* name, int dtype, int64_t rows, int64_t C) {
   CONCORD_CHECK(rows >= 0 && C >= 1 && rows < (1LL << 40) && C < (1LL << 40), "%s: bad size", name);
   CONCORD_CHECK(dtype == CONCORD_F32 || dtype == CONCORD_BF16 || dtype == CONCORD_F16, "%s: bad type", name);
-  CONCORD_CHECK(act8_count(rows, C) >= 0, "%s: too many values for a launch", name);
+  CONCORD_CHECK(act8_count(dtype, rows, C) >= 0, "%s: too many values for a launch", name);
   return CONCORD_OK;
 }
 
