@@ -20,7 +20,9 @@
 namespace concord {
 
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
-constexpr int kTile = 4096;          // pairs a block of the sort takes
+// pairs a block of the sort takes: few where the tokens are, since a wave ranks its pairs
+// one after another
+static int emb_tile(int64_t n) { return n <= 65536 ? 1024 : 4096; }
 constexpr int kOneBlock = 4096;      // pairs that one block sorts alone
 
 struct EmbArgs {
@@ -39,6 +41,7 @@ struct EmbArgs {
   float* part;          // [pieces][2][C]: sums of a run's head (it began earlier), of its first rows
   int piece;            // pairs a wave adds
   int64_t pieces;
+  int64_t slabs;        // of 64 lanes' columns
   int64_t fill_at;      // first block of those that write zeros
 };
 
@@ -48,7 +51,9 @@ CONCORD_DEV uint32_t token_key(const void* tokens, int idx64, int64_t i, uint32_
 }
 
 // ---- forward ------------------------------------------------------------------
-// 2^lg threads a row, VEC columns a thread and step
+// 2^lg threads a row, VEC columns a thread and step.  (Four rows at once, their loads
+// out together: no change.  The stores go past the caches: 16384 x 384 in fp32 9.1 -> 7.4
+// us, 32768 x 4096 in bf16 72 -> 75.)
 template <class TW, class TO, int VEC>
 __global__ __launch_bounds__(256) void emb_fwd_kernel(EmbArgs a, int lg) {
   const int64_t step = (int64_t)gridDim.x << (8 - lg);
@@ -63,7 +68,7 @@ __global__ __launch_bounds__(256) void emb_fwd_kernel(EmbArgs a, int lg) {
       Chunk<TO, VEC> r;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<TO>(to_f32(v.v[e]) * a.scale);
-      *(Chunk<TO, VEC>*)(dst + c) = r;
+      store_stream((Chunk<TO, VEC>*)(dst + c), r);
     }
   }
 }
@@ -166,21 +171,22 @@ __global__ __launch_bounds__(1024) void emb_sort_block_kernel(EmbArgs a, int pas
     }
 }
 
-// One pass over many blocks, kTile pairs each: the digits' counts of each block ...
+// One pass over many blocks of 512 IT pairs each: the digits' counts of each block ...
 struct SortPass {
   const uint32_t *keys, *pos;   // NULL in the first pass: the tokens
   uint32_t *out_keys, *out_pos;
   uint32_t* counts;             // [blocks][bins]
   int shift, bits;
 };
+template <int IT>
 __global__ __launch_bounds__(512) void emb_count_kernel(EmbArgs a, SortPass s) {
   __shared__ uint32_t cnt[kMaxBins];
   const int bins = 1 << s.bits;
   if ((int)threadIdx.x < bins) cnt[threadIdx.x] = 0;
   __syncthreads();
-  const int64_t first = (int64_t)blockIdx.x * kTile;
+  const int64_t first = (int64_t)blockIdx.x * (IT * 512);
 #pragma unroll
-  for (int j = 0; j < kTile / 512; ++j) {
+  for (int j = 0; j < IT; ++j) {
     const int64_t i = first + j * 512 + threadIdx.x;
     if (i < a.n) {
       const uint32_t k = s.keys ? s.keys[i] : token_key(a.tokens, a.idx64, i, a.V);
@@ -191,11 +197,11 @@ __global__ __launch_bounds__(512) void emb_count_kernel(EmbArgs a, SortPass s) {
   if ((int)threadIdx.x < bins) s.counts[(int64_t)blockIdx.x * bins + threadIdx.x] = cnt[threadIdx.x];
 }
 // ... and the pairs to their places: behind all smaller digits, behind the same digit of earlier blocks
+template <int IT>
 __global__ __launch_bounds__(512) void emb_scatter_kernel(EmbArgs a, SortPass s) {
-  constexpr int IT = kTile / 512;
   __shared__ uint32_t cnt[8][kMaxBins], sums[8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << s.bits;
-  const int64_t e0 = (int64_t)blockIdx.x * kTile + wave * IT * 64 + lane;
+  const int64_t e0 = (int64_t)blockIdx.x * (IT * 512) + wave * IT * 64 + lane;
   uint32_t k[IT], p[IT], rank[IT];
 #pragma unroll
   for (int j = 0; j < IT; ++j) {
@@ -206,11 +212,18 @@ __global__ __launch_bounds__(512) void emb_scatter_kernel(EmbArgs a, SortPass s)
   }
   uint32_t before = 0, all = 0;
   if ((int)threadIdx.x < bins) {
+    // sixteen blocks' counts in flight: another XCD wrote them, so each load is a long one
+    constexpr int B = 16;
     const uint32_t* c = s.counts + threadIdx.x;
-    for (int64_t b = 0; b < gridDim.x; ++b) {
-      const uint32_t v = c[b * bins];
-      before += b < blockIdx.x ? v : 0;
-      all += v;
+    for (uint32_t b = 0; b < gridDim.x; b += B) {
+      uint32_t v[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) v[i] = c[(int64_t)min(b + i, gridDim.x - 1) * bins];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        before += b + i < blockIdx.x ? v[i] : 0;
+        all += b + i < gridDim.x ? v[i] : 0;
+      }
     }
   }
   for (int i = lane; i < bins; i += 64) cnt[wave][i] = 0;
@@ -245,7 +258,7 @@ CONCORD_DEV void store_row(const EmbArgs& a, uint32_t v, int64_t c, const float 
   Chunk<TW, VEC> r;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<TW>(s[e] * a.scale);
-  *(Chunk<TW, VEC>*)((TW*)a.dst + (int64_t)v * a.ldd + c) = r;
+  store_stream((Chunk<TW, VEC>*)((TW*)a.dst + (int64_t)v * a.ldd + c), r);
 }
 template <int VEC>
 CONCORD_DEV void store_part(const EmbArgs& a, int64_t piece, int which, int64_t c, const float (&s)[VEC]) {
@@ -255,100 +268,124 @@ CONCORD_DEV void store_part(const EmbArgs& a, int64_t piece, int which, int64_t 
   for (int e = 0; e < VEC; ++e) p[e] = s[e];
 }
 
-// first of keys[lo, hi) that is not less than v
+// First of keys[lo, hi) that is not less than v, found by a wave: 64 places at once, so
+// three rounds of loads find one among a quarter of a million.
 CONCORD_DEV int64_t first_not_less(const uint32_t* keys, int64_t lo, int64_t hi, uint32_t v) {
-  while (lo < hi) {
-    const int64_t m = (lo + hi) >> 1;
-    if (keys[m] < v) lo = m + 1;
-    else hi = m;
+  const int lane = threadIdx.x & 63;
+  while (hi > lo) {
+    const int64_t step = (hi - lo + 63) >> 6, at = lo + lane * step;
+    const int less = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at < hi && keys[at] < v));
+    // keys at the first `less` places are less than v, the next is not
+    hi = min(hi, lo + less * step);
+    lo = less ? lo + (less - 1) * step + 1 : hi;
   }
   return lo;
 }
 
-constexpr int kFillRows = 16;   // rows of the table that a wave looks at for zeros
+constexpr int kFillRows = 8;   // rows of the table that a wave looks at for zeros
 
 template <class TG, class TW, int VEC>
 __global__ __launch_bounds__(256) void emb_sum_kernel(EmbArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int64_t)blockIdx.x >= a.fill_at) {
-    // rows of the table without a token (each lane looks for one)
+    // rows of the table without a token
     const int64_t v0 = (((int64_t)blockIdx.x - a.fill_at) * 4 + wave) * kFillRows;
-    const int64_t v = v0 + (lane & (kFillRows - 1));
-    bool empty = false;
-    if (v < a.V) {
-      const int64_t at = first_not_less(a.keys, 0, a.n, (uint32_t)v);
-      empty = at >= a.n || a.keys[at] != (uint32_t)v;
-    }
-    uint64_t todo = __builtin_amdgcn_ballot_w64(empty) & ((1u << kFillRows) - 1);
+    if (v0 >= a.V) return;
+    const int64_t lo = first_not_less(a.keys, 0, a.n, (uint32_t)v0);
+    const int64_t hi = first_not_less(a.keys, lo, a.n, (uint32_t)min(v0 + kFillRows, (int64_t)a.V));
     const float zero[VEC] = {};
-    while (todo) {
-      const int i = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      for (int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC; c < a.C; c += (int64_t)gridDim.y * 64 * VEC)
-        store_row<TW, VEC>(a, (uint32_t)(v0 + i), c, zero);
+    for (int64_t v = v0; v < min(v0 + kFillRows, (int64_t)a.V); ++v) {
+      const int64_t at = hi > lo ? first_not_less(a.keys, lo, hi, (uint32_t)v) : hi;
+      if (at < hi && a.keys[at] == (uint32_t)v) continue;
+      for (int64_t c = (int64_t)lane * VEC; c < a.C; c += 64 * VEC) store_row<TW, VEC>(a, (uint32_t)v, c, zero);
     }
     return;
   }
-  const int64_t piece = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave, piece = item / a.slabs;
   if (piece >= a.pieces) return;
-  const int64_t p0 = piece * a.piece, p1 = min(p0 + a.piece, a.n);
-  const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC;
-  uint32_t cur = a.keys[p0];
-  bool head = p0 > 0 && a.keys[p0 - 1] == cur;
-  float s[VEC] = {};
+  // the piece's pairs, one a lane; their rows are loaded U at a time, the next U while
+  // these are added, and no load is behind a branch (a lane past the last column loads the
+  // first, a step past the last pair its row again)
+  const int64_t p0 = piece * a.piece, p1 = min(p0 + a.piece, a.n), at = min(p0 + lane, p1 - 1);
+  const uint32_t key = a.keys[at], pos = a.pos[at];
+  const uint32_t earlier = p0 > 0 ? a.keys[p0 - 1] : ~0u, later = p1 < a.n ? a.keys[p1] : ~0u;
+  const int m = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < p1 - p0 && key < a.V));
+  if (m == 0) return;   // (tokens outside the table stand last)
+  const int64_t c = ((item - piece * a.slabs) * 64 + lane) * VEC;
+  const TG* src = (const TG*)a.src + (c < a.C ? c : 0);
   constexpr int U = 8;
-  for (int64_t i = p0; i < p1 && cur < a.V; i += U) {
-    Chunk<TG, VEC> r[U];
+  Chunk<TG, VEC> r[2][U];
+  auto load = [&](Chunk<TG, VEC> (&t)[U], int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      t[u] = *(const Chunk<TG, VEC>*)(src + (int64_t)(uint32_t)__builtin_amdgcn_readlane(pos, min(i + u, m - 1)) * a.lds);
+  };
+  uint32_t cur = __builtin_amdgcn_readlane(key, 0);
+  bool head = earlier == cur;
+  float s[VEC] = {};
+  auto add = [&](const Chunk<TG, VEC> (&t)[U], int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      r[u] = {};
-      if (i + u < p1 && c < a.C)
-        r[u] = *(const Chunk<TG, VEC>*)((const TG*)a.src + (int64_t)a.pos[i + u] * a.lds + c);
-    }
+      if (i + u >= m) break;
+      const uint32_t k = __builtin_amdgcn_readlane(key, i + u);
+      if (k != cur) {
+        if (head) store_part<VEC>(a, piece, 0, c, s);
+        else store_row<TW, VEC>(a, cur, c, s);
+        head = false;
+        cur = k;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u < p1 && cur < a.V) {
-        const uint32_t k = a.keys[i + u];
-        if (k != cur) {
-          if (head) store_part<VEC>(a, piece, 0, c, s);
-          else store_row<TW, VEC>(a, cur, c, s);
-          head = false;
-          cur = k;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[e] += to_f32(r[u].v[e]);
+        for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
       }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] += to_f32(t[u].v[e]);
     }
+  };
+  load(r[0], 0);
+  for (int i = 0; i < m; i += 2 * U) {
+    load(r[1], i + U);
+    add(r[0], i);
+    if (i + U >= m) break;
+    load(r[0], i + 2 * U);
+    add(r[1], i + U);
   }
-  if (cur >= a.V) return;   // (tokens outside the table stand last)
-  const bool goes_on = p1 < a.n && a.keys[p1] == cur;
   if (head) store_part<VEC>(a, piece, 0, c, s);
-  else if (goes_on) store_part<VEC>(a, piece, 1, c, s);
+  else if (later == cur) store_part<VEC>(a, piece, 1, c, s);
   else store_row<TW, VEC>(a, cur, c, s);
 }
 
 // Tokens that cross pieces: the block of the piece that such a run begins in
-// adds its sums, each wave every fourth of them, then the waves' sums in order.
+// adds its sums, each wave every eighth of them, then the waves' sums in order.
 template <class TW, int VEC>
-__global__ __launch_bounds__(256) void emb_join_kernel(EmbArgs a) {
-  __shared__ float part[4][64 * VEC];
+__global__ __launch_bounds__(512) void emb_join_kernel(EmbArgs a) {
+  constexpr int W = 8, U = 4;
+  __shared__ float part[W][64 * VEC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t piece = blockIdx.x, p0 = piece * a.piece, p1 = p0 + a.piece;
+  const int64_t piece = blockIdx.x / a.slabs, p0 = piece * a.piece, p1 = p0 + a.piece;
   if (p1 >= a.n) return;
   const uint32_t cur = a.keys[p1 - 1];
   if (cur >= a.V || a.keys[p1] != cur) return;
   if (p0 > 0 && a.keys[p0 - 1] == cur) return;   // it began earlier
   const int64_t last = (first_not_less(a.keys, p1, a.n, cur + 1) - 1) / a.piece;
-  const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC;
+  const int64_t c = ((blockIdx.x - piece * a.slabs) * 64 + lane) * VEC;
   float s[VEC] = {};
   if (c < a.C) {
-    for (int64_t q = piece + 1 + wave; q <= last; q += 4) {
-      const float* h = a.part + q * 2 * a.C + c;
+    const float* h = a.part + c;
+    const int64_t row = 2 * a.C;
+    int64_t q = piece + 1 + wave;
+    for (; q + (U - 1) * W <= last; q += U * W) {
+      float v[U][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[e] += h[e];
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[u][e] = h[(q + u * W) * row + e];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] += v[u][e];
     }
+    for (; q <= last; q += W)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e] += h[q * row + e];
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) part[wave][lane * VEC + e] = s[e];
@@ -359,7 +396,7 @@ __global__ __launch_bounds__(256) void emb_join_kernel(EmbArgs a) {
     for (int e = 0; e < VEC; ++e) {
       s[e] = t[e];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) s[e] += part[w][lane * VEC + e];
+      for (int w = 0; w < W; ++w) s[e] += part[w][lane * VEC + e];
     }
     store_row<TW, VEC>(a, cur, c, s);
   }
@@ -369,13 +406,11 @@ __global__ __launch_bounds__(256) void emb_join_kernel(EmbArgs a) {
 static bool emb_dtype_ok(int t) { return t == CONCORD_F32 || t == CONCORD_BF16 || t == CONCORD_F16; }
 static size_t emb_size(int t) { return t == CONCORD_F32 ? 4 : 2; }
 
-// pairs a wave adds: as many as leave about 4096 waves
-static int emb_piece(int64_t n, int64_t C) {
-  const int64_t waves = n * cdiv(C, 256);
-  int p = 8;
-  while (p < 256 && waves / p > 4096) p *= 2;
-  return p;
-}
+// Pairs a wave adds.  A lane's worth each: fewer cost the join more than they save here
+// (16384 tokens of 65, 384 wide: 8.5 + 4.6 us by 64, 10.6 + 5.7 by 16; 32768 of 50257,
+// 4096 wide: 134 + 11 and 134 + 34).  Among few tokens the chain of loads counts (4000 of
+// 65, 384 wide: 6.7 + 4.3 by 16, 9.4 + 4.0 by 64).
+static int emb_piece(int64_t n) { return n <= 4096 ? 16 : 64; }
 
 struct EmbWorkspace {
   size_t keys[2], pos[2], counts, part, bytes;
@@ -392,8 +427,8 @@ static EmbWorkspace emb_workspace(int64_t n, int64_t C) {
     w.keys[i] = take((size_t)n * 4);
     w.pos[i] = take((size_t)n * 4);
   }
-  w.counts = take((size_t)cdiv(n, kTile) * kMaxBins * 4);
-  w.part = take((size_t)cdiv(n, emb_piece(n, C)) * 2 * (size_t)C * 4);
+  w.counts = take((size_t)cdiv(n, emb_tile(n)) * kMaxBins * 4);
+  w.part = take((size_t)cdiv(n, emb_piece(n)) * 2 * (size_t)C * 4);
   w.bytes = at;
   return w;
 }
@@ -422,12 +457,12 @@ static void emb_fwd(const EmbArgs& a, hipStream_t st) {
 
 template <class TG, class TW, int V>
 static void emb_sums(EmbArgs& a, hipStream_t st) {
-  const unsigned slabs = (unsigned)cdiv(a.C, 64 * V);
-  a.fill_at = cdiv(a.pieces, 4);
-  hipLaunchKernelGGL((emb_sum_kernel<TG, TW, V>), dim3((unsigned)(a.fill_at + cdiv(a.V, 4 * kFillRows)), slabs), dim3(256),
-                     0, st, a);
+  a.slabs = cdiv(a.C, 64 * V);
+  a.fill_at = cdiv(a.pieces * a.slabs, 4);
+  hipLaunchKernelGGL((emb_sum_kernel<TG, TW, V>), dim3((unsigned)(a.fill_at + cdiv(a.V, 4 * kFillRows))), dim3(256), 0, st,
+                     a);
   if (a.pieces > 1)
-    hipLaunchKernelGGL((emb_join_kernel<TW, V>), dim3((unsigned)a.pieces, slabs), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((emb_join_kernel<TW, V>), dim3((unsigned)(a.pieces * a.slabs)), dim3(512), 0, st, a);
 }
 template <class TG, class TW>
 static void emb_bwd(EmbArgs& a, hipStream_t st) {
@@ -494,8 +529,9 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
     return CONCORD_EWORKSPACE;
   }
   CONCORD_CHECK(((uintptr_t)workspace & 15) == 0, "concord_embedding_bwd: the workspace is not on 16 bytes");
-  const int piece = emb_piece(n, C);
-  CONCORD_CHECK(grid_fits(cdiv(n, 4 * piece) + cdiv(V, 4 * kFillRows), 256) && grid_fits(cdiv(n, piece), 256),
+  const int piece = emb_piece(n);
+  // (64 columns a slab where no vector fits)
+  CONCORD_CHECK(grid_fits(cdiv(n, piece) * cdiv(C, 64) + cdiv(V, 4 * kFillRows), 512),
                 "concord_embedding_bwd: too many tokens or rows");
   hipStream_t st = (hipStream_t)stream;
   EmbArgs a{};
@@ -518,14 +554,20 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
       if (n <= 1024) hipLaunchKernelGGL((emb_sort_block_kernel<1>), dim3(1), dim3(1024), 0, st, a, passes, each, keys[0], pos[0]);
       else hipLaunchKernelGGL((emb_sort_block_kernel<kOneBlock / 1024>), dim3(1), dim3(1024), 0, st, a, passes, each, keys[0], pos[0]);
     } else {
-      const dim3 grid((unsigned)cdiv(n, kTile));
+      const int tile = emb_tile(n);
+      const dim3 grid((unsigned)cdiv(n, tile));
       for (int p = 0; p < passes; ++p) {
         SortPass s{};
         if (p) s.keys = keys[at ^ 1], s.pos = pos[at ^ 1];
         s.out_keys = keys[at], s.out_pos = pos[at], s.counts = (uint32_t*)(base + w.counts);
         s.shift = p * each, s.bits = each;
-        hipLaunchKernelGGL(emb_count_kernel, grid, dim3(512), 0, st, a, s);
-        hipLaunchKernelGGL(emb_scatter_kernel, grid, dim3(512), 0, st, a, s);
+        if (tile == 1024) {
+          hipLaunchKernelGGL((emb_count_kernel<2>), grid, dim3(512), 0, st, a, s);
+          hipLaunchKernelGGL((emb_scatter_kernel<2>), grid, dim3(512), 0, st, a, s);
+        } else {
+          hipLaunchKernelGGL((emb_count_kernel<8>), grid, dim3(512), 0, st, a, s);
+          hipLaunchKernelGGL((emb_scatter_kernel<8>), grid, dim3(512), 0, st, a, s);
+        }
         at ^= 1;
       }
       at ^= 1;
