@@ -9,7 +9,7 @@
 //
 // Bound by memory: every row is read once and written once, its statistics are
 // formed again in the backward rather than kept.  A row belongs to L adjacent
-// lanes, 8 elements each, that hold both elements of their pairs, so the rotation
+// lanes, 8 or 16 elements each, that hold both elements of their pairs, so the rotation
 // exchanges nothing; a lane's angles depend on the token alone and serve all heads
 // that it takes.  Angles are formed in 64 bits (a far position times a frequency
 // loses its fraction in 32) and reduced to an eighth of a turn before the sine and
@@ -30,24 +30,27 @@ struct QkArgs {
   uint32_t T, seq, pos_seq; // tokens; tokens of a sequence; period of pos
   int H[2];
   int D, R, adjacent;
-  int heads, parts0;        // heads of a block's slice; slices of q
+  int heads[2];             // heads of a slice
+  uint32_t blocks[2];       // blocks of a slice
+  uint32_t k_at;            // first block of k's slices
   float eps;
   double log2_base;
   float* part[2];           // backward: [blocks of q's or k's slices][D] partial dw, or NULL
 };
 
-// the lane's four pairs: elements (a + j, b + j), or (a + 2 j, a + 2 j + 1) where pairs are adjacent
+// a lane's V pairs: elements (a + j, b + j), or (a + 2 j, a + 2 j + 1) where pairs are adjacent
 struct QkLane {
   int a, b;
   bool in, turned;
 };
+template <int V>
 CONCORD_DEV QkLane qk_lane(int l, int D, int R, bool adjacent) {
   QkLane s;
-  s.in = l * 8 < D;
-  s.turned = l * 8 < R;
-  if (adjacent) s.a = l * 8, s.b = l * 8 + 4;
-  else if (s.turned) s.a = l * 4, s.b = R / 2 + l * 4;
-  else s.a = R + (l * 8 - R) / 2, s.b = s.a + (D - R) / 2;
+  s.in = l * 2 * V < D;
+  s.turned = l * 2 * V < R;
+  if (adjacent) s.a = l * 2 * V, s.b = s.a + V;
+  else if (s.turned) s.a = l * V, s.b = R / 2 + l * V;
+  else s.a = R + (l * 2 * V - R) / 2, s.b = s.a + (D - R) / 2;
   return s;
 }
 
@@ -73,128 +76,162 @@ CONCORD_DEV void sincos_quarters(double quarters, float& c, float& s) {
   s = q & 2 ? -v : v;
 }
 
-// sum over the group of L lanes, to each
+// sum over the group of L lanes, to each: lanes 1 and 2 apart, the mirrored half row, the
+// mirrored row, the other row
 template <int L>
 CONCORD_DEV float group_sum(float v) {
-#pragma unroll
-  for (int h = 1; h < L; h <<= 1) v += __shfl_xor(v, h, 64);
+#define CONCORD_DPP_ADD(ctrl) \
+  v = __fadd_rn(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true)))
+  if (L > 1) CONCORD_DPP_ADD(0xB1);
+  if (L > 2) CONCORD_DPP_ADD(0x4E);
+  if (L > 4) CONCORD_DPP_ADD(0x141);
+  if (L > 8) CONCORD_DPP_ADD(0x140);
+#undef CONCORD_DPP_ADD
+  if (L > 16) v += __shfl_xor(v, 16, 64);
   return v;
 }
 
-template <class T>
+// a lane's share of a row; a lane behind the row's end holds the row's first elements
+// and stores nothing
+template <class T, int V>
 struct QkRow {
-  typedef Chunk<T, 4> V;
-  V a, b;
-  CONCORD_DEV void load(const void* p, int64_t at, const QkLane& s) {
-    a = {}, b = {};
-    if (s.in) {
-      a = *(const V*)((const T*)p + at + s.a);
-      b = *(const V*)((const T*)p + at + s.b);
-    }
+  typedef Chunk<T, V> C;
+  C a, b;
+  CONCORD_DEV void load(const T* p, const QkLane& s) {
+    a = *(const C*)(p + (s.in ? s.a : 0));
+    b = *(const C*)(p + (s.in ? s.b : 0));
   }
-  CONCORD_DEV void get(float (&v)[8]) const {
+  CONCORD_DEV void get(float (&v)[2 * V], const QkLane& s) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = to_f32(a.v[j]), v[4 + j] = to_f32(b.v[j]);
+    for (int j = 0; j < V; ++j) v[j] = s.in ? to_f32(a.v[j]) : 0.0f, v[V + j] = s.in ? to_f32(b.v[j]) : 0.0f;
   }
-  CONCORD_DEV void put(const float (&v)[8]) {
+  CONCORD_DEV void store(T* p, const QkLane& s, const float (&v)[2 * V]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a.v[j] = from_f32<T>(v[j]), b.v[j] = from_f32<T>(v[4 + j]);
-  }
-  CONCORD_DEV void store(void* p, int64_t at, const QkLane& s) const {
+    for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(v[j]), b.v[j] = from_f32<T>(v[V + j]);
     if (s.in) {
-      *(V*)((T*)p + at + s.a) = a;
-      *(V*)((T*)p + at + s.b) = b;
+      store_stream((C*)(p + s.a), a);
+      store_stream((C*)(p + s.b), b);
     }
   }
 };
 
 // v's pairs turned by +t (dir = 1) or -t (dir = -1)
-template <bool ADJ>
-CONCORD_DEV void turn(float (&v)[8], const float (&c)[4], const float (&s)[4], float dir) {
+template <bool ADJ, int V>
+CONCORD_DEV void turn(float (&v)[2 * V], const float (&c)[V], const float (&s)[V], float dir) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int ia = ADJ ? 2 * j : j, ib = ADJ ? 2 * j + 1 : 4 + j;
+  for (int j = 0; j < V; ++j) {
+    const int ia = ADJ ? 2 * j : j, ib = ADJ ? 2 * j + 1 : V + j;
     const float a = v[ia], b = v[ib], sn = s[j] * dir;
     v[ia] = __builtin_fmaf(a, c[j], -(b * sn));
     v[ib] = __builtin_fmaf(a, sn, b * c[j]);
   }
 }
 
-// Block (x, y): tokens of groups x, x + gridDim.x, ...; slice y of the heads,
-// q's slices before k's.
-template <class T, int L, bool ADJ, bool BWD>
+// Blocks of a slice of the heads (q's slices, then k's) share the tokens: a group of L
+// lanes takes a token's heads of the slice, U at a time.
+template <class T, int V, int L, bool ADJ, bool BWD>
 __global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
-  constexpr int G = 256 / L, U = BWD ? 2 : 4;
-  __shared__ float sums[BWD ? G : 1][BWD ? L * 8 : 1];
+  constexpr int G = 256 / L, U = BWD ? 2 : 4, E = 2 * V;
+  __shared__ float sums[BWD ? G : 1][BWD ? L * E : 1];
   const int l = threadIdx.x & (L - 1), g = threadIdx.x / L;
-  const int which = (int)blockIdx.y >= a.parts0;
-  const int h0 = ((int)blockIdx.y - (which ? a.parts0 : 0)) * a.heads, H = a.H[which], h1 = min(h0 + a.heads, H);
-  const QkLane s = qk_lane(l, a.D, a.R, ADJ);
-  float w[8], dw[8];
+  const int which = blockIdx.x >= a.k_at;
+  const uint32_t bid = blockIdx.x - (which ? a.k_at : 0), slice = bid / a.blocks[which], nb = a.blocks[which];
+  const int H = a.H[which], h0 = (int)slice * a.heads[which], h1 = min(h0 + a.heads[which], H);
+  const QkLane s = qk_lane<V>(l, a.D, a.R, ADJ);
+  const T *x0 = (const T*)a.x[which], *y0 = (const T*)a.dy[which];
+  const int64_t x_t = a.x_t[which], x_h = a.x_h[which], dy_t = a.dy_t[which], dy_h = a.dy_h[which];
+  float w[E], dw[E];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    dw[j] = 0.0f;
-    w[j] = 1.0f;
-    if (a.w[which] && s.in) w[j] = load_any(a.w[which], a.wtype, (j < 4 ? s.a : s.b) + (j & 3));
+  for (int j = 0; j < E; ++j) dw[j] = 0.0f, w[j] = 1.0f;
+  if (const void* wp = a.w[which]) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) w[j] = load_any(wp, a.wtype, s.in ? (j < V ? s.a : s.b) + j % V : 0);
   }
   // the lane's first frequency, in quarter turns a position, and the step from pair to pair
   const double each = a.R ? -2.0 * a.log2_base / a.R : 0.0;
-  const double freq0 = exp2(each * (l * 4)) * 0.63661977236758134, ratio = exp2(each);
+  const double freq0 = exp2(each * (l * V)) * 0.63661977236758134, ratio = exp2(each);
   const float inv_d = 1.0f / (float)a.D;
-  for (uint32_t t = blockIdx.x * G + g; t < a.T; t += gridDim.x * G) {
-    float c[4], sn[4];
-    {
-      const uint32_t at = a.pos ? t % a.pos_seq : t % a.seq;
-      const int64_t p = !a.pos ? (int64_t)at : a.pos64 ? ((const int64_t*)a.pos)[at] : ((const int32_t*)a.pos)[at];
-      double f = freq0;
+  // The group's rows in batches of up to U heads of a token.  The next batch, the next
+  // token's included, is loaded before this one is worked on.
+  QkRow<T, V> x[2][U], y[2][BWD ? U : 1];
+  float c[V], sn[V];
+  const uint32_t step = nb * G;
+  auto load = [&](int b, uint32_t t, int h) {
+    const T *xt = x0 + t * x_t, *yt = y0 + t * dy_t;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sincos_quarters((double)p * f, c[j], sn[j]);
-        if (!s.turned) c[j] = 1.0f, sn[j] = 0.0f;
-        f *= ratio;
-      }
+    for (int u = 0; u < U; ++u) {
+      const int hu = min(h + u, h1 - 1);
+      x[b][u].load(xt + hu * x_h, s);
+      if (BWD) y[b][u].load(yt + hu * dy_h, s);
     }
-    const int64_t xt = t * a.x_t[which], ot = ((int64_t)t * H) * a.D, dt = BWD ? t * a.dy_t[which] : 0;
-    for (int h = h0; h < h1; h += U) {
-      QkRow<T> x[U], y[U];
+  };
+  auto position = [&](uint32_t t) {
+    const uint32_t at = a.pos ? t % a.pos_seq : t % a.seq;
+    return !a.pos ? (int64_t)at : a.pos64 ? ((const int64_t*)a.pos)[at] : (int64_t)((const int32_t*)a.pos)[at];
+  };
+  auto angles = [&](int64_t p) {
+    double f = freq0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int hu = min(h + u, h1 - 1);
-        x[u].load(a.x[which], xt + hu * a.x_h[which], s);
-        if (BWD) y[u].load(a.dy[which], dt + hu * a.dy_h[which], s);
-      }
+    for (int j = 0; j < V; ++j) {
+      sincos_quarters((double)p * f, c[j], sn[j]);
+      if (!s.turned) c[j] = 1.0f, sn[j] = 0.0f;
+      f *= ratio;
+    }
+  };
+  auto work = [&](int b, uint32_t t, int h) {
+    T* out = (T*)a.out[which] + ((int64_t)t * H + h) * a.D;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (h + u >= h1) continue;
-        float v[8];
-        x[u].get(v);
-        float q = 0.0f;
+    for (int u = 0; u < U; ++u) {
+      if (h + u >= h1) break;
+      float v[E];
+      x[b][u].get(v, s);
+      float q = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q = __builtin_fmaf(v[j], v[j], q);
-        const float r = 1.0f / __builtin_sqrtf(group_sum<L>(q) * inv_d + a.eps);
-        if (!BWD) {
+      for (int j = 0; j < E; ++j) q = __builtin_fmaf(v[j], v[j], q);
+      const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<L>(q), inv_d, a.eps));
+      if constexpr (!BWD) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[j];
-          turn<ADJ>(v, c, sn, 1.0f);
-        } else {
-          float d[8];
-          y[u].get(d);
-          turn<ADJ>(d, c, sn, -1.0f);
-          float along = 0.0f;
+        for (int j = 0; j < E; ++j) v[j] = v[j] * r * w[j];
+        turn<ADJ, V>(v, c, sn, 1.0f);
+      } else {
+        float d[E];
+        y[b][u].get(d, s);
+        turn<ADJ, V>(d, c, sn, -1.0f);
+        float along = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[j] *= r;
-            dw[j] = __builtin_fmaf(d[j], v[j], dw[j]);
-            d[j] *= w[j];
-            along = __builtin_fmaf(d[j], v[j], along);
-          }
-          along = group_sum<L>(along) * inv_d;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = r * __builtin_fmaf(-v[j], along, d[j]);
+        for (int j = 0; j < E; ++j) {
+          v[j] *= r;
+          dw[j] = __builtin_fmaf(d[j], v[j], dw[j]);
+          d[j] *= w[j];
+          along = __builtin_fmaf(d[j], v[j], along);
         }
-        x[u].put(v);
-        x[u].store(a.out[which], ot + (int64_t)(h + u) * a.D, s);
+        along = group_sum<L>(along) * inv_d;
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = r * __builtin_fmaf(-v[j], along, d[j]);
       }
+      x[b][u].store(out + (int64_t)u * a.D, s, v);
+    }
+  };
+  uint32_t t = (bid - slice * nb) * G + g;
+  int h = h0;
+  if (t < a.T) {
+    load(0, t, h);
+    int64_t p = position(t);
+    // one batch from buffer b; false after the last
+    auto batch = [&](int b) {
+      if (h == h0) angles(p);
+      const bool same = h + U < h1;
+      const uint32_t t2 = same ? t : t + step;
+      const int h2 = same ? h + U : h0;
+      if (t2 < a.T) {
+        load(b ^ 1, t2, h2);
+        if (!same) p = position(t2);
+      }
+      work(b, t, h);
+      t = t2, h = h2;
+      return t < a.T;
+    };
+    while (batch(0) && batch(1)) {
     }
   }
   if constexpr (BWD) {
@@ -202,15 +239,14 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
     // the block's groups in order
     if (s.in) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sums[g][(j < 4 ? s.a : s.b) + (j & 3)] = dw[j];
+      for (int j = 0; j < E; ++j) sums[g][(j < V ? s.a : s.b) + j % V] = dw[j];
     }
     __syncthreads();
-    const int64_t row = (int64_t)((int)blockIdx.y - (which ? a.parts0 : 0)) * gridDim.x + blockIdx.x;
     for (int i = threadIdx.x; i < a.D; i += 256) {
       float v = sums[0][i];
 #pragma unroll
       for (int k = 1; k < G; ++k) v += sums[k][i];
-      a.part[which][row * a.D + i] = v;
+      a.part[which][(int64_t)bid * a.D + i] = v;
     }
   }
 }
@@ -250,51 +286,88 @@ __global__ __launch_bounds__(1024) void qk_dw_kernel(const float* p0, const floa
 
 // ---- host -------------------------------------------------------------------
 struct QkPlan {
-  int lanes;        // of a row
-  int heads;        // a slice
-  int parts[2];     // slices of q and of k
-  unsigned blocks;  // of tokens
+  int v, lanes;        // elements of a lane's half, lanes of a row
+  int heads[2];        // a slice's
+  int parts[2];        // slices of q and of k
+  uint32_t blocks[2];  // of a slice
 };
-static QkPlan qk_plan(int64_t T, int H, int HK, int D, bool bwd) {
+static QkPlan qk_plan(const concord_qk_args& g, bool bwd) {
   QkPlan p{};
+  // 16 bytes a load where both halves of the turned and of the other elements are whole
+  // chunks of them (adjacent pairs take 16 bytes in two neighbouring loads); the forward of
+  // wider rows keeps to 8, whose smaller state leaves more waves (32768 x 40 heads of 128:
+  // forward 140 us by 16 bytes, 122 by 8, backward 200 and 222; 16384 x 9 heads of 64: 8.4
+  // and 10.8, 12.9 and 14.1)
+  p.v = g.dtype != CONCORD_F32 && !g.adjacent && g.R % 16 == 0 && g.D % 16 == 0 && (bwd || g.D <= 64) ? 8 : 4;
   p.lanes = 1;
-  while (p.lanes * 8 < D) p.lanes *= 2;
+  while (p.lanes * 2 * p.v < g.D) p.lanes *= 2;
   const int64_t groups = 256 / p.lanes;
-  // as many heads a slice as leave 256 blocks twice over: the angles are formed once a slice
-  p.heads = 16;
-  while (p.heads > 1 && cdiv(T, groups) * (cdiv(H, p.heads) + cdiv(HK, p.heads)) < 512) p.heads /= 2;
-  p.parts[0] = (int)cdiv(H, p.heads), p.parts[1] = (int)cdiv(HK, p.heads);
-  const int64_t most = std::max<int64_t>(1, (bwd ? 1024 : 4096) / (p.parts[0] + p.parts[1]));
-  p.blocks = (unsigned)std::min<int64_t>(cdiv(T, groups), most);
+  // as many heads a slice as leave 512 blocks: the angles are formed once a slice
+  for (int most = 16; most >= 1; most /= 2) {
+    const int H[2] = {g.H, g.HK};
+    for (int i = 0; i < 2; ++i) {
+      p.parts[i] = (int)cdiv(H[i], most);
+      p.heads[i] = p.parts[i] ? (int)cdiv(H[i], p.parts[i]) : 1;
+    }
+    if (cdiv(g.T, groups) * (p.parts[0] + p.parts[1]) >= 512) break;
+  }
+  // Many tokens: a little under two blocks a CU in all, a slice's by its share of the
+  // heads, that go on from token to token (forward of 32768 x 40 heads of 128: 122 us, 137
+  // with four a CU, 134 with a block for each group's token).  Few: no block takes two.
+  const int64_t total = cdiv(g.T, groups), all = g.H + g.HK;
+  const bool few = total * (p.parts[0] + p.parts[1]) <= 2048;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t want = few ? total : std::max<int64_t>(1, 480 * p.heads[i] / all);
+    // (an eighth over its share rather than a round of its own for the last few)
+    const int64_t rounds = cdiv(std::max<int64_t>(1, total - want / 8), want);
+    p.blocks[i] = (uint32_t)cdiv(total, rounds);
+  }
   return p;
 }
 
-template <class T, int L>
-static void qk_launch(const QkArgs& a, const QkPlan& p, bool bwd, hipStream_t st) {
-  const dim3 grid(p.blocks, p.parts[0] + p.parts[1]);
-  if (bwd) {
-    if (a.adjacent) hipLaunchKernelGGL((qk_kernel<T, L, true, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((qk_kernel<T, L, false, true>), grid, dim3(256), 0, st, a);
-  } else {
-    if (a.adjacent) hipLaunchKernelGGL((qk_kernel<T, L, true, false>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((qk_kernel<T, L, false, false>), grid, dim3(256), 0, st, a);
+template <class T, int V, int L>
+static void qk_launch(const QkArgs& a, uint32_t blocks, bool bwd, hipStream_t st) {
+  const dim3 grid(blocks);
+  if constexpr (V == 4) {
+    if (a.adjacent) {
+      if (bwd) hipLaunchKernelGGL((qk_kernel<T, V, L, true, true>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((qk_kernel<T, V, L, true, false>), grid, dim3(256), 0, st, a);
+      return;
+    }
   }
+  if (bwd) hipLaunchKernelGGL((qk_kernel<T, V, L, false, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((qk_kernel<T, V, L, false, false>), grid, dim3(256), 0, st, a);
 }
 template <class T>
-static void qk_lanes(const QkArgs& a, const QkPlan& p, bool bwd, hipStream_t st) {
+static void qk_lanes(const QkArgs& a, const QkPlan& p, uint32_t blocks, bool bwd, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.v == 8) {
+      switch (p.lanes) {
+        case 1: return qk_launch<T, 8, 1>(a, blocks, bwd, st);
+        case 2: return qk_launch<T, 8, 2>(a, blocks, bwd, st);
+        case 4: return qk_launch<T, 8, 4>(a, blocks, bwd, st);
+        case 8: return qk_launch<T, 8, 8>(a, blocks, bwd, st);
+        default: return qk_launch<T, 8, 16>(a, blocks, bwd, st);
+      }
+    }
+  }
   switch (p.lanes) {
-    case 1: return qk_launch<T, 1>(a, p, bwd, st);
-    case 2: return qk_launch<T, 2>(a, p, bwd, st);
-    case 4: return qk_launch<T, 4>(a, p, bwd, st);
-    case 8: return qk_launch<T, 8>(a, p, bwd, st);
-    case 16: return qk_launch<T, 16>(a, p, bwd, st);
-    default: return qk_launch<T, 32>(a, p, bwd, st);
+    case 1: return qk_launch<T, 4, 1>(a, blocks, bwd, st);
+    case 2: return qk_launch<T, 4, 2>(a, blocks, bwd, st);
+    case 4: return qk_launch<T, 4, 4>(a, blocks, bwd, st);
+    case 8: return qk_launch<T, 4, 8>(a, blocks, bwd, st);
+    case 16: return qk_launch<T, 4, 16>(a, blocks, bwd, st);
+    default: return qk_launch<T, 4, 32>(a, blocks, bwd, st);
   }
 }
-static void qk_run(const QkArgs& a, const QkPlan& p, int dtype, bool bwd, hipStream_t st) {
-  if (dtype == CONCORD_F32) qk_lanes<float>(a, p, bwd, st);
-  else if (dtype == CONCORD_BF16) qk_lanes<BF16>(a, p, bwd, st);
-  else qk_lanes<_Float16>(a, p, bwd, st);
+static uint32_t qk_rows(const QkPlan& p, int i) { return p.blocks[i] * (uint32_t)p.parts[i]; }
+static void qk_run(QkArgs& a, const QkPlan& p, int dtype, bool bwd, hipStream_t st) {
+  for (int i = 0; i < 2; ++i) a.heads[i] = p.heads[i], a.blocks[i] = p.blocks[i];
+  a.k_at = qk_rows(p, 0);
+  const uint32_t blocks = a.k_at + qk_rows(p, 1);
+  if (dtype == CONCORD_F32) qk_lanes<float>(a, p, blocks, bwd, st);
+  else if (dtype == CONCORD_BF16) qk_lanes<BF16>(a, p, blocks, bwd, st);
+  else qk_lanes<_Float16>(a, p, blocks, bwd, st);
 }
 
 static bool qk_aligned(const void* p, int64_t t, int64_t h) {
@@ -340,7 +413,7 @@ static int qk_args(const concord_qk_args* args, const char* name, bool bwd, QkAr
 }
 
 static size_t qk_workspace(const concord_qk_args& g, const QkPlan& p) {
-  return (size_t)p.blocks * (p.parts[0] + p.parts[1]) * g.D * sizeof(float);
+  return ((size_t)qk_rows(p, 0) + qk_rows(p, 1)) * g.D * sizeof(float);
 }
 
 }  // namespace concord
@@ -351,15 +424,13 @@ extern "C" int concord_qk_norm_rope_fwd(const concord_qk_args* args, void* strea
   QkArgs a{};
   if (const int rc = qk_args(args, "concord_qk_norm_rope_fwd", false, a)) return rc;
   if (args->T == 0) return CONCORD_OK;
-  const QkPlan p = qk_plan(args->T, args->H, args->HK, args->D, false);
-  a.heads = p.heads, a.parts0 = p.parts[0];
-  qk_run(a, p, args->dtype, false, (hipStream_t)stream);
+  qk_run(a, qk_plan(*args, false), args->dtype, false, (hipStream_t)stream);
   return launch_status("qk_norm_rope_fwd");
 }
 
 extern "C" size_t concord_qk_norm_rope_workspace_bytes(const concord_qk_args* args) {
   if (!args || !qk_sizes_ok(*args) || args->T == 0) return 0;
-  return qk_workspace(*args, qk_plan(args->T, args->H, args->HK, args->D, true));
+  return qk_workspace(*args, qk_plan(*args, true));
 }
 
 extern "C" int concord_qk_norm_rope_bwd(const concord_qk_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -369,13 +440,12 @@ extern "C" int concord_qk_norm_rope_bwd(const concord_qk_args* args, void* works
   hipStream_t st = (hipStream_t)stream;
   int rows[2] = {};
   if (g.T > 0) {
-    const QkPlan p = qk_plan(g.T, g.H, g.HK, g.D, true);
+    const QkPlan p = qk_plan(g, true);
     if ((g.dq_weight || g.dk_weight) && (!workspace || workspace_bytes < qk_workspace(g, p))) {
       set_error("concord_qk_norm_rope_bwd: workspace of %zu bytes needed", qk_workspace(g, p));
       return CONCORD_EWORKSPACE;
     }
-    a.heads = p.heads, a.parts0 = p.parts[0];
-    for (int i = 0; i < 2; ++i) rows[i] = (int)p.blocks * p.parts[i];
+    for (int i = 0; i < 2; ++i) rows[i] = (int)qk_rows(p, i);
     a.part[0] = g.dq_weight ? (float*)workspace : nullptr;
     a.part[1] = g.dk_weight ? (float*)workspace + (int64_t)rows[0] * g.D : nullptr;
     qk_run(a, p, g.dtype, true, st);
