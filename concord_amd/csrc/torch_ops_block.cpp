@@ -3,7 +3,23 @@
 // of concord_amd.h (in C++ for the reason that torch_ops.cpp gives).
 #include "torch_ops.h"
 
+#include <cstring>
+
 namespace {
+
+// A node's settings as one saved entry: each has a name to look up and a box to
+// allocate, and a step makes and reads them all.
+const char* const kSettings = "settings";
+int64_t bits_of(double v) {
+  int64_t r;
+  std::memcpy(&r, &v, sizeof r);
+  return r;
+}
+double double_of(int64_t v) {
+  double r;
+  std::memcpy(&r, &v, sizeof r);
+  return r;
+}
 
 // ---- embedding ------------------------------------------------------------------
 const char* const kEmbedding = "embedding";
@@ -40,10 +56,8 @@ Tensor embedding_forward(const Tensor& tokens, const Tensor& weight, double scal
 struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& tokens, double scale, int64_t dtype) {
     ctx->save_for_backward({tokens});
-    ctx->saved_data["index"] = (int64_t)tokens.scalar_type();
-    ctx->saved_data["vocab"] = weight.size(0);
-    ctx->saved_data["wtype"] = (int64_t)weight.scalar_type();
-    ctx->saved_data["scale"] = scale;
+    ctx->saved_data[kSettings] = std::vector<int64_t>{(int64_t)tokens.scalar_type(), weight.size(0),
+                                                      (int64_t)weight.scalar_type(), bits_of(scale)};
     return embedding_forward(tokens, weight, scale, (at::ScalarType)dtype);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -51,14 +65,15 @@ struct EmbeddingNode : torch::autograd::Function<EmbeddingNode> {
     const Tensor& dy = grads[0];
     const c10::OptionalDeviceGuard guard(dy.device());
     const Tensor tokens = ctx->get_saved_variables()[0].contiguous();
-    const int64_t vocab = ctx->saved_data["vocab"].toInt(), width = dy.size(-1), n = dy.numel() / width;
-    came_back(tokens, (at::ScalarType)ctx->saved_data["index"].toInt(), n, dy, kEmbedding, "tokens");
+    const auto settings = ctx->saved_data[kSettings].toIntVector();
+    const int64_t vocab = settings[1], width = dy.size(-1), n = dy.numel() / width;
+    came_back(tokens, (at::ScalarType)settings[0], n, dy, kEmbedding, "tokens");
     const Rows g = rows_of(dy, n, width);
-    Tensor dw = at::empty({vocab, width}, dy.options().dtype((at::ScalarType)ctx->saved_data["wtype"].toInt()));
+    Tensor dw = at::empty({vocab, width}, dy.options().dtype((at::ScalarType)settings[2]));
     const size_t need = concord_embedding_workspace_bytes(n, vocab, width);
     const Tensor ws = bytes(need, dy);
     check(concord_embedding_bwd(ptr(tokens), is_int64(tokens), n, ptr(g.t), g.ld, dtype_of(dy), vocab, width,
-                                (float)ctx->saved_data["scale"].toDouble(), ptr(dw), width, dtype_of(dw), ptr(ws), need,
+                                (float)double_of(settings[3]), ptr(dw), width, dtype_of(dw), ptr(ws), need,
                                 stream_of(dy)),
           "embedding backward");
     return {dw, Tensor(), Tensor(), Tensor()};
@@ -165,37 +180,26 @@ struct QkNormRopeNode : torch::autograd::Function<QkNormRopeNode> {
                                int64_t rotary, bool adjacent) {
     const Tensor q_weight = value(q_weight_), k_weight = value(k_weight_), positions = value(positions_);
     ctx->save_for_backward({q, k, q_weight, k_weight, positions});
-    ctx->saved_data["base"] = base;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["rotary"] = rotary;
-    ctx->saved_data["adjacent"] = adjacent;
-    ctx->saved_data["type"] = (int64_t)q.scalar_type();
-    ctx->saved_data["q_shape"] = q.sizes().vec();
-    ctx->saved_data["k_shape"] = k.sizes().vec();
+    ctx->saved_data[kSettings] = std::vector<int64_t>{bits_of(base), bits_of(eps), rotary, adjacent};
     return qk_forward(q, k, q_weight, k_weight, positions, {base, eps, rotary, adjacent});
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     only_once(kQk);
     const auto saved = ctx->get_saved_variables();
-    const Tensor& like = grads[0].defined() ? grads[0] : grads[1];
-    const c10::OptionalDeviceGuard guard(like.device());
-    const auto q_shape = ctx->saved_data["q_shape"].toIntVector(), k_shape = ctx->saved_data["k_shape"].toIntVector();
-    const QkSettings s{ctx->saved_data["base"].toDouble(), ctx->saved_data["eps"].toDouble(),
-                       ctx->saved_data["rotary"].toInt(), ctx->saved_data["adjacent"].toBool()};
-    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    const Tensor &gq = grads[0], &gk = grads[1];   // (zeros for an output that nothing used)
+    const c10::OptionalDeviceGuard guard(gq.device());
+    const auto settings = ctx->saved_data[kSettings].toIntVector();
+    const QkSettings s{double_of(settings[0]), double_of(settings[1]), settings[2], settings[3] != 0};
     const Tensor &q = saved[0], &k = saved[1];
     const Tensor q_weight = packed(saved[2]), k_weight = packed(saved[3]);
     const Tensor positions = saved[4].defined() ? saved[4].contiguous() : Tensor();
-    TORCH_CHECK(q.sizes() == at::IntArrayRef(q_shape) && k.sizes() == at::IntArrayRef(k_shape) && q.scalar_type() == type &&
-                    q.device() == like.device(),
+    TORCH_CHECK(q.sizes() == gq.sizes() && k.sizes() == gk.sizes() && q.scalar_type() == gq.scalar_type() &&
+                    q.device() == gq.device(),
                 "qk_norm_rope: the saved q or k came back as another tensor");
     qk_check(q, k, q_weight, k_weight, positions, s);
-    // (an output that nothing used has no upstream gradient)
-    const Tensor gq = grads[0].defined() ? grads[0] : at::zeros(q_shape, like.options());
-    const Tensor gk = grads[1].defined() ? grads[1] : at::zeros(k_shape, like.options());
     const Operand oq = operand(q), ok = operand(k), og = operand(gq), oh = operand(gk);
     concord_qk_args a = qk_args(oq, ok, q_weight, k_weight, positions, s);
-    Tensor dq = at::empty(q_shape, q.options()), dk = at::empty(k_shape, k.options()), dwq, dwk, ws;
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dwq, dwk, ws;
     a.dq_out = ptr(og.t), a.dq_t = og.token, a.dq_h = og.head;
     a.dk_out = ptr(oh.t), a.dk_t = oh.token, a.dk_h = oh.head;
     a.dq = ptr(dq), a.dk = ptr(dk);
@@ -306,12 +310,12 @@ struct Gelu8Node : torch::autograd::Function<Gelu8Node> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, bool gated, bool tanh) {
     const std::vector<Tensor> kept = empty8(x, gated);
     ctx->save_for_backward({kept[0], kept[1]});
-    ctx->saved_data["gated"] = gated;
-    ctx->saved_data["tanh"] = tanh;
+    ctx->saved_data[kSettings] = (int64_t)gated | (int64_t)tanh << 1;
     return gelu8_forward(x, gated, tanh, kept);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const bool gated = ctx->saved_data["gated"].toBool();
+    const int64_t settings = ctx->saved_data[kSettings].toInt();
+    const bool gated = settings & 1, tanh = settings >> 1;
     only_once(gelu8_name(gated));
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
@@ -325,7 +329,7 @@ struct Gelu8Node : torch::autograd::Function<Gelu8Node> {
     shape.back() = width * half;
     Tensor dx = at::empty(shape, dy.options());
     check(concord_gelu8_bwd(ptr(g.t), g.ld, codes_of(codes), exponents_of(exponents), dtype_of(dy), rows, width, gated,
-                            ctx->saved_data["tanh"].toBool(), ptr(dx), width * half, stream_of(dy)),
+                            tanh, ptr(dx), width * half, stream_of(dy)),
           gated ? "geglu8 backward" : "gelu8 backward");
     return {dx, Tensor(), Tensor()};
   }
