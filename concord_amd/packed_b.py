@@ -26,6 +26,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as C
+from .act8 import pack8, unpack8
 
 MANTISSA_BIAS = 15
 INT8_MIN, INT8_MAX = -128, 127
@@ -760,9 +761,11 @@ class FusedConcordLinearPackedB(torch.autograd.Function):
                 adafactor_beta2, track_adafactor_v,
                 gf_trust_delta_sq, coh_pre, *extra):
         # extra[0] (optional): the drive, 'vhat' (the reference's) or 'muon'
-        # (docs/MUON_IMPLEMENTATION.md:56-67)
+        # (docs/MUON_IMPLEMENTATION.md:56-67); extra[1]: the bits that the input
+        # is kept in for the backward, 16 (bf16) or 8
         ctx.n_extra = len(extra)
         ctx.drive = extra[0] if extra else 'vhat'
+        ctx.input_bits = extra[1] if len(extra) > 1 else 16
         K = packed_w.shape[1]
         lead = x.shape[:-1]
         x2 = x.reshape(-1, K)
@@ -774,7 +777,10 @@ class FusedConcordLinearPackedB(torch.autograd.Function):
             bias_bf16 = bias if bias.dtype == torch.bfloat16 else bias.to(torch.bfloat16)
             bias_bf16 = bias_bf16.contiguous()
         y = _gemm_fwd(x2, packed_w, row_exp, col_exp, mantissa_bias, bias_bf16, weight_buf)
-        ctx.save_for_backward(x2)
+        if ctx.input_bits == 8 and any(ctx.needs_input_grad):
+            ctx.save_for_backward(*pack8(x2))
+        else:
+            ctx.save_for_backward(x2)
         ctx.lead = lead
         ctx.packed_w, ctx.row_exp, ctx.col_exp = packed_w, row_exp, col_exp
         ctx.lr, ctx.alpha, ctx.beta1, ctx.mantissa_bias = lr, alpha, beta1, mantissa_bias
@@ -794,7 +800,7 @@ class FusedConcordLinearPackedB(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y):
-        (x2,) = ctx.saved_tensors
+        x2 = unpack8(*ctx.saved_tensors) if ctx.input_bits == 8 else ctx.saved_tensors[0]
         N, K = ctx.packed_w.shape
         dy = grad_y.reshape(-1, N)
         if dy.dtype != torch.bfloat16:
@@ -898,6 +904,7 @@ class ConcordLinearPackedB(nn.Module):
     EXP_MIN = -8
     EXP_MAX = 7
     MAX_M = 24000
+    input_bits = 16
 
     def __init__(self, in_features, out_features, bias=True, device='cuda', alpha=0.1,
                  beta1=0.0, lr=0.01, weight_cache=False, drive='vhat'):
@@ -1012,6 +1019,16 @@ class ConcordLinearPackedB(nn.Module):
         if drive not in ('vhat', 'muon'):
             raise ValueError("drive must be 'vhat' or 'muon'")
         self.drive = drive
+
+    def set_input_bits(self, bits):
+        """How the input is kept between forward and backward: 16 (bf16, the
+        default) or 8 (act8.pack8: 33 bytes for 32 values).  The forward and the
+        input's gradient are the same; the weight gradient is formed from what the
+        8-bit form stands for, each value off by at most 2^-7 of the largest of
+        its 32."""
+        if bits not in (8, 16):
+            raise ValueError(f"input bits must be 8 or 16 (got {bits!r})")
+        self.input_bits = bits
 
     def set_optimizer_kind(self, kind, weight_decay=0.0, eps=1.0, step_cap=10.0):
         if kind not in ('sgd', 'adamw'):
@@ -1214,7 +1231,7 @@ class ConcordLinearPackedB(nn.Module):
             wbuf, rmbuf, cmbuf,
             self.v_row, self.v_col, self._sum_v_inv,
             float(self.adafactor_beta2), bool(self.track_adafactor_v),
-            float(self.gf_trust_delta_sq), self._coh_pre, self.drive)
+            float(self.gf_trust_delta_sq), self._coh_pre, self.drive, self.input_bits)
         return y.to(in_dtype)
 
     @torch.no_grad()
@@ -1533,6 +1550,11 @@ class ConcordConv2dPackedB(ConcordLinearPackedB):
         super().__init__(in_features=in_channels * kh * kw, out_features=out_channels, bias=bias,
                          device=device, alpha=alpha, beta1=beta1, lr=lr, weight_cache=weight_cache,
                          drive=drive)
+
+    def set_input_bits(self, bits):
+        if bits != 16:
+            raise ValueError("ConcordConv2dPackedB: the input of a convolution is kept in bf16 (input bits 16)")
+        super().set_input_bits(bits)
 
     def _geom(self, x):
         B, cin, H, W = x.shape

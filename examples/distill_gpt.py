@@ -9,6 +9,11 @@ attends to another document.  Student and teacher are one architecture
 its largest logits and their places, as a stored teacher's output would be.
 The Concord layers step themselves in backward; the norms and embeddings are
 on SGD.
+
+    --rotary    positions by rotation, with a norm of each head's query and key, in
+                place of the learned table of positions
+    --keep8     the feed-forward's activations and the packed linears' inputs in 8 bits
+                between forward and backward
 """
 import argparse
 import os
@@ -22,37 +27,48 @@ import concord_amd as ca  # noqa: E402
 
 
 class Block(nn.Module):
-    def __init__(self, width, heads, key_heads, device, lr):
+    def __init__(self, width, heads, key_heads, device, lr, rotary=False, keep8=False):
         super().__init__()
-        self.heads, self.key_heads, self.dim = heads, key_heads, width // heads
+        self.heads, self.key_heads, self.dim, self.keep8 = heads, key_heads, width // heads, keep8
 
         def linear(i, o):
             return ca.ConcordLinearPackedB(i, o, bias=False, device=device, lr=lr)
         self.ln1, self.ln2 = ca.LayerNorm(width, device=device), ca.LayerNorm(width, device=device)
         self.qkv = linear(width, (heads + 2 * key_heads) * self.dim)
         self.proj, self.fc, self.out = linear(width, width), linear(width, 4 * width), linear(4 * width, width)
+        self.rope = ca.QKNormRope(self.dim, device=device) if rotary else None
+        if keep8:
+            for m in (self.qkv, self.proj, self.fc, self.out):
+                m.set_input_bits(8)
 
-    def forward(self, x, starts):
+    def forward(self, x, starts, positions=None):
         h, hk = self.heads, self.key_heads
         qkv = self.qkv(self.ln1(x)).to(torch.bfloat16).view(-1, h + 2 * hk, self.dim)
-        a = ca.attention(*qkv.split([h, hk, hk], dim=1), starts=starts)
+        q, k, v = qkv.split([h, hk, hk], dim=1)
+        if self.rope is not None:
+            q, k = self.rope(q, k, positions)
+        a = ca.attention(q, k, v, starts=starts)
         x = x + self.proj(a.reshape(x.shape))
-        return x + self.out(nn.functional.gelu(self.fc(self.ln2(x))))
+        f = self.fc(self.ln2(x))
+        return x + self.out(ca.gelu8(f) if self.keep8 else nn.functional.gelu(f))
 
 
 class GPT(nn.Module):
-    def __init__(self, vocab=65, width=384, heads=6, key_heads=3, layers=4, context=256, device="cuda", lr=1e-3):
+    def __init__(self, vocab=65, width=384, heads=6, key_heads=3, layers=4, context=256, device="cuda", lr=1e-3,
+                 rotary=False, keep8=False):
         super().__init__()
-        self.wte = nn.Embedding(vocab, width, device=device)
-        self.wpe = nn.Embedding(context, width, device=device)
-        self.blocks = nn.ModuleList(Block(width, heads, key_heads, device, lr) for _ in range(layers))
+        self.wte = ca.Embedding(vocab, width, device=device)
+        self.wpe = None if rotary else ca.Embedding(context, width, device=device)
+        self.blocks = nn.ModuleList(Block(width, heads, key_heads, device, lr, rotary, keep8) for _ in range(layers))
         self.ln_f = ca.LayerNorm(width, device=device)
         self.head = ca.ConcordLinearPackedB(width, vocab, bias=False, device=device, lr=lr)
 
     def forward(self, tokens, positions, starts):
-        x = self.wte(tokens) + self.wpe(positions)
+        x = self.wte(tokens)
+        if self.wpe is not None:
+            x = x + self.wpe(positions)
         for b in self.blocks:
-            x = b(x, starts)
+            x = b(x, starts, positions)
         return self.head(self.ln_f(x))
 
     def concord_layers(self):
@@ -75,11 +91,12 @@ def documents(tokens, vocab, context, gen, device):
     return letters.to(device), positions.to(device), starts.to(device)
 
 
-def train(steps, tokens=8192, top=16, temperature=2.0, device="cuda", seed=0, log=None):
+def train(steps, tokens=8192, top=16, temperature=2.0, device="cuda", seed=0, log=None, rotary=False, keep8=False):
     """Losses (mean over tokens) of `steps` distillation steps."""
     torch.manual_seed(seed)
     vocab, context = 65, 256
-    teacher, student = GPT(vocab, context=context, device=device), GPT(vocab, context=context, device=device)
+    teacher = GPT(vocab, context=context, device=device, rotary=rotary)
+    student = GPT(vocab, context=context, device=device, rotary=rotary, keep8=keep8)
     with torch.no_grad():   # a teacher with opinions: logits a few units apart
         teacher.head.load_weights(torch.randn(vocab, 384, device=device) * 0.15)
     layers = student.concord_layers()
@@ -109,8 +126,11 @@ def main():
     ap.add_argument("--tokens", type=int, default=8192)
     ap.add_argument("--top", type=int, default=16)
     ap.add_argument("--temperature", type=float, default=2.0)
+    ap.add_argument("--rotary", action="store_true")
+    ap.add_argument("--keep8", action="store_true")
     args = ap.parse_args()
-    losses = train(args.steps, args.tokens, args.top, args.temperature, log=max(1, args.steps // 20))
+    losses = train(args.steps, args.tokens, args.top, args.temperature, log=max(1, args.steps // 20), rotary=args.rotary,
+                   keep8=args.keep8)
     print(f"loss {losses[0]:.4f} -> {sum(losses[-10:]) / len(losses[-10:]):.4f}")
 
 

@@ -560,3 +560,253 @@ def test_gelu8_gradient_against_differences():
         slope = (value(1e-4) - value(-1e-4)) / 2e-4
         size = float((dx.double() * direction).abs().sum())
         assert abs(float((dx.double() * direction).sum()) - slope) <= (64 * U + 10 * 1e-8) * size
+
+
+# ---- used together -----------------------------------------------------------------
+def _chain(n, gen, width=128, heads=4, kv=2, vocab=50):
+    """(leaves, step): tokens to a feed-forward's result and all gradients"""
+    import concord_amd as ca
+    dim = width // heads
+    table = torch.randn(vocab, width, generator=gen, device=DEV)
+    wqkv = torch.randn(width, (heads + 2 * kv) * dim, generator=gen, device=DEV) / width ** 0.5
+    wfc = torch.randn(width, 4 * width, generator=gen, device=DEV) / width ** 0.5
+    wq, wk = torch.ones(dim, device=DEV), torch.ones(dim, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (table, wqkv, wq, wk, wfc)]
+    tokens = torch.randint(-1, vocab, (n,), generator=gen, device=DEV)
+    positions = torch.arange(n, device=DEV)
+    up = torch.randn(n, 2 * width, generator=gen, device=DEV).to(BF16)
+
+    def step():
+        x = ca.embedding(tokens, table, scale=2.0)
+        qkv = torch.matmul(ca.layer_norm(x), wqkv).to(BF16).view(n, heads + 2 * kv, dim)
+        q, k, v = qkv.split([heads, kv, kv], dim=1)
+        q, k = ca.qk_norm_rope(q, k, wq, wk, positions=positions)
+        x = x + ca.attention(q, k, v).reshape(n, width)
+        y = ca.geglu8(ca.gelu8(torch.matmul(ca.layer_norm(x), wfc).to(BF16)))
+        return [y] + list(torch.autograd.grad(y, leaves, up))
+    return leaves, tokens, up, step
+
+
+def test_chain_against_plain_operators():
+    """Embedding, norms and rotation, attention and both activations in one graph, against the same
+    with torch's operators in fp32 and every bf16 rounding of activations at its place.  Roundings
+    that fall otherwise (2^-8 of a value, at 5 places forward and as many backward) and the 8-bit
+    steps (2^-7 of a block's largest at 2 places, both sides' the same but where a value differs
+    already) leave 2^-3.5 of a gradient's norm at most, 2^-5 of the result's."""
+    import concord_amd as ca
+    leaves, tokens, up, step = _chain(150, _gen("chain"))
+    got = [t.detach().double() for t in step()]
+    table, wqkv, wq, wk, wfc = leaves
+
+    class Kept(torch.autograd.Function):   # f(x), its gradient at the 8-bit form of x
+        @staticmethod
+        def forward(ctx, x, f):
+            ctx.f, ctx.z = f, x
+            return f(x)
+
+        @staticmethod
+        def backward(ctx, dy):
+            halves = ctx.z.chunk(2, -1) if ctx.f is gated else (ctx.z,)
+            z = torch.cat([_kept(h)[2] for h in halves], -1).to(ctx.z.dtype).requires_grad_(True)
+            with torch.enable_grad():
+                y = ctx.f(z)
+            return torch.autograd.grad(y, z, dy)[0], None
+
+    def gelu(x):
+        return torch.nn.functional.gelu(x.float()).to(x.dtype)
+
+    def gated(x):
+        a, b = x.chunk(2, -1)
+        return (a.float() * torch.nn.functional.gelu(b.float())).to(x.dtype)
+
+    def norm_rope(x, w):
+        h = x.float() * (x.float().square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+        half = x.shape[-1] // 2
+        angle = torch.arange(x.shape[0], device=DEV)[:, None, None] * 10000.0 ** (
+            -torch.arange(half, device=DEV, dtype=torch.float64) / half)
+        c, s = angle.cos().float(), angle.sin().float()
+        return torch.cat((h[..., :half] * c - h[..., half:] * s, h[..., :half] * s + h[..., half:] * c), -1).to(BF16)
+    n, width, heads, kv, dim = 150, 128, 4, 2, 32
+    x = table[tokens.clamp_min(0)] * (tokens >= 0)[:, None] * 2.0
+    qkv = torch.matmul(torch.nn.functional.layer_norm(x, (width,)), wqkv).to(BF16).view(n, heads + 2 * kv, dim)
+    q, k, v = qkv.split([heads, kv, kv], dim=1)
+    q, k = norm_rope(q, wq), norm_rope(k, wk)
+    qf, kf, vf = (t.float().transpose(0, 1) for t in (q, k.repeat_interleave(2, 1), v.repeat_interleave(2, 1)))
+    z = torch.matmul(qf, kf.transpose(1, 2).contiguous()) / dim ** 0.5
+    z = z.masked_fill(torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1), -math.inf)
+    x = x + torch.matmul(z.softmax(-1), vf).to(BF16).transpose(0, 1).reshape(n, width)
+    y = Kept.apply(Kept.apply(torch.matmul(torch.nn.functional.layer_norm(x, (width,)), wfc).to(BF16), gelu), gated)
+    want = [y.detach().double()] + [t.double() for t in torch.autograd.grad(y, leaves, up)]
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert float((a - b).norm()) <= 2.0 ** (-5 if i == 0 else -3.5) * float(b.norm()), i
+
+
+def test_chain_in_a_captured_step():
+    """One HIP graph of the step, replayed with new inputs and with eager work between the replays:
+    the eager results, bit for bit."""
+    gen = _gen("graph")
+    leaves, tokens, up, step = _chain(700, gen)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [t.detach() for t in step()]
+    for _ in range(4):
+        with torch.no_grad():
+            tokens.copy_(torch.randint(-1, 50, tokens.shape, generator=gen, device=DEV))
+            leaves[0].copy_(torch.randn(leaves[0].shape, generator=gen, device=DEV))
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("n,vocab", [(300, 70000), (6000, 65), (70000, 300)])
+def test_embedding_gradient_in_a_graph(n, vocab):
+    """Each of the sort's forms, captured and replayed with other tokens."""
+    import concord_amd as ca
+    gen = _gen("embedding graph", n)
+    tokens = torch.randint(0, vocab, (n,), generator=gen, device=DEV)
+    w = torch.randn(vocab, 40, generator=gen, device=DEV, requires_grad=True)
+    dy = torch.randn(n, 40, generator=gen, device=DEV)
+
+    def step():
+        return torch.autograd.grad(ca.embedding(tokens, w), (w,), dy)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(3):
+        tokens.copy_(torch.randint(-3, vocab + 3, (n,), generator=gen, device=DEV))
+        graph.replay()
+        got = held.clone()
+        assert torch.equal(got, step())
+
+
+def test_streams_do_not_share_anything():
+    """The same calls on two streams at once give what each gives alone."""
+    import concord_amd as ca
+    gen = _gen("streams")
+    jobs = []
+    for n, vocab in ((9000, 300), (9000, 300)):
+        tokens = torch.randint(0, vocab, (n,), generator=gen, device=DEV)
+        w = torch.randn(vocab, 256, generator=gen, device=DEV, requires_grad=True)
+        q = torch.randn(n, 4, 64, generator=gen, device=DEV).to(BF16).requires_grad_(True)
+        x = torch.randn(n, 256, generator=gen, device=DEV).to(BF16).requires_grad_(True)
+        qw = torch.ones(64, device=DEV, requires_grad=True)
+        jobs.append((tokens, w, q, qw, x))
+
+    def run(tokens, w, q, qw, x):
+        y = ca.embedding(tokens, w)
+        a, b = ca.qk_norm_rope(q, q, qw, qw)
+        z = ca.gelu8(x)
+        return torch.autograd.grad([y, a, b, z], [w, q, qw, x], [torch.ones_like(t) for t in (y, a, b, z)])
+    alone = [run(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in jobs], []
+    for _ in range(3):
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(run(*j))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, alone[i % 2]))
+
+
+def test_block_operators_are_differentiable_once():
+    import concord_amd as ca
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    q = torch.randn(4, 1, 64, device=DEV, requires_grad=True)
+    idx = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for y, leaf in ((ca.embedding(idx, x), x), (ca.qk_norm_rope(q, q)[0], q), (ca.gelu8(x), x), (ca.geglu8(x), x)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), leaf, create_graph=True)
+
+
+def test_block_operators_see_a_change_of_a_saved_tensor():
+    import concord_amd as ca
+    q = torch.randn(4, 2, 64, device=DEV, requires_grad=True)
+    tokens = torch.zeros(4, dtype=torch.int64, device=DEV)
+    w = torch.randn(5, 64, device=DEV, requires_grad=True)
+    y, (z, _) = ca.embedding(tokens, w), ca.qk_norm_rope(q * 1.0, q * 1.0, positions=tokens)
+    tokens.add_(1)
+    for t in (y, z):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            t.sum().backward()
+
+
+def test_modules():
+    import concord_amd as ca
+    e = ca.Embedding(11, 48, scale=3.0, device=DEV, out_dtype=BF16)
+    t = torch.tensor([[1, 10], [-1, 0]], device=DEV, dtype=torch.int32)
+    assert e(t).dtype == BF16 and torch.equal(e(t), ca.embedding(t, e.weight, 3.0, BF16)) and e(t).requires_grad
+    m = ca.QKNormRope(64, base=500.0, rotary_dim=32, interleaved=True, eps=1e-5, device=DEV)
+    q = torch.randn(2, 7, 3, 64, device=DEV)
+    got, want = m(q, q[:, :, :1]), ca.qk_norm_rope(q, q[:, :, :1], m.q_weight, m.k_weight, None, 500.0, 32, True, 1e-5)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert [p.shape for p in m.parameters()] == [(64,), (64,)]
+
+
+# ---- the packed linear's input in 8 bits ------------------------------------------------
+@pytest.mark.parametrize("N,K,M", [(64, 96, 70), (136, 333, 50), (256, 512, 300)])
+def test_linear_input_in_8_bits(N, K, M):
+    """Forward and the input's gradient are bit for bit those of the bf16 input; the weight gradient,
+    v-hat and update are bit for bit those of a layer whose input is the 8-bit form's values."""
+    import concord_amd as ca
+    from concord_amd import packed_b as pb
+    g = _gen("linear 8", N, K)
+    W = torch.randn(N, K, generator=g, device=DEV) * 0.05
+    x = torch.randn(M, K, generator=g, device=DEV).to(BF16)
+    kept = ca.unpack8(*ca.pack8(x))
+    dy = (torch.randn(M, N, generator=g, device=DEV) * 1e-2).to(BF16)
+
+    def run(inp, bits):
+        pb._get_step_counter(torch.device(DEV)).zero_()
+        layer = ca.ConcordLinearPackedB(K, N, bias=True, device=DEV, lr=5e-3)
+        layer.load_weights(W)
+        layer.set_input_bits(bits)
+        leaf = inp.clone().requires_grad_(True)
+        y = layer(leaf)
+        y.backward(dy)
+        return y.detach(), leaf.grad, layer
+    y16, dx16, _ = run(x, 16)
+    y8, dx8, layer8 = run(x, 8)
+    _, _, want = run(kept, 16)
+    assert torch.equal(y8, y16) and torch.equal(dx8, dx16)
+    for n, t in want.state_dict().items():
+        if isinstance(t, torch.Tensor):
+            assert torch.equal(layer8.state_dict()[n], t), n
+    assert torch.equal(layer8.bias.grad, want.bias.grad)
+    with torch.no_grad():
+        assert torch.equal(layer8(x), layer8(x))
+
+
+def test_linear_keeps_33_bytes_for_32_values():
+    import concord_amd as ca
+    layer = ca.ConcordLinearPackedB(1024, 64, bias=False, device=DEV)
+    layer.set_input_bits(8)
+    saved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t) or t, lambda t: t):
+        layer(torch.randn(8, 1024, device=DEV, requires_grad=True))
+    assert sorted(t.numel() * t.element_size() for t in saved) == [8 * 32, 8 * 1024]
+
+
+@pytest.mark.parametrize("rotary,keep8", [(True, False), (False, True), (True, True)])
+def test_example_runs(rotary, keep8):
+    from examples import distill_gpt as ex
+    m = ex.GPT(layers=2, device=DEV, rotary=rotary, keep8=keep8)
+    batch = ex.documents(700, 65, 256, torch.Generator().manual_seed(1), DEV)
+    m(*batch).float().square().mean().backward()
+    layers = {id(p) for c in m.concord_layers() for p in c.parameters()}
+    own = [p for p in m.parameters() if id(p) not in layers]
+    assert len(own) > 5 and all(p.grad is not None and torch.isfinite(p.grad).all() and p.grad.any() for p in own)
+    assert all(math.isfinite(v) for v in ex.train(2, tokens=600, device=DEV, rotary=rotary, keep8=keep8))
