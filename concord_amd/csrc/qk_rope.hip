@@ -437,6 +437,7 @@ extern "C" int concord_qk_norm_rope_bwd(const concord_qk_args* args, void* works
   QkArgs a{};
   if (const int rc = qk_args(args, "concord_qk_norm_rope_bwd", true, a)) return rc;
   const concord_qk_args& g = *args;
+  if (g.T == 0 && !g.dq_weight && !g.dk_weight) return CONCORD_OK;
   hipStream_t st = (hipStream_t)stream;
   int rows[2] = {};
   if (g.T > 0) {
