@@ -14,6 +14,12 @@
 // that it takes.  Angles are formed in 64 bits (a far position times a frequency
 // loses its fraction in 32) and reduced to an eighth of a turn before the sine and
 // cosine, which are 32-bit polynomials.
+//
+// Kernel times, 32768 tokens of 40 heads of 128, bf16: forward 120 to 125 us (5.5 TB/s),
+// backward 200 to 228 from run to run (5.0 to 4.4), where a 1 GiB copy moves 5.1 TB/s;
+// 64 tokens 4.3 us, a chain of a position's load, an exponential and the row.  The stores go
+// past the caches: 16384 x 9 heads of 64 10.5 -> 8.3 and 14.0 -> 11.7 us, the largest
+// forward 133 -> 124, its backward 215 -> 228.
 #include "elem.h"
 
 namespace concord {
