@@ -4,7 +4,7 @@ csrc/act8.hip.
 The 8-bit form: 32 adjacent values of the last dimension share a step, the smallest
 power of two of which the largest value is at most 127; each value is stored as the
 nearest whole number of steps (ties to even).  A value is off by at most half a step,
-2^-7 of the largest of its 32.  A block that holds an infinity or NaN reads back as
+1/127 of the largest of its 32.  A block that holds an infinity or NaN reads back as
 NaN, all 32 values of it.
 """
 import torch

@@ -5,8 +5,8 @@
 //   code = x 2^-e rounded half to even, -127 .. 127;   exponent byte = e + 127 (1 .. 249)
 //   value = code 2^e, limited to the type's largest finite number
 // Scaling by a power of two is exact, so the codes have one definition whatever
-// computes them, each value is off by at most half a step (2^-7 of the block's
-// largest), and one significant byte fits bf16 and fp16 without a further rounding.
+// computes them, each value is off by at most half a step (1/127 of the
+// block's largest), and one significant byte fits bf16 and fp16 without a further rounding.
 // A block that holds an infinity or NaN has exponent byte 255 and codes 0: all of it
 // reads back as NaN.
 #pragma once

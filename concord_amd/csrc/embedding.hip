@@ -442,17 +442,23 @@ static bool emb_chunked(const void* p, int64_t ld, size_t bytes, size_t es) {
   return ((uintptr_t)p & (bytes - 1)) == 0 && (ld * es) % bytes == 0;
 }
 
+// columns of a lane and step: 16 bytes of the narrower type, or one where some row begins
+// or ends off them
 template <class TA, class TB>
 struct EmbVec {
-  // columns of a lane and step: 16 bytes of the narrower type
   static constexpr int V = sizeof(TA) == 2 || sizeof(TB) == 2 ? 8 : 4;
 };
+static int emb_columns(const EmbArgs& a, int src_type, int dst_type) {
+  const int v = emb_size(src_type) == 2 || emb_size(dst_type) == 2 ? 8 : 4;
+  return a.C % v == 0 && emb_chunked(a.src, a.lds, 16, emb_size(src_type)) &&
+                 emb_chunked(a.dst, a.ldd, 16, emb_size(dst_type)) ? v : 1;
+}
 
 template <class TW, class TO>
-static void emb_fwd(const EmbArgs& a, hipStream_t st) {
+static void emb_fwd(const EmbArgs& a, int columns, hipStream_t st) {
   constexpr int V = EmbVec<TW, TO>::V;
-  const bool vec = a.C % V == 0 && emb_chunked(a.src, a.lds, 16, sizeof(TW)) && emb_chunked(a.dst, a.ldd, 16, sizeof(TO));
-  const int64_t steps = vec ? a.C / V : a.C;
+  const bool vec = columns == V;
+  const int64_t steps = a.C / columns;
   int lg = 0;
   while (lg < 8 && (1 << lg) < steps) ++lg;
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.n, 256 >> lg), 1 << 20));
@@ -462,7 +468,6 @@ static void emb_fwd(const EmbArgs& a, hipStream_t st) {
 
 template <class TG, class TW, int V>
 static void emb_sums(EmbArgs& a, hipStream_t st) {
-  a.slabs = cdiv(a.C, 64 * V);
   a.fill_at = cdiv(a.pieces * a.slabs, 4);
   hipLaunchKernelGGL((emb_sum_kernel<TG, TW, V>), dim3((unsigned)(a.fill_at + cdiv(a.V, 4 * kFillRows))), dim3(256), 0, st,
                      a);
@@ -470,12 +475,10 @@ static void emb_sums(EmbArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((emb_join_kernel<TW, V>), dim3((unsigned)(a.pieces * a.slabs)), dim3(512), 0, st, a);
 }
 template <class TG, class TW>
-static void emb_bwd(EmbArgs& a, hipStream_t st) {
+static void emb_bwd(EmbArgs& a, int columns, hipStream_t st) {
   constexpr int V = EmbVec<TG, TW>::V;
-  if (a.C % V == 0 && emb_chunked(a.src, a.lds, 16, sizeof(TG)) && emb_chunked(a.dst, a.ldd, 16, sizeof(TW)))
-    emb_sums<TG, TW, V>(a, st);
-  else
-    emb_sums<TG, TW, 1>(a, st);
+  if (columns == V) emb_sums<TG, TW, V>(a, st);
+  else emb_sums<TG, TW, 1>(a, st);
 }
 
 // f<A, B>() for two of the three types
@@ -511,7 +514,8 @@ extern "C" int concord_embedding_fwd(const void* tokens, int index64, int64_t n,
   EmbArgs a{};
   a.tokens = tokens, a.idx64 = index64, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
   a.src = table, a.lds = ld_t, a.dst = out, a.ldd = ld_o;
-  emb_types(wdtype, dtype, [&](auto w, auto o) { emb_fwd<decltype(w), decltype(o)>(a, (hipStream_t)stream); });
+  const int columns = emb_columns(a, wdtype, dtype);
+  emb_types(wdtype, dtype, [&](auto w, auto o) { emb_fwd<decltype(w), decltype(o)>(a, columns, (hipStream_t)stream); });
   return launch_status("embedding_fwd");
 }
 
@@ -534,15 +538,15 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
     return CONCORD_EWORKSPACE;
   }
   CONCORD_CHECK(((uintptr_t)workspace & 15) == 0, "concord_embedding_bwd: the workspace is not on 16 bytes");
-  const int piece = emb_piece(n);
-  // (64 columns a slab where no vector fits)
-  CONCORD_CHECK(grid_fits(cdiv(n, piece) * cdiv(C, 64) + cdiv(V, 4 * kFillRows), 512),
-                "concord_embedding_bwd: too many tokens or rows");
   hipStream_t st = (hipStream_t)stream;
   EmbArgs a{};
   a.tokens = tokens, a.idx64 = index64, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
   a.src = dy, a.lds = ld_dy, a.dst = dtable, a.ldd = ld_dt;
-  a.piece = piece, a.pieces = cdiv(n, piece);
+  a.piece = emb_piece(n), a.pieces = cdiv(n, a.piece);
+  const int columns = emb_columns(a, dtype, wdtype);
+  a.slabs = cdiv(C, 64 * columns);
+  CONCORD_CHECK(grid_fits(cdiv(a.pieces * a.slabs, 4) + cdiv(V, 4 * kFillRows), 256) && grid_fits(a.pieces * a.slabs, 512),
+                "concord_embedding_bwd: too many tokens or rows");
   uint32_t *keys[2] = {}, *pos[2] = {};
   int at = 0;
   if (n > 0) {
@@ -579,6 +583,6 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
     }
   }
   a.keys = keys[at], a.pos = pos[at];
-  emb_types(dtype, wdtype, [&](auto g, auto t) { emb_bwd<decltype(g), decltype(t)>(a, st); });
+  emb_types(dtype, wdtype, [&](auto g, auto t) { emb_bwd<decltype(g), decltype(t)>(a, columns, st); });
   return launch_status("embedding_bwd");
 }

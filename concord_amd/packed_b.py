@@ -1024,8 +1024,8 @@ class ConcordLinearPackedB(nn.Module):
         """How the input is kept between forward and backward: 16 (bf16, the
         default) or 8 (act8.pack8: 33 bytes for 32 values).  The forward and the
         input's gradient are the same; the weight gradient is formed from what the
-        8-bit form stands for, each value off by at most 2^-7 of the largest of
-        its 32."""
+        8-bit form stands for, each value off by at most 1/127 of the largest
+        of its 32."""
         if bits not in (8, 16):
             raise ValueError(f"input bits must be 8 or 16 (got {bits!r})")
         self.input_bits = bits
