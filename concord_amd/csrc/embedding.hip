@@ -55,11 +55,27 @@ CONCORD_DEV uint32_t token_key(const void* tokens, int idx64, int64_t i, uint32_
   return (uint64_t)t < V ? (uint32_t)t : V;
 }
 
+// VEC columns of a row as they lie in memory: on their size, or (AL false) where an element
+// may begin, which this GPU takes for wide accesses too.  Rows whose length VEC does not
+// divide end in a step that is moved back to end with them: it gives the columns that it
+// shares with the one before the same values again.
+template <class T, int VEC, bool AL>
+struct alignas(AL ? sizeof(T) * VEC : sizeof(T)) Cols {
+  T v[VEC];
+};
+template <int VEC>
+CONCORD_DEV int64_t last_step(int64_t c, int64_t C) { return min(c, C - VEC); }
+template <bool AL, class V>
+CONCORD_DEV void store_cols(void* p, const V& v) {
+  if constexpr (AL) store_stream((V*)p, v);
+  else *(V*)p = v;
+}
+
 // ---- forward ------------------------------------------------------------------
 // 2^lg threads a row, VEC columns a thread and step.  (Four rows at once, their loads
 // out together: no change.  The stores go past the caches: 16384 x 384 in fp32 9.1 -> 7.4
 // us, 32768 x 4096 in bf16 72 -> 75.)
-template <class TW, class TO, int VEC>
+template <class TW, class TO, int VEC, bool AL>
 __global__ __launch_bounds__(256) void emb_fwd_kernel(EmbArgs a, int lg) {
   const int64_t step = (int64_t)gridDim.x << (8 - lg);
   for (int64_t row = ((int64_t)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg); row < a.n; row += step) {
@@ -68,12 +84,13 @@ __global__ __launch_bounds__(256) void emb_fwd_kernel(EmbArgs a, int lg) {
     const TW* src = (const TW*)a.src + (int64_t)(there ? t : 0) * a.lds;
     TO* dst = (TO*)a.dst + row * a.ldd;
     for (int64_t c = (int64_t)(threadIdx.x & ((1 << lg) - 1)) * VEC; c < a.C; c += (int64_t)VEC << lg) {
-      Chunk<TW, VEC> v = {};
-      if (there) v = *(const Chunk<TW, VEC>*)(src + c);
-      Chunk<TO, VEC> r;
+      const int64_t at = last_step<VEC>(c, a.C);
+      Cols<TW, VEC, AL> v = {};
+      if (there) v = *(const Cols<TW, VEC, AL>*)(src + at);
+      Cols<TO, VEC, AL> r;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<TO>(to_f32(v.v[e]) * a.scale);
-      store_stream((Chunk<TO, VEC>*)(dst + c), r);
+      store_cols<AL>(dst + at, r);
     }
   }
 }
@@ -257,18 +274,18 @@ __global__ __launch_bounds__(512) void emb_scatter_kernel(EmbArgs a, SortPass s)
 
 // ---- sums -------------------------------------------------------------------------
 // one row of the gradient, or zeros
-template <class TW, int VEC>
+template <class TW, int VEC, bool AL>
 CONCORD_DEV void store_row(const EmbArgs& a, uint32_t v, int64_t c, const float (&s)[VEC]) {
   if (c >= a.C) return;
-  Chunk<TW, VEC> r;
+  Cols<TW, VEC, AL> r;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) r.v[e] = from_f32<TW>(s[e] * a.scale);
-  store_stream((Chunk<TW, VEC>*)((TW*)a.dst + (int64_t)v * a.ldd + c), r);
+  store_cols<AL>((TW*)a.dst + (int64_t)v * a.ldd + last_step<VEC>(c, a.C), r);
 }
 template <int VEC>
 CONCORD_DEV void store_part(const EmbArgs& a, int64_t piece, int which, int64_t c, const float (&s)[VEC]) {
   if (c >= a.C) return;
-  float* p = a.part + (piece * 2 + which) * a.C + c;
+  float* p = a.part + (piece * 2 + which) * a.C + last_step<VEC>(c, a.C);
 #pragma unroll
   for (int e = 0; e < VEC; ++e) p[e] = s[e];
 }
@@ -289,7 +306,7 @@ CONCORD_DEV int64_t first_not_less(const uint32_t* keys, int64_t lo, int64_t hi,
 
 constexpr int kFillRows = 8;   // rows of the table that a wave looks at for zeros
 
-template <class TG, class TW, int VEC>
+template <class TG, class TW, int VEC, bool AL>
 __global__ __launch_bounds__(256) void emb_sum_kernel(EmbArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int64_t)blockIdx.x >= a.fill_at) {
@@ -302,7 +319,7 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(EmbArgs a) {
     for (int64_t v = v0; v < min(v0 + kFillRows, (int64_t)a.V); ++v) {
       const int64_t at = hi > lo ? first_not_less(a.keys, lo, hi, (uint32_t)v) : hi;
       if (at < hi && a.keys[at] == (uint32_t)v) continue;
-      for (int64_t c = (int64_t)lane * VEC; c < a.C; c += 64 * VEC) store_row<TW, VEC>(a, (uint32_t)v, c, zero);
+      for (int64_t c = (int64_t)lane * VEC; c < a.C; c += 64 * VEC) store_row<TW, VEC, AL>(a, (uint32_t)v, c, zero);
     }
     return;
   }
@@ -317,25 +334,25 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(EmbArgs a) {
   const int m = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < p1 - p0 && key < a.V));
   if (m == 0) return;   // (tokens outside the table stand last)
   const int64_t c = ((item - piece * a.slabs) * 64 + lane) * VEC;
-  const TG* src = (const TG*)a.src + (c < a.C ? c : 0);
+  const TG* src = (const TG*)a.src + (c < a.C ? last_step<VEC>(c, a.C) : 0);
   constexpr int U = 8;
-  Chunk<TG, VEC> r[2][U];
-  auto load = [&](Chunk<TG, VEC> (&t)[U], int i) {
+  Cols<TG, VEC, AL> r[2][U];
+  auto load = [&](Cols<TG, VEC, AL> (&t)[U], int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      t[u] = *(const Chunk<TG, VEC>*)(src + (int64_t)(uint32_t)__builtin_amdgcn_readlane(pos, min(i + u, m - 1)) * a.lds);
+      t[u] = *(const Cols<TG, VEC, AL>*)(src + (int64_t)(uint32_t)__builtin_amdgcn_readlane(pos, min(i + u, m - 1)) * a.lds);
   };
   uint32_t cur = __builtin_amdgcn_readlane(key, 0);
   bool head = earlier == cur;
   float s[VEC] = {};
-  auto add = [&](const Chunk<TG, VEC> (&t)[U], int i) {
+  auto add = [&](const Cols<TG, VEC, AL> (&t)[U], int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= m) break;
       const uint32_t k = __builtin_amdgcn_readlane(key, i + u);
       if (k != cur) {
         if (head) store_part<VEC>(a, piece, 0, c, s);
-        else store_row<TW, VEC>(a, cur, c, s);
+        else store_row<TW, VEC, AL>(a, cur, c, s);
         head = false;
         cur = k;
 #pragma unroll
@@ -355,12 +372,12 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(EmbArgs a) {
   }
   if (head) store_part<VEC>(a, piece, 0, c, s);
   else if (later == cur) store_part<VEC>(a, piece, 1, c, s);
-  else store_row<TW, VEC>(a, cur, c, s);
+  else store_row<TW, VEC, AL>(a, cur, c, s);
 }
 
 // Tokens that cross pieces: the block of the piece that such a run begins in
 // adds its sums, each wave every eighth of them, then the waves' sums in order.
-template <class TW, int VEC>
+template <class TW, int VEC, bool AL>
 __global__ __launch_bounds__(512) void emb_join_kernel(EmbArgs a) {
   constexpr int W = 8, U = 4;
   __shared__ float part[W][64 * VEC];
@@ -374,7 +391,7 @@ __global__ __launch_bounds__(512) void emb_join_kernel(EmbArgs a) {
   const int64_t c = ((blockIdx.x - piece * a.slabs) * 64 + lane) * VEC;
   float s[VEC] = {};
   if (c < a.C) {
-    const float* h = a.part + c;
+    const float* h = a.part + last_step<VEC>(c, a.C);
     const int64_t row = 2 * a.C;
     int64_t q = piece + 1 + wave;
     for (; q + (U - 1) * W <= last; q += U * W) {
@@ -396,14 +413,14 @@ __global__ __launch_bounds__(512) void emb_join_kernel(EmbArgs a) {
   for (int e = 0; e < VEC; ++e) part[wave][lane * VEC + e] = s[e];
   __syncthreads();
   if (wave == 0 && c < a.C) {
-    const float* t = a.part + (piece * 2 + 1) * a.C + c;
+    const float* t = a.part + (piece * 2 + 1) * a.C + last_step<VEC>(c, a.C);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       s[e] = t[e];
 #pragma unroll
       for (int w = 0; w < W; ++w) s[e] += part[w][lane * VEC + e];
     }
-    store_row<TW, VEC>(a, cur, c, s);
+    store_row<TW, VEC, AL>(a, cur, c, s);
   }
 }
 
@@ -442,43 +459,48 @@ static bool emb_chunked(const void* p, int64_t ld, size_t bytes, size_t es) {
   return ((uintptr_t)p & (bytes - 1)) == 0 && (ld * es) % bytes == 0;
 }
 
-// columns of a lane and step: 16 bytes of the narrower type, or one where some row begins
-// or ends off them
+// columns of a lane and step: 16 bytes of the narrower type, or one of a row shorter than that
 template <class TA, class TB>
 struct EmbVec {
   static constexpr int V = sizeof(TA) == 2 || sizeof(TB) == 2 ? 8 : 4;
 };
-static int emb_columns(const EmbArgs& a, int src_type, int dst_type) {
+struct EmbColumns {
+  int n;
+  bool aligned;
+};
+static EmbColumns emb_columns(const EmbArgs& a, int src_type, int dst_type) {
   const int v = emb_size(src_type) == 2 || emb_size(dst_type) == 2 ? 8 : 4;
-  return a.C % v == 0 && emb_chunked(a.src, a.lds, 16, emb_size(src_type)) &&
-                 emb_chunked(a.dst, a.ldd, 16, emb_size(dst_type)) ? v : 1;
+  if (a.C < v) return {1, true};
+  return {v, a.C % v == 0 && emb_chunked(a.src, a.lds, 16, emb_size(src_type)) &&
+                 emb_chunked(a.dst, a.ldd, 16, emb_size(dst_type))};
 }
 
 template <class TW, class TO>
-static void emb_fwd(const EmbArgs& a, int columns, hipStream_t st) {
+static void emb_fwd(const EmbArgs& a, EmbColumns columns, hipStream_t st) {
   constexpr int V = EmbVec<TW, TO>::V;
-  const bool vec = columns == V;
-  const int64_t steps = a.C / columns;
+  const int64_t steps = cdiv(a.C, columns.n);
   int lg = 0;
   while (lg < 8 && (1 << lg) < steps) ++lg;
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(a.n, 256 >> lg), 1 << 20));
-  if (vec) hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, V>), grid, dim3(256), 0, st, a, lg);
-  else hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, 1>), grid, dim3(256), 0, st, a, lg);
+  if (columns.n == 1) hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, 1, true>), grid, dim3(256), 0, st, a, lg);
+  else if (columns.aligned) hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, V, true>), grid, dim3(256), 0, st, a, lg);
+  else hipLaunchKernelGGL((emb_fwd_kernel<TW, TO, V, false>), grid, dim3(256), 0, st, a, lg);
 }
 
-template <class TG, class TW, int V>
+template <class TG, class TW, int V, bool AL>
 static void emb_sums(EmbArgs& a, hipStream_t st) {
   a.fill_at = cdiv(a.pieces * a.slabs, 4);
-  hipLaunchKernelGGL((emb_sum_kernel<TG, TW, V>), dim3((unsigned)(a.fill_at + cdiv(a.V, 4 * kFillRows))), dim3(256), 0, st,
+  hipLaunchKernelGGL((emb_sum_kernel<TG, TW, V, AL>), dim3((unsigned)(a.fill_at + cdiv(a.V, 4 * kFillRows))), dim3(256), 0, st,
                      a);
   if (a.pieces > 1)
-    hipLaunchKernelGGL((emb_join_kernel<TW, V>), dim3((unsigned)(a.pieces * a.slabs)), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((emb_join_kernel<TW, V, AL>), dim3((unsigned)(a.pieces * a.slabs)), dim3(512), 0, st, a);
 }
 template <class TG, class TW>
-static void emb_bwd(EmbArgs& a, int columns, hipStream_t st) {
+static void emb_bwd(EmbArgs& a, EmbColumns columns, hipStream_t st) {
   constexpr int V = EmbVec<TG, TW>::V;
-  if (columns == V) emb_sums<TG, TW, V>(a, st);
-  else emb_sums<TG, TW, 1>(a, st);
+  if (columns.n == 1) emb_sums<TG, TW, 1, true>(a, st);
+  else if (columns.aligned) emb_sums<TG, TW, V, true>(a, st);
+  else emb_sums<TG, TW, V, false>(a, st);
 }
 
 // f<A, B>() for two of the three types
@@ -514,7 +536,7 @@ extern "C" int concord_embedding_fwd(const void* tokens, int index64, int64_t n,
   EmbArgs a{};
   a.tokens = tokens, a.idx64 = index64, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
   a.src = table, a.lds = ld_t, a.dst = out, a.ldd = ld_o;
-  const int columns = emb_columns(a, wdtype, dtype);
+  const EmbColumns columns = emb_columns(a, wdtype, dtype);
   emb_types(wdtype, dtype, [&](auto w, auto o) { emb_fwd<decltype(w), decltype(o)>(a, columns, (hipStream_t)stream); });
   return launch_status("embedding_fwd");
 }
@@ -543,8 +565,8 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
   a.tokens = tokens, a.idx64 = index64, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
   a.src = dy, a.lds = ld_dy, a.dst = dtable, a.ldd = ld_dt;
   a.piece = emb_piece(n), a.pieces = cdiv(n, a.piece);
-  const int columns = emb_columns(a, dtype, wdtype);
-  a.slabs = cdiv(C, 64 * columns);
+  const EmbColumns columns = emb_columns(a, dtype, wdtype);
+  a.slabs = cdiv(C, 64 * columns.n);
   CONCORD_CHECK(grid_fits(cdiv(a.pieces * a.slabs, 4) + cdiv(V, 4 * kFillRows), 256) && grid_fits(a.pieces * a.slabs, 512),
                 "concord_embedding_bwd: too many tokens or rows");
   uint32_t *keys[2] = {}, *pos[2] = {};

@@ -810,3 +810,59 @@ def test_example_runs(rotary, keep8):
     own = [p for p in m.parameters() if id(p) not in layers]
     assert len(own) > 5 and all(p.grad is not None and torch.isfinite(p.grad).all() and p.grad.any() for p in own)
     assert all(math.isfinite(v) for v in ex.train(2, tokens=600, device=DEV, rotary=rotary, keep8=keep8))
+
+
+# ---- offsets past 32 bits ------------------------------------------------------------------
+def test_embedding_offsets_past_32_bits():
+    """2^31 elements and more of the result, of its gradient and of the table."""
+    import concord_amd as ca
+    n, width, vocab = 33000, 65600, 33001
+    w = torch.zeros(vocab, width, device=DEV, dtype=BF16)
+    w[-1], w[5] = 3.0, 2.0
+    w.requires_grad_(True)
+    tokens = torch.full((n,), 7, device=DEV)
+    tokens[-1], tokens[-2] = vocab - 1, 5
+    y = ca.embedding(tokens, w)
+    assert (y[-1] == 3).all() and (y[-2] == 2).all() and not y[-3].any()
+    dy = torch.zeros(n, width, device=DEV, dtype=BF16)
+    dy[-1], dy[-2], dy[0] = 0.5, 0.25, 1.0
+    dw, = torch.autograd.grad(y, (w,), dy)
+    assert (dw[-1] == 0.5).all() and (dw[5] == 0.25).all() and (dw[7] == 1).all() and not dw[-2].any() and not dw[0].any()
+
+
+def test_qk_offsets_past_32_bits():
+    import concord_amd as ca
+    n, heads, dim = 131100, 128, 128
+    q = torch.ones(n, heads, dim, device=DEV, dtype=BF16)
+    g = _gen("large qk")
+    last = torch.randn(3, heads, dim, generator=g, device=DEV).to(BF16)
+    q[-3:] = last
+    q.requires_grad_(True)
+    k = torch.ones(n, 1, dim, device=DEV, dtype=BF16)
+    pos = torch.arange(n, device=DEV)
+    y, _ = ca.qk_norm_rope(q, k, positions=pos)
+    dq, = torch.autograd.grad(y, (q,), y.detach().flip(2).contiguous())
+    part = q.detach()[-3:].clone().requires_grad_(True)
+    z, _ = ca.qk_norm_rope(part, k[-3:], positions=pos[-3:])
+    dz, = torch.autograd.grad(z, (part,), z.detach().flip(2).contiguous())
+    # (few tokens and many take lanes of other widths: sums in another order, so a rounding apart)
+    _close(y.detach()[-3:], z.detach().double(), z.detach().double().abs() * 2.0 ** -8 + 24 * U, BF16)
+    _close(dq[-3:], dz.double(), dz.double().abs() * 2.0 ** -8 + 64 * U * 16, BF16)
+
+
+@pytest.mark.parametrize("width", [4096, 4099])
+def test_act8_offsets_past_32_bits(width):
+    import concord_amd as ca
+    rows = 2 ** 31 // 4096 + 10
+    x = torch.zeros(rows, width, device=DEV, dtype=BF16)
+    g = _gen("large act", width)
+    x[-2:] = torch.randn(2, width, generator=g, device=DEV).to(BF16)
+    x.requires_grad_(True)
+    y = ca.gelu8(x)
+    dx, = torch.autograd.grad(y, (x,), torch.ones_like(y))
+    small = x.detach()[-2:].clone().requires_grad_(True)
+    z = ca.gelu8(small)
+    dz, = torch.autograd.grad(z, (small,), torch.ones_like(z))
+    assert torch.equal(y[-2:], z) and torch.equal(dx[-2:], dz) and not y[-3].any() and (dx[-3] == 0.5).all()
+    codes, exps = ca.pack8(x.detach())
+    assert torch.equal(ca.unpack8(codes, exps, BF16)[-2:].double(), _kept(small.detach())[2])
