@@ -13,8 +13,8 @@
 // with the same wide accesses at the alignment of one element, which this GPU
 // takes; what is left at a row's end goes one by one.
 //
-// Kernel times, bf16: gelu of 16384 x 1536 23 us forward and 26 backward (127 MB each, 5.4
-// and 4.8 TB/s; a 1 GiB copy moves 5.1), the gated form of 8192 x 2560 29 and 29 to 35
+// Kernel times, bf16: gelu of 16384 x 1536 23 us forward and 25 backward (127 MB each, 5.4
+// and 5.1 TB/s; a 1 GiB copy moves 5.1), the gated form of 8192 x 2560 27 and 29
 // (169 MB), pack and unpack of 2048 x 5120 6.3 and 5.8 (31 MB, latencies included).  Odd
 // rows, 4099 x 2051 fp16: 12.1 and 13.5 (3.3 TB/s).  Results go past the caches: the gated
 // backward 37 -> 30 us, unpacking 6.6 -> 5.2.
@@ -67,10 +67,15 @@ struct Values {
   typedef Run<T, V, ALIGNED> All;
   All r;
   CONCORD_DEV void load(const T* p, int n) {
+    if constexpr (ALIGNED) {   // (all of them or none: p is readable either way)
+      r = *(const All*)p;
+      if (n < V) r = All{};
+      return;
+    }
     r = All{};
     if (n >= V) {
       r = *(const All*)p;
-    } else if (!ALIGNED) {
+    } else {
 #pragma unroll
       for (int i = 0; i < V - 1; ++i)
         if (i < n) r.v[i] = p[i];
@@ -119,10 +124,14 @@ struct Codes {
     uint32_t w[V / 4];
   } c;
   CONCORD_DEV void load(const uint8_t* p, int n) {
+    if constexpr (ALIGNED) {
+      c = __builtin_bit_cast(Words, *(const All*)p);
+      return;
+    }
     c = {};
     if (n >= V) {
       c = __builtin_bit_cast(Words, *(const All*)p);
-    } else if (!ALIGNED) {
+    } else {
 #pragma unroll
       for (int i = 0; i < V - 1; ++i)
         if (i < n) c.w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
@@ -139,9 +148,11 @@ struct Codes {
   }
 };
 
-// a thread's place: V columns from c of a row
+// A thread's place: V columns from c of a row.  It loads from `at`, which is c or, behind the
+// row's end, the row's beginning: no load of aligned rows waits behind a branch, which the
+// compiler would not move it over.
 struct Place {
-  int64_t row, c;
+  int64_t row, c, at;
   int n;            // columns that the row still has, V for more (0 or less: none)
   uint32_t block;
 };
@@ -153,6 +164,7 @@ CONCORD_DEV Place place(const Act8Args& a, uint32_t id) {
   p.row = row;
   p.c = (int64_t)in * V;
   p.n = (int)min(a.C - p.c, (int64_t)V);
+  p.at = p.n > 0 ? p.c : 0;
   p.block = in / EACH;
   return p;
 }
@@ -201,7 +213,7 @@ template <class T, bool ALIGNED>
 __global__ __launch_bounds__(256) void pack8_kernel(Act8Args a, uint32_t count) {
   constexpr int V = kWide<T>, K = places(false, ALIGNED);
   Values<T, ALIGNED> x[K];
-  each_place<K, V>(a, count, [&](int k, const Place& p) { x[k].load((const T*)a.x + p.row * a.ldx + p.c, p.n); });
+  each_place<K, V>(a, count, [&](int k, const Place& p) { x[k].load((const T*)a.x + p.row * a.ldx + p.at, p.n); });
   each_place<K, V>(a, count, [&](int k, const Place& p) {
     float v[V];
     x[k].get(v);
@@ -215,7 +227,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(Act8Args a, uint32_t count
   Codes<T, ALIGNED> c[K];
   uint32_t e8[K];
   each_place<K, V>(a, count, [&](int k, const Place& p) {
-    c[k].load(a.codes + p.row * a.C + p.c, p.n);
+    c[k].load(a.codes + p.row * a.C + p.at, p.n);
     e8[k] = a.exps[p.row * a.nb + p.block];
   });
   each_place<K, V>(a, count, [&](int k, const Place& p) {
@@ -231,7 +243,7 @@ __global__ __launch_bounds__(256) void gelu8_fwd_kernel(Act8Args a, uint32_t cou
   constexpr int V = kWide<T>, K = places(GATED, ALIGNED);
   Values<T, ALIGNED> x[K], g[K];
   each_place<K, V>(a, count, [&](int k, const Place& p) {
-    const T* at = (const T*)a.x + p.row * a.ldx + p.c;
+    const T* at = (const T*)a.x + p.row * a.ldx + p.at;
     x[k].load(at, p.n);
     if (GATED) g[k].load(at + a.C, p.n);
   });
@@ -259,8 +271,8 @@ __global__ __launch_bounds__(256) void gelu8_bwd_kernel(Act8Args a, uint32_t cou
   uint32_t e8[K], eg[K];
   each_place<K, V>(a, count, [&](int k, const Place& p) {
     const int wide = GATED ? 2 : 1;
-    const uint8_t *codes = a.codes + p.row * wide * a.C + p.c, *exps = a.exps + p.row * wide * a.nb + p.block;
-    r[k].load((const T*)a.dy + p.row * a.lddy + p.c, p.n);
+    const uint8_t *codes = a.codes + p.row * wide * a.C + p.at, *exps = a.exps + p.row * wide * a.nb + p.block;
+    r[k].load((const T*)a.dy + p.row * a.lddy + p.at, p.n);
     c[k].load(codes, p.n);
     e8[k] = exps[0];
     if (GATED) {

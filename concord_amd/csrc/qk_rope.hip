@@ -16,10 +16,8 @@
 // cosine, which are 32-bit polynomials.
 //
 // Kernel times, 32768 tokens of 40 heads of 128, bf16: forward 120 to 125 us (5.5 TB/s),
-// backward 200 to 228 from run to run (5.0 to 4.4), where a 1 GiB copy moves 5.1 TB/s;
-// 64 tokens 4.3 us, a chain of a position's load, an exponential and the row.  The stores go
-// past the caches: 16384 x 9 heads of 64 10.5 -> 8.3 and 14.0 -> 11.7 us, the largest
-// forward 133 -> 124, its backward 215 -> 228.
+// backward 213 us (4.7 TB/s), where a 1 GiB copy moves 5.1 TB/s; 64 tokens 4.3 us, a
+// chain of a position's load, an exponential and the row.
 #include "elem.h"
 
 namespace concord {
@@ -111,12 +109,17 @@ struct QkRow {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = s.in ? to_f32(a.v[j]) : 0.0f, v[V + j] = s.in ? to_f32(b.v[j]) : 0.0f;
   }
+  template <bool PAST>
   CONCORD_DEV void store(T* p, const QkLane& s, const float (&v)[2 * V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) a.v[j] = from_f32<T>(v[j]), b.v[j] = from_f32<T>(v[V + j]);
-    if (s.in) {
+    if (!s.in) return;
+    if constexpr (PAST) {
       store_stream((C*)(p + s.a), a);
       store_stream((C*)(p + s.b), b);
+    } else {
+      *(C*)(p + s.a) = a;
+      *(C*)(p + s.b) = b;
     }
   }
 };
@@ -135,7 +138,7 @@ CONCORD_DEV void turn(float (&v)[2 * V], const float (&c)[V], const float (&s)[V
 
 // Blocks of a slice of the heads (q's slices, then k's) share the tokens: a group of L
 // lanes takes a token's heads of the slice, U at a time.
-template <class T, int V, int L, bool ADJ, bool BWD>
+template <class T, int V, int L, bool ADJ, bool BWD, bool PAST>
 __global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
   constexpr int G = 256 / L, U = BWD ? 2 : 4, E = 2 * V;
   __shared__ float sums[BWD ? G : 1][BWD ? L * E : 1];
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = r * __builtin_fmaf(-v[j], along, d[j]);
       }
-      x[b][u].store(out + (int64_t)u * a.D, s, v);
+      x[b][u].template store<PAST>(out + (int64_t)u * a.D, s, v);
     }
   };
   uint32_t t = (bid - slice * nb) * G + g;
@@ -296,6 +299,7 @@ struct QkPlan {
   int heads[2];        // a slice's
   int parts[2];        // slices of q and of k
   uint32_t blocks[2];  // of a slice
+  bool past;           // results past the caches
 };
 static QkPlan qk_plan(const concord_qk_args& g, bool bwd) {
   QkPlan p{};
@@ -322,6 +326,9 @@ static QkPlan qk_plan(const concord_qk_args& g, bool bwd) {
   // with four a CU, 134 with a block for each group's token).  Few: no block takes two.
   const int64_t total = cdiv(g.T, groups), all = g.H + g.HK;
   const bool few = total * (p.parts[0] + p.parts[1]) <= 2048;
+  // (16384 x 9 heads of 64 10.5 -> 8.3 us forward, 14.0 -> 11.7 backward; 32768 x 40 of 128
+  // 133 -> 124 forward, but 215 -> 228 backward, whose many blocks store as they read)
+  p.past = few || !bwd;
   for (int i = 0; i < 2; ++i) {
     const int64_t want = few ? total : std::max<int64_t>(1, 480 * p.heads[i] / all);
     // (an eighth over its share rather than a round of its own for the last few)
@@ -331,39 +338,40 @@ static QkPlan qk_plan(const concord_qk_args& g, bool bwd) {
   return p;
 }
 
-template <class T, int V, int L>
-static void qk_launch(const QkArgs& a, uint32_t blocks, bool bwd, hipStream_t st) {
+template <class T, int V, int L, bool ADJ>
+static void qk_pass(const QkArgs& a, uint32_t blocks, bool bwd, bool past, hipStream_t st) {
   const dim3 grid(blocks);
+  if (!bwd) hipLaunchKernelGGL((qk_kernel<T, V, L, ADJ, false, true>), grid, dim3(256), 0, st, a);
+  else if (past) hipLaunchKernelGGL((qk_kernel<T, V, L, ADJ, true, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((qk_kernel<T, V, L, ADJ, true, false>), grid, dim3(256), 0, st, a);
+}
+template <class T, int V, int L>
+static void qk_launch(const QkArgs& a, uint32_t blocks, bool bwd, bool past, hipStream_t st) {
   if constexpr (V == 4) {
-    if (a.adjacent) {
-      if (bwd) hipLaunchKernelGGL((qk_kernel<T, V, L, true, true>), grid, dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((qk_kernel<T, V, L, true, false>), grid, dim3(256), 0, st, a);
-      return;
-    }
+    if (a.adjacent) return qk_pass<T, V, L, true>(a, blocks, bwd, past, st);
   }
-  if (bwd) hipLaunchKernelGGL((qk_kernel<T, V, L, false, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((qk_kernel<T, V, L, false, false>), grid, dim3(256), 0, st, a);
+  qk_pass<T, V, L, false>(a, blocks, bwd, past, st);
 }
 template <class T>
 static void qk_lanes(const QkArgs& a, const QkPlan& p, uint32_t blocks, bool bwd, hipStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (p.v == 8) {
       switch (p.lanes) {
-        case 1: return qk_launch<T, 8, 1>(a, blocks, bwd, st);
-        case 2: return qk_launch<T, 8, 2>(a, blocks, bwd, st);
-        case 4: return qk_launch<T, 8, 4>(a, blocks, bwd, st);
-        case 8: return qk_launch<T, 8, 8>(a, blocks, bwd, st);
-        default: return qk_launch<T, 8, 16>(a, blocks, bwd, st);
+        case 1: return qk_launch<T, 8, 1>(a, blocks, bwd, p.past, st);
+        case 2: return qk_launch<T, 8, 2>(a, blocks, bwd, p.past, st);
+        case 4: return qk_launch<T, 8, 4>(a, blocks, bwd, p.past, st);
+        case 8: return qk_launch<T, 8, 8>(a, blocks, bwd, p.past, st);
+        default: return qk_launch<T, 8, 16>(a, blocks, bwd, p.past, st);
       }
     }
   }
   switch (p.lanes) {
-    case 1: return qk_launch<T, 4, 1>(a, blocks, bwd, st);
-    case 2: return qk_launch<T, 4, 2>(a, blocks, bwd, st);
-    case 4: return qk_launch<T, 4, 4>(a, blocks, bwd, st);
-    case 8: return qk_launch<T, 4, 8>(a, blocks, bwd, st);
-    case 16: return qk_launch<T, 4, 16>(a, blocks, bwd, st);
-    default: return qk_launch<T, 4, 32>(a, blocks, bwd, st);
+    case 1: return qk_launch<T, 4, 1>(a, blocks, bwd, p.past, st);
+    case 2: return qk_launch<T, 4, 2>(a, blocks, bwd, p.past, st);
+    case 4: return qk_launch<T, 4, 4>(a, blocks, bwd, p.past, st);
+    case 8: return qk_launch<T, 4, 8>(a, blocks, bwd, p.past, st);
+    case 16: return qk_launch<T, 4, 16>(a, blocks, bwd, p.past, st);
+    default: return qk_launch<T, 4, 32>(a, blocks, bwd, p.past, st);
   }
 }
 static uint32_t qk_rows(const QkPlan& p, int i) { return p.blocks[i] * (uint32_t)p.parts[i]; }

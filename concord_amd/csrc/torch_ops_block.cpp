@@ -257,6 +257,7 @@ int8_t* codes_of(const Tensor& t) { return (int8_t*)ptr(t); }
 uint8_t* exponents_of(const Tensor& t) { return (uint8_t*)ptr(t); }
 
 std::vector<Tensor> pack8(const Tensor& x) {
+  no_tangent("pack8", {&x});
   act8_check(x, "pack8", false);
   const c10::OptionalDeviceGuard guard(x.device());
   const int64_t width = x.size(-1), rows = x.numel() / width;

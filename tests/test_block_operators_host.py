@@ -299,6 +299,6 @@ def test_tangents_are_errors(stub):
         d = [fwd.make_dual(t, torch.ones_like(t)) for t in (w, q, x)]
         for call in (lambda: stub.embedding(torch.arange(12), d[0], 1.0, None),
                      lambda: stub.qk_norm_rope(q, d[1], None, None, None, 1e4, None, False, 1e-6),
-                     lambda: stub.gelu8(d[2], "none"), lambda: stub.geglu8(d[2], "none")):
+                     lambda: stub.gelu8(d[2], "none"), lambda: stub.geglu8(d[2], "none"), lambda: stub.pack8(d[2])):
             with pytest.raises(RuntimeError, match="forward mode"):
                 call()
