@@ -530,6 +530,7 @@ extern "C" int concord_embedding_fwd(const void* tokens, int index64, int64_t n,
                                      void* stream) {
   CONCORD_CHECK(emb_sizes_ok(n, V, C), "concord_embedding_fwd: bad size");
   CONCORD_CHECK(emb_dtype_ok(dtype) && emb_dtype_ok(wdtype), "concord_embedding_fwd: bad type");
+  CONCORD_CHECK(__builtin_isfinite(scale), "concord_embedding_fwd: the scale must be finite");
   CONCORD_CHECK(ld_t >= C && ld_o >= C, "concord_embedding_fwd: leading dimension < C");
   if (n == 0) return CONCORD_OK;
   CONCORD_CHECK(tokens && out && (table || V == 0), "concord_embedding_fwd: NULL argument");
@@ -551,6 +552,7 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   CONCORD_CHECK(emb_sizes_ok(n, V, C), "concord_embedding_bwd: bad size");
   CONCORD_CHECK(emb_dtype_ok(dtype) && emb_dtype_ok(wdtype), "concord_embedding_bwd: bad type");
+  CONCORD_CHECK(__builtin_isfinite(scale), "concord_embedding_bwd: the scale must be finite");
   CONCORD_CHECK(ld_dy >= C && ld_dt >= C, "concord_embedding_bwd: leading dimension < C");
   if (V == 0) return CONCORD_OK;
   CONCORD_CHECK(dtable && (n == 0 || (tokens && dy)), "concord_embedding_bwd: NULL argument");

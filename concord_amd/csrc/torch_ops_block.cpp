@@ -35,7 +35,8 @@ void embedding_check(const Tensor& tokens, const Tensor& weight, double scale, a
                    "embedding: dtype must be float32, bfloat16 or float16 (got ", dtype, ")");
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) >= 1, "embedding: weight must be [vocabulary, width] (got ",
                     weight.sizes(), ")");
-  TORCH_CHECK_VALUE(std::isfinite(scale), "embedding: the scale must be finite (got ", scale, ")");
+  // (as the kernels hold it: 0 times an infinite scale would not be the zero of a token outside the table)
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), "embedding: the scale must be finite in 32 bits (got ", scale, ")");
   TORCH_CHECK_VALUE(tokens.device() == weight.device(), "embedding: tokens are on ", tokens.device(), ", weight on ",
                     weight.device());
   need_gpu(weight, kEmbedding, "weight");

@@ -606,7 +606,7 @@ int concord_attention_bwd(const concord_attn_args* args, void* workspace, size_t
 
 /* y[i] = scale table[tokens[i]] for n tokens (int64 where index64, else int32,
  * one after another), table [V, ld_t] of type wdtype, y [n, ld_o] of type dtype.
- * A token outside [0, V) gives a row of zeros. */
+ * A token outside [0, V) gives a row of zeros.  scale: finite. */
 int concord_embedding_fwd(const void* tokens, int index64, int64_t n, const void* table, int64_t ld_t, int wdtype,
                           int64_t V, int64_t C, float scale, void* out, int64_t ld_o, int dtype, void* stream);
 /* dtable[v] = scale sum of dy[i] over the tokens i that name v, all V rows

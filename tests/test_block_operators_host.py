@@ -44,6 +44,21 @@ def test_embedding_refusals():
             ca.embedding(*args, **kw)
 
 
+def test_embedding_scales_past_32_bits_are_refused(L):
+    # the kernels hold the scale in fp32: infinite there, a token outside the table would get NaN for zeros
+    import concord_amd as ca
+    from concord_amd import _lib as C
+    i, w = torch.zeros(3, dtype=torch.int64), torch.zeros(5, 8)
+    for scale in (1e39, -1e300):
+        with pytest.raises(ValueError, match="embedding: the scale"):
+            ca.embedding(i, w, scale=scale)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        ca.embedding(i, w, scale=3e38)
+    for scale in (float("inf"), float("nan")):
+        assert L.concord_embedding_fwd(None, 1, 0, None, 8, C.F32, 5, 8, scale, None, 8, C.F32, None) == C.EINVAL
+        assert L.concord_embedding_bwd(None, 1, 0, None, 8, C.F32, 0, 8, scale, None, 8, C.F32, None, 0, None) == C.EINVAL
+
+
 def test_qk_refusals():
     import concord_amd as ca
 
