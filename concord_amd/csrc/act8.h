@@ -37,21 +37,21 @@ CONCORD_DEV uint32_t codes8(const float* x, float inv) {
 }
 
 template <class T>
-struct Largest;   // the type's largest finite number, and the exponent byte from which 127 steps exceed it
+struct Largest;   // the type's largest finite number, and the exponent byte from which 128 steps exceed it
 template <>
 struct Largest<float> {
   static constexpr float value = 3.4028234663852886e38f;
-  static constexpr uint32_t e8 = 249;
+  static constexpr uint32_t e8 = 248;
 };
 template <>
 struct Largest<BF16> {
   static constexpr float value = 3.3895313892515355e38f;
-  static constexpr uint32_t e8 = 249;
+  static constexpr uint32_t e8 = 248;
 };
 template <>
 struct Largest<_Float16> {
   static constexpr float value = 65504.0f;
-  static constexpr uint32_t e8 = 137;
+  static constexpr uint32_t e8 = 136;
 };
 
 // Four codes as values of T; NaN for a block of byte 255.  u = code + 128 is a byte
@@ -60,11 +60,12 @@ struct Largest<_Float16> {
 // whose step is infinite) the product is formed from the code itself: 0 times infinity is
 // NaN, and what exceeds T is limited.
 template <class T>
-CONCORD_DEV void values8(float* v, uint32_t w, float step, float less, bool large) {
+CONCORD_DEV void values8(float* v, uint32_t w, uint32_t e8) {
+  const float step = step8(e8), less = -128.0f * step;
   const uint32_t u = w ^ 0x80808080u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf((float)((u >> (8 * i)) & 0xFFu), step, less);
-  if (large) {
+  if (e8 >= Largest<T>::e8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float x = (float)(int)__builtin_amdgcn_sbfe(w, 8 * i, 8) * step;

@@ -204,9 +204,8 @@ CONCORD_DEV void keep8(const Values<T, ALIGNED>& x, const float (&v)[kWide<T>], 
 }
 template <class T, bool ALIGNED>
 CONCORD_DEV void kept8(float (&v)[kWide<T>], const Codes<T, ALIGNED>& c, uint32_t e8) {
-  const float step = step8(e8), less = -128.0f * step;
 #pragma unroll
-  for (int i = 0; i < kWide<T> / 4; ++i) values8<T>(v + 4 * i, c.c.w[i], step, less, e8 >= Largest<T>::e8);
+  for (int i = 0; i < kWide<T> / 4; ++i) values8<T>(v + 4 * i, c.c.w[i], e8);
 }
 
 template <class T, bool ALIGNED>
