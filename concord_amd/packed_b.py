@@ -1220,6 +1220,9 @@ class ConcordLinearPackedB(nn.Module):
                 C.ptr(pw), pw.stride(0), C.ptr(self.row_exp), C.ptr(self.col_exp), pw.shape[0],
                 pw.shape[1], self.MANTISSA_BIAS, float(fast_gain), C.ptr(wbuf), wbuf.stride(0),
                 C.stream_of(pw.device)), "materialize_gated")
+        # (inside apply gradients are always off, and needs_input_grad is the inputs'
+        # requires_grad: neither tells whether a backward can come)
+        input_bits = self.input_bits if torch.is_grad_enabled() else 16
         y = FusedConcordLinearPackedB.apply(
             x, self.packed_w, self.row_exp, self.col_exp, self.bias,
             self._lr_buf, self.alpha, self.beta1, self.MANTISSA_BIAS,
@@ -1231,7 +1234,7 @@ class ConcordLinearPackedB(nn.Module):
             wbuf, rmbuf, cmbuf,
             self.v_row, self.v_col, self._sum_v_inv,
             float(self.adafactor_beta2), bool(self.track_adafactor_v),
-            float(self.gf_trust_delta_sq), self._coh_pre, self.drive, self.input_bits)
+            float(self.gf_trust_delta_sq), self._coh_pre, self.drive, input_bits)
         return y.to(in_dtype)
 
     @torch.no_grad()
