@@ -198,16 +198,31 @@ struct QkNormRopeNode : torch::autograd::Function<QkNormRopeNode> {
                     q.device() == gq.device(),
                 "qk_norm_rope: the saved q or k came back as another tensor");
     qk_check(q, k, q_weight, k_weight, positions, s);
-    const Operand oq = operand(q), ok = operand(k), og = operand(gq), oh = operand(gk);
-    concord_qk_args a = qk_args(oq, ok, q_weight, k_weight, positions, s);
-    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dwq, dwk, ws;
-    a.dq_out = ptr(og.t), a.dq_t = og.token, a.dq_h = og.head;
-    a.dk_out = ptr(oh.t), a.dk_t = oh.token, a.dk_h = oh.head;
-    a.dq = ptr(dq), a.dk = ptr(dk);
     // (numbered among the tensors that were given)
+    Tensor dq, dk, dwq, dwk, ws;
     if (q_weight.defined() && ctx->needs_input_grad(2)) dwq = at::empty_like(q_weight);
     if (k_weight.defined() && ctx->needs_input_grad(q_weight.defined() ? 3 : 2)) dwk = at::empty_like(k_weight);
+    // what is frozen has no heads: no row of it is read or written
+    const bool with_q = ctx->needs_input_grad(0) || dwq.defined(), with_k = ctx->needs_input_grad(1) || dwk.defined();
+    if (!with_q && !with_k) return variable_list(9);
+    const Operand oq = with_q ? operand(q) : Operand{q, 0, 0}, ok = with_k ? operand(k) : Operand{k, 0, 0};
+    concord_qk_args a = qk_args(oq, ok, q_weight, k_weight, positions, s);
     a.dq_weight = ptr(dwq), a.dk_weight = ptr(dwk);
+    Operand og, oh;
+    if (with_q) {
+      og = operand(gq);
+      dq = at::empty(q.sizes(), q.options());
+      a.dq_out = ptr(og.t), a.dq_t = og.token, a.dq_h = og.head, a.dq = ptr(dq);
+    } else {
+      a.H = 0, a.q = a.q_weight = nullptr;
+    }
+    if (with_k) {
+      oh = operand(gk);
+      dk = at::empty(k.sizes(), k.options());
+      a.dk_out = ptr(oh.t), a.dk_t = oh.token, a.dk_h = oh.head, a.dk = ptr(dk);
+    } else {
+      a.HK = 0, a.k = a.k_weight = nullptr;
+    }
     size_t need = 0;
     if (dwq.defined() || dwk.defined()) {
       need = concord_qk_norm_rope_workspace_bytes(&a);
