@@ -400,7 +400,7 @@ static int qk_args(const concord_qk_args* args, const char* name, bool bwd, QkAr
   CONCORD_CHECK(qk_sizes_ok(g), "%s: bad size", name);
   for (int t : {g.dtype, g.wtype})
     CONCORD_CHECK(t == CONCORD_F32 || t == CONCORD_BF16 || t == CONCORD_F16, "%s: bad type", name);
-  CONCORD_CHECK(g.base > 0 && g.base < 1e300 && g.eps >= 0, "%s: bad base or eps", name);
+  CONCORD_CHECK(g.base > 0 && g.base < 1e300 && g.eps >= 0 && __builtin_isfinite(g.eps), "%s: bad base or eps", name);
   if (g.T == 0) return CONCORD_OK;
   CONCORD_CHECK(g.seq >= 1 && g.seq <= g.T && (!g.positions || (g.pos_seq >= 1 && g.pos_seq <= g.T)), "%s: bad sequence length",
                 name);

@@ -121,7 +121,10 @@ at::ScalarType qk_check(const Tensor& q, const Tensor& k, const Tensor& q_weight
   TORCH_CHECK_VALUE(s.rotary >= 0 && s.rotary <= d && s.rotary % 8 == 0,
                     "qk_norm_rope: rotary_dim must be a multiple of 8 up to ", d, " (got ", s.rotary, ")");
   TORCH_CHECK_VALUE(s.base > 0 && s.base < 1e300, "qk_norm_rope: the base must be positive (got ", s.base, ")");
-  TORCH_CHECK_VALUE(s.eps >= 0 && std::isfinite(s.eps), "qk_norm_rope: eps must not be negative (got ", s.eps, ")");
+  // (as the kernels hold it: an infinite one would make every row zeros, one that is lost a row of zeros NaN)
+  const float eps = (float)s.eps;
+  TORCH_CHECK_VALUE(s.eps >= 0 && std::isfinite(eps) && (eps > 0 || s.eps == 0),
+                    "qk_norm_rope: eps must be 0 or a positive number of 32 bits (got ", s.eps, ")");
   at::ScalarType wtype = at::kFloat;
   bool given = false;
   for (const Tensor* w : {&q_weight, &k_weight}) {
