@@ -95,6 +95,12 @@ CONCORD_DEV float group_sum(float v) {
   return v;
 }
 
+// A mean square below 2^-96, whose terms 32 bits may have lost, or infinite (or NaN).  Its
+// row is taken times k = 2^48 or 2^-48, and the squares of that times k: they lie in range
+// for every row there is, and every factor stays a normal number.  (The test costs nothing
+// that shows: forward of 32768 x 40 heads of 128 130 us with it and without, backward 213.)
+CONCORD_DEV bool out_of_range(float square) { return __float_as_uint(square) - 0x0F800000u >= 0x7F800000u - 0x0F800000u; }
+
 // a lane's share of a row; a lane behind the row's end holds the row's first elements
 // and stores nothing
 template <class T, int V>
@@ -197,7 +203,19 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
       float q = 0.0f;
 #pragma unroll
       for (int j = 0; j < E; ++j) q = __builtin_fmaf(v[j], v[j], q);
-      const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<L>(q), inv_d, a.eps));
+      const float square = __builtin_fmaf(group_sum<L>(q), inv_d, a.eps);
+      float r = __builtin_amdgcn_rsqf(square), k = 1.0f;   // (1 / sqrt is r k)
+      const bool rescaled = out_of_range(square);
+      if (rescaled) {
+        k = square < 1.0f ? 0x1p48f : 0x1p-48f;
+        q = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          v[j] *= k;
+          q = __builtin_fmaf(v[j] * k, v[j] * k, q);
+        }
+        r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<L>(q), inv_d, a.eps * k * k * k * k)) * k;
+      }
       if constexpr (!BWD) {
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = v[j] * r * w[j];
@@ -217,6 +235,10 @@ __global__ __launch_bounds__(256) void qk_kernel(QkArgs a) {
         along = group_sum<L>(along) * inv_d;
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = r * __builtin_fmaf(-v[j], along, d[j]);
+        if (rescaled) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[j] *= k;
+        }
       }
       x[b][u].template store<PAST>(out + (int64_t)u * a.D, s, v);
     }
