@@ -29,6 +29,11 @@ constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 // one after another
 static int emb_tile(int64_t n) { return n <= 65536 ? 1024 : 4096; }
 constexpr int kOneBlock = 4096;      // pairs that one block sorts alone
+// Up to this many blocks each sums the counts of all of them for itself; past it, where that
+// work would grow with the square of the tokens, a kernel of its own sums them up once a pass
+// (whole backward of tokens of 511, 8 wide, bf16: 2^19 tokens 79 to 90 us without it, 89 to
+// 92 with; 2^20 128 to 138 and 133 to 137; 2^21 224 to 233 and 211; 2^24 3045 and 1450).
+constexpr unsigned kScanBlocks = 256;
 
 struct EmbArgs {
   const void* tokens;
@@ -198,6 +203,7 @@ struct SortPass {
   const uint32_t *keys, *pos;   // NULL in the first pass: the tokens
   uint32_t *out_keys, *out_pos;
   uint32_t* counts;             // [blocks][bins]
+  uint32_t* totals;             // [bins] where the counts are summed up before, else NULL
   int shift, bits;
 };
 template <int IT>
@@ -218,6 +224,40 @@ __global__ __launch_bounds__(512) void emb_count_kernel(EmbArgs a, SortPass s) {
   __syncthreads();
   if ((int)threadIdx.x < bins) s.counts[(int64_t)blockIdx.x * bins + threadIdx.x] = cnt[threadIdx.x];
 }
+// ... the counts' exclusive sums over the blocks, in place, and their totals: a wave a
+// sixteenth of the blocks, its sum first, then the running sums behind those of the waves before it ...
+__global__ __launch_bounds__(1024) void emb_scan_kernel(SortPass s, uint32_t blocks) {
+  constexpr int B = 16;
+  __shared__ uint32_t sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << s.bits;
+  const int bin = blockIdx.x * 64 + lane;
+  const uint32_t per = (blocks + 15) / 16, first = min(wave * per, blocks), last = min(first + per, blocks);
+  uint32_t* c = s.counts + min(bin, bins - 1);
+  uint32_t v[B], sum = 0;
+  auto load = [&](uint32_t b) {
+#pragma unroll
+    for (int i = 0; i < B; ++i) v[i] = b + i < last ? c[(int64_t)(b + i) * bins] : 0;
+  };
+  for (uint32_t b = first; b < last; b += B) {
+    load(b);
+#pragma unroll
+    for (int i = 0; i < B; ++i) sum += v[i];
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  uint32_t at = 0;
+  for (int w = 0; w < wave; ++w) at += sums[w][lane];
+  if (bin >= bins) return;
+  if (wave == 15) s.totals[bin] = at + sum;
+  for (uint32_t b = first; b < last; b += B) {
+    load(b);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (b + i < last) c[(int64_t)(b + i) * bins] = at;
+      at += v[i];
+    }
+  }
+}
 // ... and the pairs to their places: behind all smaller digits, behind the same digit of earlier blocks
 template <int IT>
 __global__ __launch_bounds__(512) void emb_scatter_kernel(EmbArgs a, SortPass s) {
@@ -233,7 +273,12 @@ __global__ __launch_bounds__(512) void emb_scatter_kernel(EmbArgs a, SortPass s)
     p[j] = in && s.pos ? s.pos[i] : (uint32_t)i;
   }
   uint32_t before = 0, all = 0;
-  if ((int)threadIdx.x < bins) {
+  if (s.totals) {
+    if ((int)threadIdx.x < bins) {
+      before = s.counts[(int64_t)blockIdx.x * bins + threadIdx.x];
+      all = s.totals[threadIdx.x];
+    }
+  } else if ((int)threadIdx.x < bins) {
     // sixteen blocks' counts in flight: another XCD wrote them, so each load is a long one
     constexpr int B = 16;
     const uint32_t* c = s.counts + threadIdx.x;
@@ -435,7 +480,7 @@ static size_t emb_size(int t) { return t == CONCORD_F32 ? 4 : 2; }
 static int emb_piece(int64_t n) { return n <= 4096 ? 16 : 64; }
 
 struct EmbWorkspace {
-  size_t keys[2], pos[2], counts, part, bytes;
+  size_t keys[2], pos[2], counts, totals, part, bytes;
 };
 static EmbWorkspace emb_workspace(int64_t n, int64_t C) {
   EmbWorkspace w{};
@@ -450,6 +495,7 @@ static EmbWorkspace emb_workspace(int64_t n, int64_t C) {
     w.pos[i] = take((size_t)n * 4);
   }
   w.counts = take((size_t)cdiv(n, emb_tile(n)) * kMaxBins * 4);
+  w.totals = take(kMaxBins * 4);
   w.part = take((size_t)cdiv(n, emb_piece(n)) * 2 * (size_t)C * 4);
   w.bytes = at;
   return w;
@@ -589,16 +635,19 @@ extern "C" int concord_embedding_bwd(const void* tokens, int index64, int64_t n,
     } else {
       const int tile = emb_tile(n);
       const dim3 grid((unsigned)cdiv(n, tile));
+      const bool scan = grid.x > kScanBlocks;
       for (int p = 0; p < passes; ++p) {
         SortPass s{};
         if (p) s.keys = keys[at ^ 1], s.pos = pos[at ^ 1];
         s.out_keys = keys[at], s.out_pos = pos[at], s.counts = (uint32_t*)(base + w.counts);
+        if (scan) s.totals = (uint32_t*)(base + w.totals);
         s.shift = p * each, s.bits = each;
         if (tile == 1024) {
           hipLaunchKernelGGL((emb_count_kernel<2>), grid, dim3(512), 0, st, a, s);
           hipLaunchKernelGGL((emb_scatter_kernel<2>), grid, dim3(512), 0, st, a, s);
         } else {
           hipLaunchKernelGGL((emb_count_kernel<8>), grid, dim3(512), 0, st, a, s);
+          if (scan) hipLaunchKernelGGL(emb_scan_kernel, dim3((unsigned)cdiv(1 << each, 64)), dim3(1024), 0, st, s, grid.x);
           hipLaunchKernelGGL((emb_scatter_kernel<8>), grid, dim3(512), 0, st, a, s);
         }
         at ^= 1;
