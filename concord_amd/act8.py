@@ -4,8 +4,9 @@ csrc/act8.hip.
 The 8-bit form: 32 adjacent values of the last dimension share a step, the smallest
 power of two of which the largest value is at most 127; each value is stored as the
 nearest whole number of steps (ties to even).  A value is off by at most half a step,
-1/127 of the largest of its 32.  A block that holds an infinity or NaN reads back as
-NaN, all 32 values of it.
+1/127 of the largest of its 32; no step is smaller than 2^-126, so values of a block of
+nothing above 127 2^-127 (fp32 and bf16 have such) are off by up to 2^-127 instead.  A
+block that holds an infinity or NaN reads back as NaN, all 32 values of it.
 """
 import torch
 

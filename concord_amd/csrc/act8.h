@@ -5,8 +5,10 @@
 //   code = x 2^-e rounded half to even, -127 .. 127;   exponent byte = e + 127 (1 .. 249)
 //   value = code 2^e, limited to the type's largest finite number
 // Scaling by a power of two is exact, so the codes have one definition whatever
-// computes them, each value is off by at most half a step (1/127 of the
-// block's largest), and one significant byte fits bf16 and fp16 without a further rounding.
+// computes them, each value is off by at most half a step (less than 1/127 of the
+// block's largest; 2^-127 where the step is held at 2^-126, in fp32 and bf16 blocks of
+// nothing above 127 2^-127), and one significant byte fits bf16 and fp16 without a further
+// rounding.
 // A block that holds an infinity or NaN has exponent byte 255 and codes 0: all of it
 // reads back as NaN.
 #pragma once
@@ -81,8 +83,9 @@ CONCORD_DEV void values8(float* v, uint32_t w, uint32_t e8) {
 // digits far out, where 1 + erf would have lost every one, and
 //   x Phi(x) = max(x, 0) - a tail,   Phi(x) = tail or 1 - tail.
 // Past a = 16 both are at their limits, and a stands at 16.
-//   FINE (fp32): degree 8, relative error 3.2e-8, and the exponent's rounding taken
-// back with its remainder: 4e-7 of the tail in all.
+//   FINE (fp32): degree 8, relative error 5.2e-8 with its coefficients as they stand (at
+// a = 0, where it is largest), and the exponent's rounding taken back with its remainder:
+// 4e-7 of the tail in all.
 //   else (bf16, fp16): degree 5, 8.8e-6, a 28th of half a step of fp16, and the
 // exponent's rounding (at most a^2 2^-24 of the tail) stays.  The kernels are bound by their
 // instructions as much as by memory.

@@ -1025,7 +1025,7 @@ class ConcordLinearPackedB(nn.Module):
         default) or 8 (act8.pack8: 33 bytes for 32 values).  The forward and the
         input's gradient are the same; the weight gradient is formed from what the
         8-bit form stands for, each value off by at most 1/127 of the largest
-        of its 32."""
+        of its 32 (or 2^-127, see act8).  Without gradients nothing is packed."""
         if bits not in (8, 16):
             raise ValueError(f"input bits must be 8 or 16 (got {bits!r})")
         self.input_bits = bits

@@ -14,7 +14,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, base=10000.
     q [batch, token, head, dim] and k [batch, token, key head, dim], or both without
     the batch (documents packed one after another), as attention takes them; one of
     float32, bfloat16, float16, in any strides; dim a multiple of 8 up to 256.
-    q_weight, k_weight [dim]: a type of their own (either may be None: ones).
+    q_weight, k_weight [dim]: a type of their own.  None is a weight of ones: the rows
+    are divided by their root mean square all the same.
 
     positions: int64 or int32, [batch, token] or [token] for all of the batch; each
     token's place in its sequence unless given.  Pair i of the first rotary_dim
