@@ -16,8 +16,10 @@
 // Kernel times, bf16: gelu of 16384 x 1536 23 us forward and 25 backward (127 MB each, 5.4
 // and 5.1 TB/s; a 1 GiB copy moves 5.1), the gated form of 8192 x 2560 27 and 29
 // (169 MB), pack and unpack of 2048 x 5120 6.3 and 5.8 (31 MB, latencies included).  Odd
-// rows, 4099 x 2051 fp16: 12.1 and 13.5 (3.3 TB/s).  Results go past the caches: the gated
-// backward 37 -> 30 us, unpacking 6.6 -> 5.2.
+// rows, 4099 x 2051 fp16: 12.1 and 13.5 (3.3 TB/s).  fp32, the same sizes: 34 and 38 (227
+// MB), gated 48 and 46 (295 MB), odd rows 17.6 and 18 (76 MB, 4.3 TB/s), the tanh form as
+// fast: bound by memory, the longer polynomial does not show.  Results go past the caches:
+// the gated backward 37 -> 30 us, unpacking 6.6 -> 5.2.
 #include "act8.h"
 
 namespace concord {

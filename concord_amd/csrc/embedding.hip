@@ -16,10 +16,10 @@
 // adds those in order.  No sum depends on the order in which waves run: there are
 // no atomics on floating point numbers.
 //
-// Kernel times, 32768 tokens of 50257, 4096 wide, bf16: forward 77 us (268 MB written and
+// Kernel times, 32768 tokens of 50257, 4096 wide, bf16: forward 75 us (268 MB written and
 // as much read, a third of it from memory), sort 21 us in four launches, sums and zeros
-// 135 us (680 MB, 5.0 TB/s), join 12 us.  16384 tokens of 65, 384 wide, fp32: 7.6, 7.3, 7.9
-// and 4.5 us, near the cost of the launches and their latencies.
+// 136 us (680 MB, 5.0 TB/s), join 12 us.  16384 tokens of 65, 384 wide, fp32: 7.8, 7.8, 7.9
+// and 5.1 us, near the cost of the launches and their latencies.
 #include "elem.h"
 
 namespace concord {

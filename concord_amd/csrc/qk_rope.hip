@@ -15,9 +15,10 @@
 // loses its fraction in 32) and reduced to an eighth of a turn before the sine and
 // cosine, which are 32-bit polynomials.
 //
-// Kernel times, 32768 tokens of 40 heads of 128, bf16: forward 120 to 125 us (5.5 TB/s),
-// backward 213 us (4.7 TB/s), where a 1 GiB copy moves 5.1 TB/s; 64 tokens 4.3 us, a
-// chain of a position's load, an exponential and the row.
+// Kernel times, 32768 tokens of 40 heads of 128, bf16: forward 116 to 130 us (5.8 to 5.2
+// TB/s), backward 196 to 213 us (5.1 to 4.7; the longer ones with positions given), where a
+// 1 GiB copy moves 5.1 TB/s; fp32 252 and 378 us (5.3); 64 tokens 4.3 us, a chain of a
+// position's load, an exponential and the row.
 #include "elem.h"
 
 namespace concord {
@@ -328,9 +329,11 @@ static QkPlan qk_plan(const concord_qk_args& g, bool bwd) {
   QkPlan p{};
   // 16 bytes a load where both halves of the turned and of the other elements are whole
   // chunks of them (adjacent pairs take 16 bytes in two neighbouring loads); the forward of
-  // wider rows keeps to 8, whose smaller state leaves more waves (32768 x 40 heads of 128:
-  // forward 140 us by 16 bytes, 122 by 8, backward 200 and 222; 16384 x 9 heads of 64: 8.4
-  // and 10.8, 12.9 and 14.1)
+  // wider rows keeps to 8, whose smaller state leaves more waves (bf16, 32768 x 40 heads,
+  // us by 16 bytes and by 8: of 64 forward 64 and 70, backward 94 and 145; of 80 130 and 106,
+  // 165 and 244; of 96 126 and 105, 161 and 252; of 112 177 and 115, 185 and 260; of 128 145
+  // and 116, 196 and 260.  16384 x 9 heads: of 64 8.1 and 10.1, 11.5 and 13.0; of 80 to 128
+  // the two are within a tenth but for the forward of 96, 13.2 and 15.1, and 112, 19.5 and 15.6)
   p.v = g.dtype != CONCORD_F32 && !g.adjacent && g.R % 16 == 0 && g.D % 16 == 0 && (bwd || g.D <= 64) ? 8 : 4;
   p.lanes = 1;
   while (p.lanes * 2 * p.v < g.D) p.lanes *= 2;
