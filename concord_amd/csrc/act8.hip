@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256) void gelu8_bwd_kernel(Act8Args a, uint32_t cou
       for (int i = 0; i < V; ++i) {
         float v, d;
         F::both(g[i], v, d);
-        g[i] = dy[i] * z[i] * d;
+        g[i] = dy[i] * d * z[i];   // (|d| < 1.13: only the whole product can overflow)
         z[i] = dy[i] * v;
       }
       r[k].store(out, p.n, z);

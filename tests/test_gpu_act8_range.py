@@ -77,3 +77,20 @@ def test_gradients_of_large_blocks(dtype, aligned):
     v, dv, rel, bound = _gelu64(kb, False, dtype)
     _close(dg[:, :w], d * v, (d * v).abs() * (rel + U) + d * 2.0 ** -120, dtype, "da")
     _close(dg[:, w:], d * ka * dv, (d * ka).abs() * (bound + 2 * U * dv.abs() + 2.0 ** -120), dtype, "dg")
+
+
+@pytest.mark.parametrize("tanh", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gated_gradient_of_a_large_half(dtype, tanh):
+    """dy times the large half passes 32 bits, the whole product with a small derivative does not."""
+    import concord_amd as ca
+    a = torch.full((4, 64), 2.0 ** 127, device=DEV)
+    g = torch.empty(4, 64, device=DEV)
+    g[0], g[1], g[2], g[3] = -30.0, -9.0, -6.0, -20.0
+    x = torch.cat((a, g), 1).to(dtype).requires_grad_(True)
+    dy = torch.full((4, 64), 8.0, device=DEV, dtype=dtype)
+    dx, = torch.autograd.grad(ca.geglu8(x, approximate="tanh" if tanh else "none"), (x,), dy)
+    d = dy.double()
+    ka, kb = (_kept(t)[2] for t in x.detach().chunk(2, -1))
+    _, dv, _, bound = _gelu64(kb, tanh, dtype)
+    _close(dx[:, 64:], d * ka * dv, (d * ka).abs() * (bound + 2 * U * dv.abs() + 2.0 ** -120), dtype, "dg")
