@@ -628,7 +628,8 @@ int concord_embedding_bwd(const void* tokens, int index64, int64_t n, const void
  * elements, multiples of 8; 16-byte aligned), likewise the others; results are
  * [T][H][D] and [T][HK][D] without gaps, 16-byte aligned.  Weights [D] of type
  * wdtype, NULL: ones.  Token t has position positions[t % pos_seq] (int64 where
- * pos64, else int32), or t % seq where positions is NULL. */
+ * pos64, else int32), or t % seq where positions is NULL.  H or HK may be 0: that
+ * one is left out.  base: positive, below 1e300; eps: finite, not negative. */
 typedef struct concord_qk_args {
   const void *q, *k;
   int64_t q_t, q_h, k_t, k_h;
